@@ -9,7 +9,7 @@ import ctypes as C
 
 import numpy as np
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 MAX_BATCH = 64
 COMM_ID_BYTES = 128
 # hidden-layer activations the kernels implement (ids = DIMN_ACT_* of include/dimn.h; Keras names)
@@ -43,12 +43,20 @@ class Layer(C.Structure):
     _fields_ = [("neurons", C.c_int32), ("activation", C.c_int32), ("dropout_rate", C.c_float)]
 
 
+class OutputLoss(C.Structure):
+    """struct dimn_output_loss (include/dimn.h): a linear output layer and its targets, device pointers as integers."""
+    _fields_ = [("device_id", C.c_int32), ("type", C.c_int32), ("rows", C.c_int64), ("width", C.c_int64), ("classes", C.c_int64),
+                ("x", C.c_void_p), ("x_row", C.c_int64), ("kernel", C.c_void_p), ("kernel_in", C.c_int64), ("kernel_out", C.c_int64),
+                ("bias", C.c_void_p), ("target", C.c_void_p), ("target_row", C.c_int64), ("target_kind", C.c_int32)]
+
+
 PRECISIONS = {"fp32": 0, "f32": 0, "float32": 0, "bf16": 1, "bfloat16": 1}
 LOSSES = {"wmse": 0, "wmse_binary": 1, "mean_squared_error": 2, "mse": 2, "mean_absolute_error": 3, "mae": 3,
           # round 5: the other element-wise keras.losses names (and their Keras aliases)
           "mean_squared_logarithmic_error": 4, "msle": 4, "logcosh": 5, "log_cosh": 5, "huber": 6, "huber_loss": 6, "poisson": 7}
 
 _H = C.c_void_p
+_P = C.c_void_p
 _i32 = C.c_int32
 _i64 = C.c_int64
 _pf = C.POINTER(C.c_float)
@@ -130,6 +138,13 @@ GPU_ONLY = {
     "col_stats_var": [_pd, _i64, _i64, _i64, _pd, _pd, _i32],
     "col_stats": [_pd, _i64, _i64, _i64, _pd, _pd, _pd, _pi, _i32],
     "select_predictors": [_i32, _pd, _i64, _i64, _pi, _i32, _i32, _pi, _i32, _pi],
+    # row operators on device arrays (device pointers and streams as integers)
+    "layer_norm": [_i32, _P, _i32, _i64, _i64, _i64, _P, _i64, _i64, _P, _P, C.c_float, _P, _i64, _i64, _P, _P],
+    "layer_norm_grad_workspace": [_i32, _i32, _i64, _i64, _i64, C.POINTER(_i64)],
+    "layer_norm_grad": [_i32, _P, _i32, _i64, _i64, _i64, _P, _i64, _i64, _P, _i64, _i64, _P, _P, _P, _P, _i64, _i64, _P, _P, _P, _i64],
+    "linear_cross_entropy_workspace": [C.POINTER(OutputLoss), _i32, C.POINTER(_i64)],
+    "linear_cross_entropy": [C.POINTER(OutputLoss), _P, _P, _P, _P, _i64],
+    "linear_cross_entropy_grad": [C.POINTER(OutputLoss), _P, _P, _P, _P, _i64, _P, _i64, _i64, _P, _P, _i64],
 }
 
 

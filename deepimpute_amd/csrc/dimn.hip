@@ -32,8 +32,9 @@
 #include "dimn_csv.h"
 #include "dimn_hoststats.h"
 #include "dimn_counts_dev.h"
+#include "dimn_rowops.h"
 
-#define DIMN_ABI_VERSION 9
+#define DIMN_ABI_VERSION 10
 
 // DIMN_TRACE=1: stage times of the host-heavy entry points on stderr (diagnostic)
 struct Trace {
@@ -48,6 +49,13 @@ struct Trace {
 };
 static thread_local char g_err[1024];
 static int fail(int code, const char* fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof g_err, fmt, ap);
+    va_end(ap);
+    return code;
+}
+int dimn_fail(int code, const char* fmt, ...) {      // the same for the row operators' translation unit
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof g_err, fmt, ap);

@@ -1,0 +1,477 @@
+// dimn_rowops.hip -- the row operators of libdimn on device arrays of the caller: layer normalisation (dimn_norm.h) and the softmax
+// cross entropy of a linear output layer (dimn_xent.h).
+// No handle: a call names its device and its stream, works on the caller's memory only, and returns when its kernels are queued.
+#include "dimn_rowops.h"
+
+#include <algorithm>
+#include <atomic>
+
+#include "dimn_norm.h"
+#include "dimn_xent.h"
+
+#define HIPCHK(expr)                                                                            \
+    do {                                                                                        \
+        hipError_t e_ = (expr);                                                                 \
+        if (e_ != hipSuccess)                                                                   \
+            return dimn_fail(DIMN_ERR_HIP, "%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
+    } while (0)
+#define CHK(expr)              \
+    do {                       \
+        int rc_ = (expr);      \
+        if (rc_) return rc_;   \
+    } while (0)
+
+namespace {
+
+int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// the caller's current device comes back when the call ends
+struct OnDevice {
+    int before = -1, now = -1;
+    int enter(const char* who, int32_t device) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return dimn_fail(DIMN_ERR_HIP, "%s: no HIP device visible", who);
+        if (device < 0 || device >= n) return dimn_fail(DIMN_ERR_ARG, "%s: device_id %d out of range (%d devices)", who, device, n);
+        HIPCHK(hipGetDevice(&before));
+        now = device;
+        if (before != now) HIPCHK(hipSetDevice(now));
+        return DIMN_OK;
+    }
+    ~OnDevice() { if (now >= 0 && before != now) (void)hipSetDevice(before); }
+};
+
+// compute units of the current device (256 on MI355X), asked once per device
+int compute_units() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+// ---- layer normalisation: which kernel a width takes -----------------------------------------------------------------------
+// `tpr` threads hold a row in `e` pieces of `v` elements (16 bytes; 1 for rows shorter than that); tpr = 0: the row does not fit the registers
+// (k_norm_long).  As few threads per row as the registers allow: sums then need fewer steps and more rows are in flight.  The limits keep a thread
+// below 256 registers, 128 at 1024 threads (backward holds gamma, two gradient sums, two row values and the next row's pieces per element).
+struct NormForm { int tpr, e, v; };
+NormForm norm_form(int32_t type, bool grad, int32_t width) {
+    const bool bf = type == DIMN_TYPE_BF16;
+    const int v = bf ? 8 : 4;
+    if (width < v) return {16, 1, 1};
+    const int nv = (int)ceil_div64(width, v);
+    const int most = bf ? (grad ? 3 : 5) : 6, most1k = bf ? 2 : 4;
+    if (nv <= 32) return {16, (int)ceil_div64(nv, 16), v};
+    for (int tpr : {64, 256})
+        if (nv <= tpr * most) return {tpr, (int)ceil_div64(nv, tpr), v};
+    if (nv <= 1024 * most1k) return {1024, (int)ceil_div64(nv, 1024), v};
+    return {0, 0, v};
+}
+
+// workgroups per group: enough to fill the device, every one with the same number of rows (the last one apart)
+int64_t norm_blocks(const NormForm& f, bool grad, int64_t groups, int64_t rows) {
+    if (rows == 0) return 1;
+    const int sets = f.tpr == 0 ? 1 : std::max(1, 256 / f.tpr);
+    const int64_t per_cu = grad ? 2 : 4;
+    const int64_t budget = std::max<int64_t>(1, per_cu * compute_units() / (f.tpr == 1024 || f.tpr == 0 ? 2 : 1) / std::max<int64_t>(1, groups));
+    const int64_t all = ceil_div64(rows, sets);
+    const int64_t each = ceil_div64(all, budget);
+    return std::max<int64_t>(1, ceil_div64(all, each));
+}
+
+template <typename T, bool GRAD, int TPR, int E, int V>
+void norm_launch_one(dim3 grid, hipStream_t st, const NormP& p) {
+    if constexpr (GRAD) hipLaunchKernelGGL((rowops::k_norm_grad<T, TPR, E, V>), grid, dim3(TPR < 256 ? 256 : TPR), 0, st, p);
+    else hipLaunchKernelGGL((rowops::k_norm<T, TPR, E, V>), grid, dim3(TPR < 256 ? 256 : TPR), 0, st, p);
+}
+template <typename T, bool GRAD>
+void norm_launch(const NormForm& f, dim3 grid, hipStream_t st, const NormP& p) {
+    constexpr bool bf = sizeof(T) == 2;
+    constexpr int V = rowops::kWide<T>;
+    if (f.v == 1) { norm_launch_one<T, GRAD, 16, 1, 1>(grid, st, p); return; }
+    switch (f.tpr * 16 + f.e) {
+#define FORM(TPR, E) case TPR * 16 + E: norm_launch_one<T, GRAD, TPR, E, V>(grid, st, p); return
+        FORM(16, 1); FORM(16, 2);
+        FORM(64, 1); FORM(64, 2); FORM(64, 3);
+        FORM(256, 1); FORM(256, 2); FORM(256, 3);
+        FORM(1024, 1); FORM(1024, 2);
+    }
+    if constexpr (!bf || !GRAD) {
+        switch (f.tpr * 16 + f.e) { FORM(64, 4); FORM(64, 5); FORM(256, 4); FORM(256, 5); }
+    }
+    if constexpr (!bf) {
+        switch (f.tpr * 16 + f.e) { FORM(64, 6); FORM(256, 6); FORM(1024, 3); FORM(1024, 4); }
+    }
+#undef FORM
+    if constexpr (GRAD) hipLaunchKernelGGL((rowops::k_norm_grad_long<T>), grid, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((rowops::k_norm_long<T>), grid, dim3(1024), 0, st, p);
+}
+
+constexpr int64_t kGridY = 65535;
+
+}  // namespace
+
+int64_t norm_workspace_floats(int32_t type, int64_t groups, int64_t rows, int32_t width) {
+    return groups * norm_blocks(norm_form(type, true, width), true, groups, rows) * 2 * (int64_t)width;
+}
+
+// p with its group-th plane first
+static NormP norm_from(const NormP& p, int64_t group, int64_t parts, int size) {
+    NormP q = p;
+    auto move = [&](const void* base, int64_t stride) { return base ? (const char*)base + group * stride * size : nullptr; };
+    q.x = move(p.x, p.x_group);
+    q.dy = move(p.dy, p.dy_group);
+    q.out = const_cast<char*>((const char*)move(p.out, p.out_group));
+    if (p.gate) q.gate = p.gate + group * p.out_group;
+    if (p.gamma) q.gamma = p.gamma + group * p.width;
+    if (p.beta) q.beta = p.beta + group * p.width;
+    if (p.mean) q.mean = p.mean + group * p.rows;
+    if (p.rstd) q.rstd = p.rstd + group * p.rows;
+    if (p.part) q.part = p.part + group * parts * 2 * p.width;
+    return q;
+}
+
+int norm_forward(hipStream_t st, int32_t type, int64_t groups, const NormP& p) {
+    if (groups == 0 || p.rows == 0) return DIMN_OK;
+    const NormForm f = norm_form(type, false, p.width);
+    const int64_t blocks = norm_blocks(f, false, groups, p.rows);
+    for (int64_t g0 = 0; g0 < groups; g0 += kGridY) {
+        const dim3 grid((unsigned)blocks, (unsigned)std::min(kGridY, groups - g0));
+        const NormP q = norm_from(p, g0, 0, type == DIMN_TYPE_BF16 ? 2 : 4);
+        if (type == DIMN_TYPE_BF16) norm_launch<bf16_t, false>(f, grid, st, q);
+        else norm_launch<float, false>(f, grid, st, q);
+    }
+    HIPCHK(hipGetLastError());
+    return DIMN_OK;
+}
+
+int norm_backward(hipStream_t st, int32_t type, int64_t groups, NormP p, float* dgamma, float* dbeta, float* workspace) {
+    if (groups == 0) return DIMN_OK;
+    const NormForm f = norm_form(type, true, p.width);
+    const int64_t blocks = norm_blocks(f, true, groups, p.rows);
+    p.part = dgamma || dbeta ? workspace : nullptr;
+    if (p.rows == 0 && !p.part) return DIMN_OK;
+    for (int64_t g0 = 0; g0 < groups; g0 += kGridY) {
+        const dim3 grid((unsigned)blocks, (unsigned)std::min(kGridY, groups - g0));
+        const NormP q = norm_from(p, g0, blocks, type == DIMN_TYPE_BF16 ? 2 : 4);      // (rows = 0: the kernels write partial rows of zeros)
+        if (type == DIMN_TYPE_BF16) norm_launch<bf16_t, true>(f, grid, st, q);
+        else norm_launch<float, true>(f, grid, st, q);
+        if (p.part)
+            hipLaunchKernelGGL(rowops::k_norm_param_grad, dim3((unsigned)ceil_div64(2 * (int64_t)p.width, 64), grid.y), dim3(1024), 0, st, q.part, (int)blocks, p.width,
+                               dgamma ? dgamma + g0 * p.width : nullptr, dbeta ? dbeta + g0 * p.width : nullptr);
+    }
+    HIPCHK(hipGetLastError());
+    return DIMN_OK;
+}
+
+static int norm_check(const char* who, int32_t type, int64_t groups, int64_t rows, int64_t width) {
+    if (type != DIMN_TYPE_F32 && type != DIMN_TYPE_BF16) return dimn_fail(DIMN_ERR_UNSUP, "%s: element type %d (DIMN_TYPE_F32 or DIMN_TYPE_BF16)", who, type);
+    if (groups < 0 || rows < 0 || groups > INT32_MAX || rows > INT32_MAX) return dimn_fail(DIMN_ERR_ARG, "%s: %lld groups of %lld rows", who, (long long)groups, (long long)rows);
+    if (width < 1 || width > (1 << 28)) return dimn_fail(DIMN_ERR_ARG, "%s: width %lld not in 1..2^28", who, (long long)width);
+    return DIMN_OK;
+}
+
+extern "C" int dimn_layer_norm(int32_t device_id, void* stream, int32_t type, int64_t groups, int64_t rows, int64_t width, const void* x, int64_t x_group, int64_t x_row,
+                               const float* gamma, const float* beta, float eps, void* y, int64_t y_group, int64_t y_row, float* mean, float* rstd) {
+    CHK(norm_check("dimn_layer_norm", type, groups, rows, width));
+    if (!(eps >= 0.f)) return dimn_fail(DIMN_ERR_ARG, "dimn_layer_norm: eps %g is negative or not a number", (double)eps);
+    if (groups == 0 || rows == 0) return DIMN_OK;
+    if (!x || !y) return dimn_fail(DIMN_ERR_ARG, "dimn_layer_norm: null array");
+    OnDevice on;
+    CHK(on.enter("dimn_layer_norm", device_id));
+    NormP p{};
+    p.x = x; p.x_group = x_group; p.x_row = x_row; p.out = y; p.out_group = y_group; p.out_row = y_row;
+    p.gamma = gamma; p.beta = beta; p.mean = mean; p.rstd = rstd; p.rows = rows; p.width = (int32_t)width; p.eps = eps;
+    return norm_forward((hipStream_t)stream, type, groups, p);
+}
+
+extern "C" int dimn_layer_norm_grad_workspace(int32_t device_id, int32_t type, int64_t groups, int64_t rows, int64_t width, int64_t* bytes) {
+    CHK(norm_check("dimn_layer_norm_grad_workspace", type, groups, rows, width));
+    if (!bytes) return dimn_fail(DIMN_ERR_ARG, "dimn_layer_norm_grad_workspace: null");
+    OnDevice on;
+    CHK(on.enter("dimn_layer_norm_grad_workspace", device_id));
+    *bytes = norm_workspace_floats(type, groups, rows, (int32_t)width) * 4;
+    return DIMN_OK;
+}
+
+extern "C" int dimn_layer_norm_grad(int32_t device_id, void* stream, int32_t type, int64_t groups, int64_t rows, int64_t width, const void* dy, int64_t dy_group, int64_t dy_row,
+                                    const void* x, int64_t x_group, int64_t x_row, const float* mean, const float* rstd, const float* gamma,
+                                    void* dx, int64_t dx_group, int64_t dx_row, float* dgamma, float* dbeta, void* workspace, int64_t workspace_bytes) {
+    CHK(norm_check("dimn_layer_norm_grad", type, groups, rows, width));
+    if (groups == 0) return DIMN_OK;
+    if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return dimn_fail(DIMN_ERR_ARG, "dimn_layer_norm_grad: null array");
+    OnDevice on;
+    CHK(on.enter("dimn_layer_norm_grad", device_id));
+    if (dgamma || dbeta) {
+        const int64_t need = norm_workspace_floats(type, groups, rows, (int32_t)width) * 4;
+        if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
+            return dimn_fail(DIMN_ERR_ARG, "dimn_layer_norm_grad: a 16-byte aligned workspace of %lld bytes is needed, got %lld", (long long)need, (long long)workspace_bytes);
+    }
+    NormP p{};
+    p.x = x; p.x_group = x_group; p.x_row = x_row; p.dy = dy; p.dy_group = dy_group; p.dy_row = dy_row; p.out = dx; p.out_group = dx_group; p.out_row = dx_row;
+    p.gamma = gamma; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd); p.rows = rows; p.width = (int32_t)width;
+    return norm_backward((hipStream_t)stream, type, groups, p, dgamma, dbeta, (float*)workspace);
+}
+
+// ---- softmax cross entropy of a linear output layer -----------------------------------------------------------------------------
+namespace {
+using rowops::XentGemm;
+
+int64_t up(int64_t a, int64_t b) { return ceil_div64(a, b) * b; }
+
+// tile shapes of k_xent_gemm: 256 x 256 (8 waves), 128 x 128 (4), 64 x 128 (4)
+struct Tile { int bm, bn, wm; };
+constexpr Tile kTiles[3] = {{256, 256, 2}, {128, 128, 2}, {64, 128, 1}};
+int64_t tile_count(const Tile& t, int64_t M, int64_t N) { return ceil_div64(M, t.bm) * ceil_div64(N, t.bn); }
+int pick_tile(int64_t M, int64_t N, int ncu) {
+    if (M <= 64) return 2;
+    return tile_count(kTiles[0], M, N) >= ncu * 3 / 4 ? 0 : 1;
+}
+
+// what a call needs: operand forms, pieces of the classes, and where everything lies in the workspace
+struct XentPlan {
+    const dimn_output_loss* d;
+    bool grad, f32, labels, out_in;           // out_in: the kernel is stored [classes][width]
+    int planes, segments, ncu;
+    uint32_t a_of, b_of;
+    int64_t N, H, V, Hp, Np, P;               // Hp, Np: width / rows rounded up to 64; P: classes per piece
+    bool x_direct, w_direct, wt_direct;
+    int t_logits;
+    int64_t tiles_m, tiles_n;                 // logits
+    int t_dx, splits;
+    size_t x, xt, w, wt, g, gt, part, part_t, picked, scale, tsum, dbias, acc, bytes;
+
+    size_t take(int64_t n) { const size_t at = bytes; bytes += (size_t)up(n, 256); return at; }
+    void make(const dimn_output_loss* desc, bool with_grad, int compute_units) {
+        d = desc; grad = with_grad; ncu = compute_units;
+        N = d->rows; H = d->width; V = d->classes;
+        f32 = d->type == DIMN_TYPE_F32;
+        labels = d->target_kind <= DIMN_TARGET_I64;
+        out_in = d->kernel_in == 1;
+        planes = f32 ? 3 : 1;
+        segments = f32 ? 6 : 1;
+        a_of = f32 ? 0x001102u : 0;           // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), small terms first
+        b_of = f32 ? 0x010120u : 0;
+        Hp = up(H, 64); Np = up(N, 64);
+        const int64_t far = 1 << 22;          // (operand rows are reached by 32-bit offsets inside a tile of 256)
+        auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+        x_direct = !f32 && H % 64 == 0 && aligned(d->x) && d->x_row % 8 == 0 && d->x_row <= far && d->x_row >= 0;
+        w_direct = !f32 && out_in && H % 64 == 0 && aligned(d->kernel) && d->kernel_out % 8 == 0 && d->kernel_out <= far && d->kernel_out >= 0;
+        wt_direct = !f32 && !out_in && V % 64 == 0 && aligned(d->kernel) && d->kernel_in % 8 == 0 && d->kernel_in <= far && d->kernel_in >= 0;
+        const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0));
+        const int64_t budget = (int64_t)512 << 20;
+        P = per_class ? std::max<int64_t>(256, budget / per_class / 256 * 256) : up(V, 256);
+        P = std::min(P, far);
+        P = up(ceil_div64(V, ceil_div64(V, P)), 256);
+        t_logits = pick_tile(N, std::min(P, V), ncu);
+        tiles_m = ceil_div64(N, kTiles[t_logits].bm);
+        tiles_n = ceil_div64(V, kTiles[t_logits].bn);
+        bytes = 0;
+        x = x_direct ? 0 : take(2 * planes * N * Hp);
+        w = w_direct ? 0 : take(2 * planes * P * Hp);
+        if (!grad) {
+            part = take(8 * tiles_n * N);
+            part_t = labels ? 0 : take(8 * tiles_n * N);
+            picked = take(4 * N);
+            return;
+        }
+        xt = take(2 * planes * H * Np);
+        wt = wt_direct ? 0 : take(2 * planes * H * P);
+        g = take(2 * planes * N * P);
+        gt = take(2 * planes * P * Np);
+        scale = take(4 * N);
+        tsum = take(4 * N);
+        dbias = take(4 * tiles_m * kTiles[t_logits].wm * V);
+        t_dx = pick_tile(N, H, ncu);
+        const int64_t steps = ceil_div64(std::min(P, V), 64) * segments;
+        splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)16, ncu / tile_count(kTiles[t_dx], N, H), steps / 8}));
+        acc = take(4 * (int64_t)splits * N * H);
+    }
+};
+
+template <int EPI>
+void xent_gemm(int tile, int splits, XentGemm& p, hipStream_t st) {
+    const Tile& t = kTiles[tile];
+    p.tiles_m = (int)ceil_div64(p.M, t.bm);
+    p.tiles_n = (int)ceil_div64(p.N, t.bn);
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)splits);
+    if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, st, p);
+    else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI>), grid, dim3(256), 0, st, p);
+}
+
+// to[plane][rows][ldk] from a plane of the caller; transposed: the caller's memory runs along the rows
+void xent_lay(bool f32, bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane, hipStream_t st) {
+    const dim3 grid((unsigned)(ceil_div64(rows, 64) * (ldk / 64)));
+    if (f32) {
+        if (transposed) hipLaunchKernelGGL((rowops::k_xent_lay<float, true>), grid, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
+        else hipLaunchKernelGGL((rowops::k_xent_lay<float, false>), grid, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
+    } else {
+        if (transposed) hipLaunchKernelGGL((rowops::k_xent_lay<bf16_t, true>), grid, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
+        else hipLaunchKernelGGL((rowops::k_xent_lay<bf16_t, false>), grid, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
+    }
+}
+
+const void* at(const dimn_output_loss* d, const void* base, int64_t elements) { return (const char*)base + elements * (d->type == DIMN_TYPE_F32 ? 4 : 2); }
+
+// the logits' operands of the piece that starts at class c0 and has pv classes
+void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& p, hipStream_t st) {
+    const dimn_output_loss* d = q.d;
+    p = XentGemm{};
+    if (q.x_direct) { p.A = (const uint16_t*)d->x; p.lda = d->x_row; }
+    else {
+        p.A = (const uint16_t*)(ws + q.x); p.lda = q.Hp; p.a_plane = q.N * q.Hp;
+        if (c0 == 0) xent_lay(q.f32, false, d->x, d->x_row, q.N, q.H, (uint16_t*)(ws + q.x), q.Hp, p.a_plane, st);
+    }
+    if (q.w_direct) { p.B = (const uint16_t*)at(d, d->kernel, c0 * d->kernel_out); p.ldb = d->kernel_out; }
+    else {
+        p.B = (const uint16_t*)(ws + q.w); p.ldb = q.Hp; p.b_plane = q.P * q.Hp;
+        if (q.out_in) xent_lay(q.f32, false, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane, st);
+        else xent_lay(q.f32, true, at(d, d->kernel, c0), d->kernel_in, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane, st);
+    }
+    p.M = (int)q.N; p.N = (int)pv;
+    p.ksteps = (int)(q.Hp / 64); p.segments = q.segments; p.a_of = q.a_of; p.b_of = q.b_of;
+    p.bias = d->bias ? d->bias + c0 : nullptr;
+    p.target = d->target; p.target_row = d->target_row; p.target_kind = d->target_kind;
+    if (!q.labels) p.target = (const char*)d->target + c0 * (d->target_kind == DIMN_TARGET_F32 ? 4 : 2);
+    p.class0 = c0; p.classes = q.V;
+}
+
+int xent_check(const char* who, const dimn_output_loss* d) {
+    if (!d) return dimn_fail(DIMN_ERR_ARG, "%s: null description", who);
+    if (d->type != DIMN_TYPE_F32 && d->type != DIMN_TYPE_BF16) return dimn_fail(DIMN_ERR_UNSUP, "%s: element type %d (DIMN_TYPE_F32 or DIMN_TYPE_BF16)", who, d->type);
+    if (d->target_kind < DIMN_TARGET_I32 || d->target_kind > DIMN_TARGET_BF16) return dimn_fail(DIMN_ERR_UNSUP, "%s: target kind %d", who, d->target_kind);
+    const int64_t most = 1 << 22;
+    if (d->rows < 0 || d->rows > most || d->width < 1 || d->width > most || d->classes < 1 || d->classes > most)
+        return dimn_fail(DIMN_ERR_ARG, "%s: %lld rows, width %lld, %lld classes (each up to 2^22, the latter two at least 1)", who, (long long)d->rows, (long long)d->width, (long long)d->classes);
+    if (ceil_div64(d->rows, 64) * ceil_div64(d->classes, 128) > INT32_MAX || ceil_div64(d->width, 64) * ceil_div64(std::max(d->rows, d->classes), 64) > INT32_MAX)
+        return dimn_fail(DIMN_ERR_ARG, "%s: %lld rows, width %lld, %lld classes are too many tiles for one launch", who, (long long)d->rows, (long long)d->width, (long long)d->classes);
+    if (d->kernel_in != 1 && d->kernel_out != 1) return dimn_fail(DIMN_ERR_ARG, "%s: one of the kernel's strides (%lld, %lld) has to be 1", who, (long long)d->kernel_in, (long long)d->kernel_out);
+    if (d->rows > 0 && (!d->x || !d->kernel || !d->target)) return dimn_fail(DIMN_ERR_ARG, "%s: null array", who);
+    return DIMN_OK;
+}
+int xent_space(const char* who, const XentPlan& q, const void* workspace, int64_t bytes) {
+    if (!workspace || ((uintptr_t)workspace & 255) || bytes < (int64_t)q.bytes)
+        return dimn_fail(DIMN_ERR_ARG, "%s: a 256-byte aligned workspace of %lld bytes is needed, got %lld", who, (long long)q.bytes, (long long)bytes);
+    return DIMN_OK;
+}
+}  // namespace
+
+extern "C" int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, int32_t grad, int64_t* bytes) {
+    const char* who = "dimn_linear_cross_entropy_workspace";
+    CHK(xent_check(who, d));
+    if (!bytes) return dimn_fail(DIMN_ERR_ARG, "%s: null", who);
+    OnDevice on;
+    CHK(on.enter(who, d->device_id));
+    XentPlan q;
+    q.make(d, grad != 0, compute_units());
+    *bytes = (int64_t)q.bytes;
+    return DIMN_OK;
+}
+
+extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream, float* loss, float* lse, void* workspace, int64_t workspace_bytes) {
+    const char* who = "dimn_linear_cross_entropy";
+    CHK(xent_check(who, d));
+    if (d->rows == 0) return DIMN_OK;
+    if (!loss || !lse) return dimn_fail(DIMN_ERR_ARG, "%s: null array", who);
+    OnDevice on;
+    CHK(on.enter(who, d->device_id));
+    hipStream_t st = (hipStream_t)stream;
+    XentPlan q;
+    q.make(d, false, compute_units());
+    CHK(xent_space(who, q, workspace, workspace_bytes));
+    char* ws = (char*)workspace;
+    const Tile& t = kTiles[q.t_logits];
+    for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
+        XentGemm p;
+        xent_logits(q, ws, c0, std::min(q.P, q.V - c0), p, st);
+        p.part = (float2*)(ws + q.part) + c0 / t.bn * q.N;
+        if (!q.labels) p.part_t = (float2*)(ws + q.part_t) + c0 / t.bn * q.N;
+        p.picked = (float*)(ws + q.picked);
+        xent_gemm<rowops::XE_LSE>(q.t_logits, 1, p, st);
+    }
+    rowops::XentRows r{};
+    r.part = (const float2*)(ws + q.part);
+    r.part_t = q.labels ? nullptr : (const float2*)(ws + q.part_t);
+    r.picked = (const float*)(ws + q.picked);
+    r.tiles = q.tiles_n; r.rows = q.N; r.classes = q.V;
+    r.target = d->target; r.target_kind = d->target_kind;
+    r.loss = loss; r.lse = lse;
+    hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, 64)), dim3(1024), 0, st, r);
+    HIPCHK(hipGetLastError());
+    return DIMN_OK;
+}
+
+extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* stream, const float* dloss, const float* lse, void* dx, int64_t dx_row,
+                                              void* dkernel, int64_t dkernel_in, int64_t dkernel_out, float* dbias, void* workspace, int64_t workspace_bytes) {
+    const char* who = "dimn_linear_cross_entropy_grad";
+    CHK(xent_check(who, d));
+    if (!dkernel || (d->rows > 0 && (!dloss || !lse || !dx))) return dimn_fail(DIMN_ERR_ARG, "%s: null array", who);
+    if (dkernel_in != 1 && dkernel_out != 1) return dimn_fail(DIMN_ERR_ARG, "%s: one of the strides of dkernel (%lld, %lld) has to be 1", who, (long long)dkernel_in, (long long)dkernel_out);
+    OnDevice on;
+    CHK(on.enter(who, d->device_id));
+    hipStream_t st = (hipStream_t)stream;
+    XentPlan q;
+    q.make(d, true, compute_units());
+    if (d->rows == 0) return dimn_fail(DIMN_ERR_ARG, "%s: no rows", who);
+    CHK(xent_space(who, q, workspace, workspace_bytes));
+    char* ws = (char*)workspace;
+    float* scale = (float*)(ws + q.scale);
+    float* tsum = (float*)(ws + q.tsum);
+    hipLaunchKernelGGL(rowops::k_xent_rows, dim3((unsigned)(q.labels ? ceil_div64(q.N, 256) : q.N)), dim3(256), 0, st, d->target, d->target_kind, d->target_row, q.N, q.V, dloss, scale, tsum);
+    uint16_t* xt = (uint16_t*)(ws + q.xt);
+    const int64_t xt_plane = q.H * q.Np;
+    xent_lay(q.f32, true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane, st);
+    const bool dk_out_in = dkernel_in == 1;
+    for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
+        const int64_t pv = std::min(q.P, q.V - c0), ldg = up(pv, 64);
+        XentGemm p;
+        xent_logits(q, ws, c0, pv, p, st);
+        p.lse = lse; p.scale = scale; p.tsum = tsum;
+        p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
+        p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
+        p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = q.V;
+        xent_gemm<rowops::XE_GRAD>(q.t_logits, 1, p, st);
+        // dx += G W^T
+        XentGemm a{};
+        a.A = p.G; a.lda = ldg; a.a_plane = p.g_plane;
+        if (q.wt_direct) { a.B = (const uint16_t*)at(d, d->kernel, c0); a.ldb = d->kernel_in; }
+        else {
+            uint16_t* wt = (uint16_t*)(ws + q.wt);
+            a.B = wt; a.ldb = ldg; a.b_plane = q.H * ldg;
+            if (q.out_in) xent_lay(q.f32, true, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, q.H, pv, wt, ldg, a.b_plane, st);
+            else xent_lay(q.f32, false, at(d, d->kernel, c0), d->kernel_in, q.H, pv, wt, ldg, a.b_plane, st);
+        }
+        a.M = (int)q.N; a.N = (int)q.H;
+        a.ksteps = (int)(ldg / 64); a.segments = q.segments; a.a_of = q.a_of; a.b_of = q.b_of;
+        a.acc = (float*)(ws + q.acc); a.acc_split = q.N * q.H; a.acc_first = c0 == 0;
+        xent_gemm<rowops::XE_ADD>(q.t_dx, q.splits, a, st);
+        // dW of the piece
+        XentGemm w{};
+        w.ksteps = (int)(q.Np / 64); w.segments = q.segments; w.a_of = q.a_of; w.b_of = q.b_of;
+        w.c_type = d->type;
+        const uint16_t *gt = p.GT, *xa = xt;
+        if (dk_out_in) {
+            w.A = gt; w.lda = q.Np; w.a_plane = p.gt_plane; w.M = (int)pv;
+            std::swap(w.a_of, w.b_of);           // the operands change sides: the same products in the same order, the same bits
+            w.B = xa; w.ldb = q.Np; w.b_plane = xt_plane; w.N = (int)q.H;
+            w.C = const_cast<void*>(at(d, dkernel, c0 * dkernel_out)); w.ldc = dkernel_out;
+        } else {
+            w.A = xa; w.lda = q.Np; w.a_plane = xt_plane; w.M = (int)q.H;
+            w.B = gt; w.ldb = q.Np; w.b_plane = p.gt_plane; w.N = (int)pv;
+            w.C = const_cast<void*>(at(d, dkernel, c0)); w.ldc = dkernel_in;
+        }
+        xent_gemm<rowops::XE_STORE>(pick_tile(w.M, w.N, q.ncu), 1, w, st);
+    }
+    const unsigned blocks = (unsigned)ceil_div64(q.N * q.H, 1024);
+    if (q.f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (float*)dx, dx_row);
+    else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (bf16_t*)dx, dx_row);
+    if (dbias)
+        hipLaunchKernelGGL(rowops::k_xent_dbias, dim3((unsigned)ceil_div64(q.V, 256)), dim3(256), 0, st, (const float*)(ws + q.dbias), q.V,
+                           (int)(q.tiles_m * kTiles[q.t_logits].wm), q.V, dbias);
+    HIPCHK(hipGetLastError());
+    return DIMN_OK;
+}

@@ -1,0 +1,506 @@
+// dimn_xent.h -- softmax cross entropy of a linear output layer, in pieces of the classes, the logits never kept (gfx950).
+//
+//   z = x W + b,  lse = log sum_v exp z_v
+//   label y:    loss = lse - z_y                          G_v = dloss (exp(z_v - lse) - [v = y])
+//   profile t:  loss = sum_v t_v lse - sum_v t_v z_v       G_v = dloss (sum(t) exp(z_v - lse) - t_v)
+//   dx = G W^T,  dW = x^T G,  db = sum over rows of G
+//
+// Everything is one matrix product with different epilogues (k_xent_gemm): C[m][n] = sum_k A[m][k] B[n][k], both operands bfloat16 and
+// k-contiguous, float32 accumulation on the bf16 matrix cores.
+//   * Forward: A = rows, B = classes.  A workgroup leaves the running maximum and the sum of exponentials of each row over its classes (8 bytes
+//     for 256 logits), k_xent_lse joins them.
+//   * Backward, per piece of the classes: the logits again, G of the piece in the epilogue -- kept in both memory orders, because each of the
+//     two products that read it wants its own inner dimension contiguous --, then dx += G W^T and dW = x^T G of the piece.
+//   * float32 operands are split into three bfloat16 terms each (8 + 8 + 8 bits of the 24-bit significand, exact), and the six products whose
+//     weight is 2^-16 or more are summed: what is left out is below 2^-23 of a product, the rounding of a float32 product itself.  Six passes
+//     of the bf16 matrix cores still have 2.7 times the rate of the float32 ones.
+//   * Operands that are k-contiguous, aligned and a multiple of 64 long are read in place; everything else is laid out by k_xent_lay.
+#pragma once
+#include "dimn_rowops.h"
+
+namespace rowops {
+
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
+__device__ __forceinline__ float from_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
+
+// x = hi + mid + lo, each a bfloat16.  The remainders are exact (Sterbenz); an infinity or NaN stays in the first term alone.
+__device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
+    b[0] = to_bf16(x);
+    const float hi = from_bf16(b[0]);
+    const bool finite = fabsf(hi) <= 3.38953139e38f;
+    const float r1 = finite ? x - hi : 0.f;
+    b[1] = to_bf16(r1);
+    const float r2 = r1 - from_bf16(b[1]);
+    b[2] = to_bf16(r2);
+}
+
+// ---- operand layout -----------------------------------------------------------------------------------------------------------
+// to[plane][r][k] = bfloat16 term `plane` of from[r][k], zero for cols <= k < ldk (ldk: a multiple of 64).  T = float: three planes, T = bf16_t: one.
+// TRANSPOSED: from is [k][r] with r contiguous (row stride `ld` along k).  64 x 64 tiles, through LDS when transposed.
+template <typename T, bool TRANSPOSED>
+__global__ __launch_bounds__(256) void k_xent_lay(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
+    constexpr int PL = sizeof(T) == 4 ? 3 : 1;
+    const int64_t tiles_k = ldk >> 6;
+    const int64_t tr = blockIdx.x / tiles_k, tk = blockIdx.x - tr * tiles_k;
+    const int64_t r0 = tr * 64, k0 = tk * 64;
+    const int q = threadIdx.x & 15, s = threadIdx.x >> 4;        // 16 pieces of four x 16 lines
+    __shared__ T tile[TRANSPOSED ? 64 : 1][TRANSPOSED ? 66 : 1];
+    if constexpr (TRANSPOSED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t k = k0 + s + 16 * i;
+            T v[4] = {0, 0, 0, 0};
+            if (k < cols) {
+                const T* p = from + k * ld + r0 + 4 * q;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (r0 + 4 * q + j < rows) v[j] = p[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tile[s + 16 * i][4 * q + j] = v[j];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + s + 16 * i;
+        if (r >= rows) continue;
+        T v[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (TRANSPOSED) v[j] = tile[4 * q + j][s + 16 * i];
+            else if (k0 + 4 * q + j < cols) v[j] = from[r * ld + k0 + 4 * q + j];
+        }
+        u16x4 o[PL];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (PL == 3) {
+                uint16_t b[3];
+                split3(v[j], b);
+                o[0][j] = b[0]; o[1][j] = b[1]; o[2][j] = b[2];
+            } else o[0][j] = v[j];
+        }
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl) *(u16x4*)(to + pl * plane + r * ldk + k0 + 4 * q) = o[pl];
+    }
+}
+
+// ---- the product --------------------------------------------------------------------------------------------------------------
+struct XentGemm {
+    const uint16_t* A; const uint16_t* B;      // [plane][m][lda], [plane][n][ldb]; 16-byte aligned, lda / ldb multiples of 8
+    int64_t lda, ldb, a_plane, b_plane;
+    int32_t M, N;                              // columns from N on are not classes / not stored
+    int32_t ksteps;                            // 64-deep steps of one plane
+    int32_t segments;                          // plane pairs (1 or 6): pair i multiplies plane (a_of >> 4 i) & 15 of A with plane (b_of >> 4 i) & 15 of B
+    uint32_t a_of, b_of;
+    int32_t tiles_m, tiles_n;
+    // epilogues over logits: z = C + bias
+    const float* bias;                         // [N] or NULL
+    const void* target; int64_t target_row;    // labels (int32 / int64 [M]), or a profile [M][..] of float32 / bfloat16 (class 0 of the piece first)
+    int32_t target_kind;
+    int64_t class0, classes;                   // first class of the piece; classes in all
+    // forward
+    float2* part;                              // [tiles_n][M]: (maximum, sum of exp(z - maximum))
+    float2* part_t;                            // profile: [tiles_n][M]: (sum of t, sum of t z)
+    float* picked;                             // labels: [M], z of the label, written by the workgroup that holds it
+    // G
+    const float* lse; const float* scale;      // [M]: dloss (0 for a row without a target)
+    const float* tsum;                         // profile: [M]
+    uint16_t* G; int64_t ldg, g_plane;         // [plane][M][ldg], columns N .. ldg zero
+    uint16_t* GT; int64_t ldgt, gt_plane;      // [plane][N][ldgt], columns M .. ldgt zero
+    float* dbias_part; int64_t dbias_ld;       // [2 tiles_m][dbias_ld]: column sums of G over the rows of one wave row
+    // result
+    void* C; int64_t ldc; int32_t c_type;      // epilogue 2: C[m][n], DIMN_TYPE_*
+    float* acc; int64_t acc_split; int32_t acc_first;   // epilogue 3: acc[split][M][N] (+)= C
+};
+enum { XE_LSE = 0, XE_GRAD = 1, XE_STORE = 2, XE_ADD = 3 };
+enum { XT_I32 = 0, XT_I64 = 1, XT_F32 = 2, XT_BF16 = 3 };        // DIMN_TARGET_*
+
+__device__ __forceinline__ int64_t xent_label(const XentGemm& p, int64_t row) {
+    return p.target_kind == XT_I64 ? ((const int64_t*)p.target)[row] : (int64_t)((const int32_t*)p.target)[row];
+}
+// four consecutive entries of a profile row, 0 from `n` on
+__device__ __forceinline__ f32x4 xent_profile4(const XentGemm& p, int64_t row, int col, int n) {
+    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+    if (p.target_kind == XT_F32) {
+        const float* q = (const float*)p.target + row * p.target_row + col;
+        if (col + 4 <= n) t = *(const f32x4u*)q;
+        else
+#pragma unroll
+            for (int r = 0; r < 4; ++r) if (col + r < n) t[r] = q[r];
+    } else {
+        const uint16_t* q = (const uint16_t*)p.target + row * p.target_row + col;
+        if (col + 4 <= n) {
+            const u16x4u v = *(const u16x4u*)q;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[r] = from_bf16(v[r]);
+        } else
+#pragma unroll
+            for (int r = 0; r < 4; ++r) if (col + r < n) t[r] = from_bf16(q[r]);
+    }
+    return t;
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+
+// Tile BM x BN per workgroup, WM x WN waves; k in steps of 64, two stages of LDS filled by 16-byte DMA while the other one is multiplied, one
+// barrier per step.  A row of a tile is 128 bytes; its eight 16-byte pieces are stored at piece ^ (row & 7), so that the sixteen rows a
+// fragment reads spread over all banks (the DMA writes LDS in lane order: the permutation is made on the global side).
+// The matrix instruction takes B's rows as its rows and A's as its columns: a lane then holds four consecutive n of one m, so that
+// sums along n are mostly inside a lane and results leave in pieces of four.
+template <int BM, int BN, int WM, int WN, int EPI>
+__global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
+    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
+    constexpr int LOADS = (BM + BN) / 8 / NW;
+    static_assert(LOADS * 8 * NW == BM + BN, "whole requests per wave");
+    __shared__ __attribute__((aligned(1024))) uint16_t lds[2][(BM + BN) * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN, li = lane & 15, lj = lane >> 4;
+    // Workgroup b runs on XCD b % 8: each XCD gets a consecutive range of the tiles, ordered in columns of eight m tiles, so that the 32
+    // workgroups of an XCD at a time share eight A and four B tiles in its L2.
+    int tile;
+    {
+        const int total = p.tiles_m * p.tiles_n, b = blockIdx.x, x = b & 7, q = total >> 3, rem = total & 7;
+        tile = x * q + (x < rem ? x : rem) + (b >> 3);
+    }
+    int tm, tn;
+    {
+        const int per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
+        const int h = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
+        tn = in / h;
+        tm = grp * 8 + in - tn * h;
+    }
+    const int m0 = tm * BM, n0 = tn * BN;
+    // requests: request c of this wave brings rows 8 (wave LOADS + c) .. + 7 of the stacked [A; B] tile
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int c = 0; c < LOADS; ++c) {
+        const int row = (wave * LOADS + c) * 8 + (lane >> 3);
+        const int piece = (lane & 7) ^ (row & 7);
+        const bool isA = (wave * LOADS + c) * 8 < BM;
+        int r = isA ? row : row - BM;
+        const int lim = isA ? p.M - 1 - m0 : p.N - 1 - n0;       // rows past the end read the last one: their results are never used
+        r = r < lim ? r : lim;
+        off[c] = (uint32_t)((int64_t)r * (isA ? p.lda : p.ldb) * 2 + piece * 16);
+    }
+    const char* Abase = (const char*)(p.A + (int64_t)m0 * p.lda);
+    const char* Bbase = (const char*)(p.B + (int64_t)n0 * p.ldb);
+    const int total = p.ksteps * p.segments;
+    const int S = gridDim.y, sp = blockIdx.y;
+    const int tbeg = (int)((int64_t)total * sp / S), tend = (int)((int64_t)total * (sp + 1) / S);
+    int seg = tbeg / p.ksteps, ks = tbeg - seg * p.ksteps;       // of the next request
+    auto request = [&](int stage) {
+        const char* a = Abase + (int64_t)((p.a_of >> (4 * seg)) & 15) * p.a_plane * 2 + (int64_t)ks * 128;
+        const char* b = Bbase + (int64_t)((p.b_of >> (4 * seg)) & 15) * p.b_plane * 2 + (int64_t)ks * 128;
+#pragma unroll
+        for (int c = 0; c < LOADS; ++c) {
+            const bool isA = (wave * LOADS + c) * 8 < BM;
+            __builtin_amdgcn_global_load_lds((global_void*)((isA ? a : b) + off[c]), (lds_void*)&lds[stage][(wave * LOADS + c) * 512], 16, 0, 0);
+        }
+        if (++ks == p.ksteps) { ks = 0; ++seg; }
+    };
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int stage) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            bf8 a[FM], b[FN];
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int row = BM + wn * TN + 16 * j + li;
+                b[j] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ (row & 7)) << 3)];
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int row = wm * TM + 16 * i + li;
+                a[i] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ (row & 7)) << 3)];
+            }
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        }
+    };
+    if (tbeg < tend) request(0);
+    for (int t = tbeg; t < tend; ++t) {
+        const int stage = (t - tbeg) & 1;
+        __syncthreads();                                         // the stage's bytes have landed (the barrier waits for this wave's requests first) and
+        if (t + 1 < tend) request(stage ^ 1);                    // everybody is done with the other stage
+        multiply(stage);
+    }
+    // a lane's results: C[m0 + wm TM + 16 i + li][n0 + wn TN + 16 j + 4 lj + r] in acc[i][j][r]
+    const int nb = n0 + wn * TN + 4 * lj;
+    if constexpr (EPI == XE_STORE || EPI == XE_ADD) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int64_t m = m0 + wm * TM + 16 * i + li;
+            if (m >= p.M) continue;
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int n = nb + 16 * j;
+                if (n >= p.N) continue;
+                const f32x4 v = acc[i][j];
+                if constexpr (EPI == XE_ADD) {
+                    float* q = p.acc + (int64_t)sp * p.acc_split + m * p.N + n;
+                    if (n + 4 <= p.N) *(f32x4u*)q = p.acc_first ? v : *(const f32x4u*)q + v;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) if (n + r < p.N) q[r] = p.acc_first ? v[r] : q[r] + v[r];
+                } else if (p.c_type == DIMN_TYPE_F32) {
+                    float* q = (float*)p.C + m * p.ldc + n;
+                    if (n + 4 <= p.N) *(f32x4u*)q = v;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) if (n + r < p.N) q[r] = v[r];
+                } else {
+                    uint16_t* q = (uint16_t*)p.C + m * p.ldc + n;
+                    u16x4u o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = to_bf16(v[r]);
+                    if (n + 4 <= p.N) *(u16x4u*)q = o;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) if (n + r < p.N) q[r] = o[r];
+                }
+            }
+        }
+        return;
+    }
+    if constexpr (EPI == XE_LSE || EPI == XE_GRAD) {
+        const bool labels = p.target_kind <= XT_I64, split = p.segments > 1;
+        f32x4 bias[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = nb + 16 * j;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[j][r] = p.bias && n + r < p.N ? p.bias[n + r] : 0.f;
+        }
+        if constexpr (EPI == XE_LSE) {
+            float2* red = (float2*)&lds[0][0];                   // [WN][BM] (maximum, sum), then [WN][BM] (sum t, sum t z)
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int mr = wm * TM + 16 * i + li;
+                const int64_t m = m0 + mr;
+                const bool mine = m < p.M;
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[i][j][r] += bias[j][r];
+                        if (nb + 16 * j + r < p.N) top = fmaxf(top, acc[i][j][r]);
+                    }
+                if (labels) {
+                    const int64_t y = mine ? xent_label(p, m) - p.class0 - nb : -1;
+                    if (y >= 0 && y < TN && (y & 15) < 4 && nb + y < p.N) {
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) if (y == 16 * j + r) p.picked[m] = acc[i][j][r];
+                    }
+                } else {
+                    float st = 0.f, stz = 0.f;
+                    if (mine)
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) {
+                            const f32x4 t = xent_profile4(p, m, nb + 16 * j, p.N);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) { st += t[r]; stz += t[r] != 0.f ? t[r] * acc[i][j][r] : 0.f; }
+                        }
+                    st += __shfl_xor(st, 16); stz += __shfl_xor(stz, 16);
+                    st += __shfl_xor(st, 32); stz += __shfl_xor(stz, 32);
+                    if (lj == 0) red[(WN + wn) * BM + mr] = make_float2(st, stz);
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float ref = top == -INFINITY ? 0.f : top;
+                float s = 0.f;
+#pragma unroll
+                for (int j = 0; j < FN; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) if (nb + 16 * j + r < p.N) s += split ? expf(acc[i][j][r] - ref) : __expf(acc[i][j][r] - ref);
+                s += __shfl_xor(s, 16);
+                s += __shfl_xor(s, 32);
+                if (lj == 0) red[wn * BM + mr] = make_float2(top, s);
+            }
+            __syncthreads();
+            for (int mr = tid; mr < BM; mr += 64 * NW) {
+                if (m0 + mr >= p.M) break;
+                float top = -INFINITY, s = 0.f;
+#pragma unroll
+                for (int w = 0; w < WN; ++w) top = fmaxf(top, red[w * BM + mr].x);
+                const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                for (int w = 0; w < WN; ++w) { const float2 v = red[w * BM + mr]; s += v.y * __expf((v.x == -INFINITY ? ref : v.x) - ref); }
+                const int64_t at = (int64_t)tn * p.M + m0 + mr;
+                p.part[at] = make_float2(top, s);
+                if (!labels) {
+                    float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < WN; ++w) { const float2 v = red[(WN + w) * BM + mr]; t.x += v.x; t.y += v.y; }
+                    p.part_t[at] = t;
+                }
+            }
+        } else {
+            float col[FN][4];
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) col[j][r] = 0.f;
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const int64_t m = m0 + wm * TM + 16 * i + li;
+                const bool mine = m < p.M;
+                const float lse = mine ? p.lse[m] : 0.f, d = mine ? p.scale[m] : 0.f;
+                const float ts = labels ? 1.f : (mine ? p.tsum[m] : 0.f);
+                const int64_t y = labels && mine ? xent_label(p, m) - p.class0 - nb : -1;
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int n = nb + 16 * j;
+                    f32x4 t = {0.f, 0.f, 0.f, 0.f};
+                    if (!labels && mine && n < p.N) t = xent_profile4(p, m, n, p.N);
+                    float g[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float z = acc[i][j][r] + bias[j][r];
+                        const float e = z == -INFINITY ? 0.f : (split ? expf(z - lse) : __expf(z - lse));   // (__expf: 2^-24 |z - lse| off, too much only for float32 results)
+                        const float hot = labels ? (y == 16 * j + r ? 1.f : 0.f) : t[r];
+                        g[r] = d != 0.f && n + r < p.N ? d * (ts * e - hot) : 0.f;
+                        col[j][r] += g[r];
+                    }
+#pragma unroll
+                    for (int pl = 0; pl < 3; ++pl) {
+                        if (pl > 0 && !split) break;
+                        u16x4 o;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            o[r] = to_bf16(g[r]);
+                            g[r] -= from_bf16(o[r]);
+                        }
+                        if (mine && n < p.ldg) *(u16x4*)(p.G + pl * p.g_plane + m * p.ldg + n) = o;
+                        if (m < p.ldgt)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) if (n + r < p.N) p.GT[pl * p.gt_plane + (int64_t)(n + r) * p.ldgt + m] = o[r];
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float s = col[j][r];
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+                    if (li == 0 && nb + 16 * j + r < p.N) p.dbias_part[(int64_t)(tm * WM + wm) * p.dbias_ld + p.class0 + nb + 16 * j + r] = s;
+                }
+        }
+    }
+}
+
+// loss and lse of every row from the partial sums of the class tiles.  grid ceil(rows / 64), 1024 threads: 64 rows x 16 strands of tiles.
+struct XentRows {
+    const float2* part; const float2* part_t; const float* picked;
+    int64_t tiles, rows, classes;
+    const void* target; int32_t target_kind;
+    float* loss; float* lse;
+};
+__global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
+    __shared__ float2 red[16][64];
+    __shared__ float2 red_t[16][64];
+    const int c = threadIdx.x & 63, strand = threadIdx.x >> 6;
+    const int64_t row = (int64_t)blockIdx.x * 64 + c;
+    float top = -INFINITY, s = 0.f;
+    float2 t = make_float2(0.f, 0.f);
+    if (row < p.rows) {
+#pragma unroll 4
+        for (int64_t k = strand; k < p.tiles; k += 16) {
+            const float2 v = p.part[k * p.rows + row];
+            const float m = fmaxf(top, v.x);
+            if (m > -INFINITY) { s = s * __expf(top - m) + v.y * __expf(v.x - m); top = m; }
+            else if (v.y != v.y || v.x != v.x) s = NAN;          // a tile of NaNs has no maximum: its sum says so
+        }
+        if (p.part_t)
+            for (int64_t k = strand; k < p.tiles; k += 16) { const float2 v = p.part_t[k * p.rows + row]; t.x += v.x; t.y += v.y; }
+    }
+    red[strand][c] = make_float2(top, s);
+    red_t[strand][c] = t;
+    __syncthreads();
+    if (strand != 0 || row >= p.rows) return;
+    top = -INFINITY; s = 0.f; t = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w][c].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const float2 v = red[w][c];
+        s += v.y * (v.x == -INFINITY ? 1.f : __expf(v.x - ref));
+        t.x += red_t[w][c].x;
+        t.y += red_t[w][c].y;
+    }
+    const float lse = top == -INFINITY && s == 0.f ? -INFINITY : ref + __logf(s);
+    p.lse[row] = lse;
+    float loss;
+    if (p.target_kind <= XT_I64) {
+        const int64_t y = p.target_kind == XT_I64 ? ((const int64_t*)p.target)[row] : (int64_t)((const int32_t*)p.target)[row];
+        if (y < 0) loss = 0.f;
+        else if (y >= p.classes) loss = NAN;
+        else { const float z = p.picked[row]; loss = z == -INFINITY ? INFINITY : lse - z; }
+    } else loss = t.x == 0.f && t.y == 0.f ? 0.f : t.x * lse - t.y;
+    p.loss[row] = loss;
+}
+
+// Backward, per row: scale = dloss, or 0 for a row without a target (label negative or not a class); tsum = the sum of its profile.
+__global__ __launch_bounds__(256) void k_xent_rows(const void* target, int32_t kind, int64_t target_row, int64_t rows, int64_t classes, const float* __restrict__ dloss,
+                                                   float* __restrict__ scale, float* __restrict__ tsum) {
+    if (kind <= XT_I64) {
+        const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (row >= rows) return;
+        const int64_t y = kind == XT_I64 ? ((const int64_t*)target)[row] : (int64_t)((const int32_t*)target)[row];
+        scale[row] = y >= 0 && y < classes ? dloss[row] : 0.f;
+        return;
+    }
+    const int64_t row = blockIdx.x;                              // one workgroup per row
+    __shared__ float red[4];
+    float s = 0.f;
+    if (kind == XT_F32) { const float* t = (const float*)target + row * target_row; for (int64_t c = threadIdx.x; c < classes; c += 256) s += t[c]; }
+    else { const uint16_t* t = (const uint16_t*)target + row * target_row; for (int64_t c = threadIdx.x; c < classes; c += 256) s += from_bf16(t[c]); }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) { tsum[row] = (red[0] + red[1]) + (red[2] + red[3]); scale[row] = dloss[row]; }
+}
+
+// out[m][n] = sum of the splits' float32 sums, rounded once.  256 threads, four elements each.
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ acc, int64_t split, int splits, int64_t rows, int64_t cols, T* __restrict__ out, int64_t ld) {
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, total = rows * cols;
+    for (int r = 0; r < 4 && e + r < total; ++r) {
+        float s = 0.f;
+        for (int k = 0; k < splits; ++k) s += acc[k * split + e + r];
+        const int64_t m = (e + r) / cols, n = e + r - m * cols;
+        if constexpr (sizeof(T) == 4) out[m * ld + n] = s; else out[m * ld + n] = to_bf16(s);
+    }
+}
+
+// dbias = the partial column sums, added in order
+__global__ __launch_bounds__(256) void k_xent_dbias(const float* __restrict__ part, int64_t ld, int parts, int64_t classes, float* __restrict__ dbias) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= classes) return;
+    float s = 0.f;
+    for (int k = 0; k < parts; ++k) s += part[k * ld + c];
+    dbias[c] = s;
+}
+
+}  // namespace rowops

@@ -391,6 +391,62 @@ int dimn_col_stats_first(const double* a, int64_t n, int64_t g, int64_t ld, doub
                          double* vmax, int32_t* has_nan, int32_t threads);
 int dimn_col_stats_var(const double* a, int64_t n, int64_t g, int64_t ld, const double* avg, double* var, int32_t threads);
 
+/* ---- row operators on device arrays (no handle; the reference has no analogue: Keras layers and losses a sub-network may be built
+ * from beside Dense / Dropout).  ABI 10. ----------------------------------------------------------------------------------------
+ * Every array is device memory of `device_id`; `stream` is a hipStream_t of that device (NULL: its default stream).  A call queues its
+ * kernels on the stream and returns; nothing is allocated, copied to the host or waited for, so it can be captured into a graph, and two
+ * calls on different streams run side by side as long as their workspaces and outputs differ.  The calling thread's current device is
+ * left as it was.  Strides count elements; the last axis of every plane is contiguous and nothing else is assumed about alignment
+ * (workspaces: 16 bytes).  Rows past `rows` are neither read nor written.  The same arguments give the same bits. */
+#define DIMN_TYPE_F32 0
+#define DIMN_TYPE_BF16 1
+/* Layer normalisation of [groups][rows] rows of `width` elements (keras.layers.LayerNormalization, axis -1):
+ *   y = (x - mean) * rstd * gamma + beta,  rstd = 1 / sqrt(mean((x - mean)^2) + eps).
+ * x, y of element type `type`; gamma, beta float32 [groups][width] (NULL: 1 / 0); mean, rstd float32 [groups][rows] (NULL: not wanted).
+ * y may be x when their strides agree. */
+int dimn_layer_norm(int32_t device_id, void* stream, int32_t type, int64_t groups, int64_t rows, int64_t width,
+                    const void* x, int64_t x_group, int64_t x_row, const float* gamma, const float* beta, float eps,
+                    void* y, int64_t y_group, int64_t y_row, float* mean, float* rstd);
+/* Its backward pass from the forward's mean and rstd: dx, and dgamma / dbeta float32 [groups][width] summed over the rows (NULL: not
+ * wanted; neither wanted: no workspace needed; groups without rows get zeros).  dx may be dy, or x, when their strides agree. */
+int dimn_layer_norm_grad_workspace(int32_t device_id, int32_t type, int64_t groups, int64_t rows, int64_t width, int64_t* bytes);
+int dimn_layer_norm_grad(int32_t device_id, void* stream, int32_t type, int64_t groups, int64_t rows, int64_t width,
+                         const void* dy, int64_t dy_group, int64_t dy_row, const void* x, int64_t x_group, int64_t x_row,
+                         const float* mean, const float* rstd, const float* gamma,
+                         void* dx, int64_t dx_group, int64_t dx_row, float* dgamma, float* dbeta,
+                         void* workspace, int64_t workspace_bytes);
+
+/* Softmax cross entropy of a linear output layer z = x W + b over many classes, computed in pieces of the classes: the logits are never
+ * kept.  Per row, with lse = log(sum over the classes of exp(z)):
+ *   labels:   loss = lse - z[label].  A negative label is a row without a target: loss 0, no gradient.  A label >= classes: loss NaN, no
+ *             gradient.  A label whose logit is -infinity (masked by the bias): loss +infinity.
+ *   profiles: loss = sum(t) lse - sum(t z) for a row t of weights over the classes (counts, probabilities); t = 0 takes no part.
+ * A class with z = -infinity has probability 0, also in a row that has no other class left. */
+#define DIMN_TARGET_I32 0         /* labels                                                     */
+#define DIMN_TARGET_I64 1
+#define DIMN_TARGET_F32 2         /* profiles, [rows][classes]                                  */
+#define DIMN_TARGET_BF16 3
+typedef struct dimn_output_loss {
+    int32_t device_id, type;      /* DIMN_TYPE_* of x and the kernel                            */
+    int64_t rows, width, classes; /* up to 2^22 each                                            */
+    const void* x;                /* [rows][width], row stride x_row                            */
+    int64_t x_row;
+    const void* kernel;           /* [width][classes], strides kernel_in (along width) and kernel_out (along classes); one of them is 1 */
+    int64_t kernel_in, kernel_out;
+    const float* bias;            /* [classes], or NULL: 0                                      */
+    const void* target;           /* labels [rows], or profiles with row stride target_row      */
+    int64_t target_row;
+    int32_t target_kind;          /* DIMN_TARGET_*                                              */
+} dimn_output_loss;
+/* Bytes of workspace (256-byte aligned) of the forward (grad = 0) / backward (grad != 0) call. */
+int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, int32_t grad, int64_t* bytes);
+/* loss, lse: float32 [rows]. */
+int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream, float* loss, float* lse, void* workspace, int64_t workspace_bytes);
+/* The backward pass from the forward's lse and the gradient dloss [rows] of the losses: dx [rows][width], dkernel [width][classes] (strides
+ * as the kernel's, one of them 1), both of element type `type`, and dbias float32 [classes] (NULL: not wanted). */
+int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* stream, const float* dloss, const float* lse, void* dx, int64_t dx_row,
+                                   void* dkernel, int64_t dkernel_in, int64_t dkernel_out, float* dbias, void* workspace, int64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,390 @@
+"""Softmax cross entropy of a linear output layer on device tensors (deepimpute_amd.ops.linear_cross_entropy / _grad, include/dimn.h
+dimn_linear_cross_entropy*) against the formulas in float64.
+
+Tolerances, all propagated element by element in float64 (u = 2^-24, half a float32 step):
+  * a product of bfloat16 numbers is exact in float32; a float32 operand is three bfloat16 terms and the products left out are below 4 u of
+    a product; a sum over K in steps of 32 accumulates at most K / 16 + 32 roundings of partial sums bounded by sum |a b|:
+    E(A B) = 2 u (K / 16 + 32) |A| |B|
+  * exp(z - c) is off by the error of z, by 2 u |z - c| from the scaled argument and by 8 u of its own; sums of them by 64 u
+  * a bfloat16 G (the operand of two more products) is rounded by half a step, as is a bfloat16 result."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+from deepimpute_amd import _cabi, _lib  # noqa: E402
+
+U = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _products(K):
+    return 2 * U * (K / 16 + 32)
+
+
+def _problem(rows, width, classes, dtype, order="out_in", target="labels", seed=0, bias=True, ignored=True):
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1000 * seed + rows + 7 * width + 13 * classes)
+    n = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    x = n(rows, width).to(dtype)
+    kernel = (n(classes, width) * (2.0 / math.sqrt(width))).to(dtype)
+    kernel = kernel.t() if order == "out_in" else kernel.t().contiguous()
+    b = n(classes) * 0.5 if bias else None
+    u = torch.rand((rows,), generator=gen, device="cuda")
+    if target in ("labels", "labels64"):
+        t = (u * classes).long().clamp(max=classes - 1)
+        if ignored and rows > 2:
+            t[::5] = -1
+        t = t if target == "labels64" else t.int()
+    else:
+        t = torch.log1p(torch.floor(torch.exp(1.5 * n(rows, classes)))) / classes
+        t[:: 4] = 0 if rows > 2 else t[:: 4]                         # some rows without any target
+        t = t.to(torch.float32 if target == "profile" else torch.bfloat16)
+    dloss = (0.5 + torch.rand((rows,), generator=gen, device="cuda")) / rows
+    return x, kernel, t, b, dloss
+
+
+def _target64(t, classes):
+    if t.dim() == 2:
+        return t.double()
+    hot = torch.zeros((t.numel(), classes), dtype=torch.float64, device=t.device)
+    at = torch.nonzero(t >= 0).squeeze(1)
+    hot[at, t[at].long()] = 1.0
+    return hot
+
+
+def _reference(x, kernel, t, b, dloss=None):
+    """Everything in float64, with the room each result gets."""
+    X, W = x.double(), kernel.double()
+    H, V, N = W.shape[0], W.shape[1], X.shape[0]
+    z = X @ W + (0 if b is None else b.double())
+    ez = (_products(H) + 4 * U) * (X.abs() @ W.abs()) + 2 * U * z.abs()
+    lse = torch.logsumexp(z, 1)
+    T = _target64(t, V)
+    ts = T.sum(1)
+    masked = torch.where(T > 0, z, torch.zeros_like(z))
+    loss = ts * lse - (T * masked).sum(1)
+    fin = torch.where(torch.isfinite(ez), ez, torch.zeros_like(ez))
+    elog = fin.amax(1) + 2 * U * (72 + 2 * math.log(V) + lse.abs())
+    eloss = ts * elog + (T * fin).sum(1) + 2 * U * (V / 16 + 32 if t.dim() == 2 else 4) * (ts * lse.abs() + (T * masked).abs().sum(1))
+    out = dict(lse=(lse, elog), loss=(loss, eloss))
+    if dloss is None:
+        return out
+    d = dloss.double()[:, None]
+    p = torch.exp(z - lse[:, None])
+    G = d * (ts[:, None] * p - T)
+    eG = d * (ts[:, None] * p * (fin + elog[:, None] + 2 * U * (torch.where(torch.isfinite(z), (z - lse[:, None]).abs(), torch.zeros_like(z)) + 40 + (V / 64 + 8 if t.dim() == 2 else 0))) + 4 * U * T)
+    rounded = eG + (_half(torch.bfloat16) * G.abs() if x.dtype == torch.bfloat16 else 4 * U * G.abs())
+    h = _half(x.dtype)
+    dx, dW, db = G @ W.t(), X.t() @ G, G.sum(0)
+    out["dx"] = (dx, rounded @ W.abs().t() + (_products(V) + 4 * U) * (G.abs() @ W.abs().t()) + h * dx.abs())
+    out["dkernel"] = (dW, X.abs().t() @ rounded + (_products(N) + 4 * U) * (X.abs().t() @ G.abs()) + h * dW.abs())
+    out["dbias"] = (db, eG.sum(0) + 2 * U * (N / 2 + 32) * G.abs().sum(0))
+    return out
+
+
+def _close(name, got, want, room):
+    off = (got.double() - want).abs()
+    bad = ~(off <= room + 1e-30)
+    assert not bool(bad.any()), "%s: %d of %d off, by up to %.3g times the room" % (name, int(bad.sum()), bad.numel(), float((off / (room + 1e-30)).max()))
+
+
+def _check(rows, width, classes, dtype, order="out_in", target="labels", **kw):
+    from deepimpute_amd import ops
+    x, kernel, t, b, dloss = _problem(rows, width, classes, DTYPES[dtype], order, target, **kw)
+    loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+    ref = _reference(x, kernel, t, b, dloss)
+    _close("lse", lse, *ref["lse"])
+    _close("loss", loss, *ref["loss"])
+    dx, dk, db = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+    assert dx.shape == x.shape and dx.dtype == x.dtype and dk.shape == kernel.shape and dk.dtype == kernel.dtype and db.dtype == torch.float32
+    assert dk.stride() == kernel.stride() or min(kernel.shape) == 1
+    for name, got in (("dx", dx), ("dkernel", dk), ("dbias", db)):
+        _close(name, got, *ref[name])
+    if t.dim() == 1:
+        assert not bool(dx[t < 0].any()) and not bool(loss[t < 0].any())
+
+
+SIZES = [
+    (1, 1, 1), (1, 64, 2), (2, 3, 5), (3, 64, 100), (5, 65, 127), (16, 63, 128), (17, 128, 129), (63, 100, 255), (64, 256, 512), (65, 64, 257),
+    (127, 200, 300), (128, 192, 640), (130, 301, 1001), (256, 128, 256), (257, 64, 4097), (300, 1000, 77), (1000, 40, 3001),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("target", ["labels", "profile"])
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_sizes(dtype, order, target):
+    """One row, one class, one input; everything around the tiles' 64 / 128 / 256 and the steps of 64; both memory orders of the kernel."""
+    for rows, width, classes in SIZES:
+        print(dtype, order, target, rows, width, classes, flush=True)
+        _check(rows, width, classes, dtype, order, target, bias=classes % 3 != 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,classes,order,target", [
+    ("bf16", 1, 1024, 32000, "out_in", "labels"),
+    ("bf16", 1100, 512, 20011, "out_in", "labels64"),
+    ("bf16", 2048, 256, 50000, "in_out", "labels"),
+    ("f32", 64, 256, 20000, "in_out", "profile"),
+    ("f32", 700, 300, 9001, "out_in", "labels64"),
+    ("bf16", 999, 300, 20011, "in_out", "profile16"),
+    ("f32", 33, 2048, 5000, "out_in", "profile16"),
+])
+def test_large(dtype, rows, width, classes, order, target):
+    _check(rows, width, classes, dtype, order, target)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_strides(dtype):
+    """Row strides and base addresses of every remainder, a kernel that is a slice of a larger one in either order, a strided profile: the
+    values of contiguous copies."""
+    from deepimpute_amd import ops
+    dt = DTYPES[dtype]
+    x, kernel, t, b, dloss = _problem(50, 72, 333, dt, "in_out", "profile")
+    want = ops.linear_cross_entropy(x, kernel, t, b)
+    wgrad = ops.linear_cross_entropy_grad(dloss, x, kernel, t, want[1], b)
+    for pad, first in ((1, 0), (3, 1), (8, 5), (56, 8)):
+        xs = torch.full((50, 72 + pad + first), float("nan"), dtype=dt, device="cuda")
+        xs[:, first:first + 72] = x
+        ks = torch.full((72 + 2, 333 + pad + first), float("nan"), dtype=dt, device="cuda")
+        ks[1:73, first:first + 333] = kernel
+        kt = torch.full((333 + 1, 72 + pad + first), float("nan"), dtype=dt, device="cuda")
+        kt[1:, first:first + 72] = kernel.t()
+        ts = torch.full((50, 333 + pad + first), float("nan"), device="cuda")
+        ts[:, first:first + 333] = t
+        for k in (ks[1:73, first:first + 333], kt[1:, first:first + 72].t()):
+            a, tt = xs[:, first:first + 72], ts[:, first:first + 333]
+            got = ops.linear_cross_entropy(a, k, tt, b)
+            grad = ops.linear_cross_entropy_grad(dloss, a, k, tt, got[1], b)
+            for u, v in zip(got + grad, want + wgrad):
+                assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masks_and_odd_labels(dtype):
+    """Classes masked by a bias of -infinity or of the lowest float32, a masked label, rows with no class left, labels past the classes, huge logits."""
+    from deepimpute_amd import ops
+    dt = DTYPES[dtype]
+    inf = float("inf")
+    for classes in (40, 700):
+        x, kernel, t, _, dloss = _problem(70, 64, classes, dt, ignored=False)
+        b = torch.zeros(classes, device="cuda")
+        b[1::2] = -inf
+        t = t // 2 * 2                                               # labels that are there
+        t = t.clamp(max=classes - 2 if classes % 2 == 0 else classes - 1)
+        loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+        keep = list(range(0, classes, 2))
+        sub = kernel[:, keep].contiguous()
+        ref = _reference(x, sub, t // 2, None, dloss)
+        _close("lse", lse, *ref["lse"])
+        _close("loss", loss, *ref["loss"])
+        dx, dk, db = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+        _close("dx", dx, *ref["dx"])
+        _close("dkernel", dk[:, keep], *ref["dkernel"])
+        assert not bool(dk[:, 1::2].any()) and not bool(db[1::2].any())
+        low = torch.where(torch.isinf(b), torch.full_like(b, torch.finfo(torch.float32).min), b)
+        loss2, lse2 = ops.linear_cross_entropy(x, kernel, t, low)
+        assert torch.equal(loss2, loss) and torch.equal(lse2, lse)
+        # a masked label: probability 0
+        odd = torch.full_like(t, 1)
+        loss3, lse3 = ops.linear_cross_entropy(x, kernel, odd, b)
+        assert bool((loss3 == inf).all()) and torch.equal(lse3, lse)
+        g = ops.linear_cross_entropy_grad(dloss, x, kernel, odd, lse3, b)
+        assert all(bool(torch.isfinite(v).all()) for v in g)
+        # nothing left at all
+        none = torch.full_like(b, -inf)
+        loss4, lse4 = ops.linear_cross_entropy(x, kernel, t, none)
+        assert bool((lse4 == -inf).all()) and bool((loss4 == inf).all())
+        g = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse4, none)
+        assert all(bool(torch.isfinite(v).all()) for v in g)
+        # labels that are no classes: a loss that says so, no gradient, nothing out of bounds
+        bad = t.clone()
+        bad[3], bad[7], bad[9] = classes, 2 ** 31 - 1, -(2 ** 31)
+        loss5, lse5 = ops.linear_cross_entropy(x, kernel, bad, None)
+        assert bool(loss5[3].isnan()) and bool(loss5[7].isnan()) and float(loss5[9]) == 0 and int(loss5.isnan().sum()) == 2
+        dx, _, _ = ops.linear_cross_entropy_grad(dloss, x, kernel, bad, lse5, None)
+        assert not bool(dx[[3, 7, 9]].any())
+    x, kernel, t, b, dloss = _problem(20, 64, 300, dt, ignored=False)
+    loss, lse = ops.linear_cross_entropy(x * 1000, kernel, t, b)     # far over exp's range
+    ref = _reference(x * 1000, kernel, t, b)
+    _close("lse", lse, *ref["lse"])
+    _close("loss", loss, *ref["loss"])
+    x[5, 3] = float("nan")                                           # stays in its row
+    l2, s2 = ops.linear_cross_entropy(x, kernel, t, b)
+    assert bool(s2[5].isnan()) and int(s2.isnan().sum()) == 1
+    clean, _ = ops.linear_cross_entropy(torch.where(x.isnan(), torch.zeros_like(x), x), kernel, t, b)
+    rest = [r for r in range(20) if r != 5]
+    assert torch.equal(l2[rest], clean[rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("target", ["labels", "profile"])
+def test_gradient_against_differences(target):
+    """Central differences of sum(dloss * loss) of the float64 formula at the float32 point."""
+    from deepimpute_amd import ops
+    x, kernel, t, b, dloss = _problem(5, 6, 9, torch.float32, "in_out", target)
+    _, lse = ops.linear_cross_entropy(x, kernel, t, b)
+    grads = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+    T = _target64(t, 9)
+
+    def f(X, W, B):
+        z = X @ W + B
+        return float((dloss.double() * (T.sum(1) * torch.logsumexp(z, 1) - (T * z).sum(1))).sum())
+    point = [x.double(), kernel.double(), b.double()]
+    h = 1e-5
+    for i, g in enumerate(grads):
+        for at in np.ndindex(*point[i].shape):
+            v = []
+            for s in (h, -h):
+                q = [p.clone() for p in point]
+                q[i][at] += s
+                v.append(f(*q))
+            assert abs(float(g[at]) - (v[0] - v[1]) / (2 * h)) < 2e-6
+
+
+@pytest.mark.gpu
+def test_streams_graphs_and_repeats():
+    """On a side stream, two calls at once on two streams, captured and replayed with new inputs and eager work between: the same bits."""
+    from deepimpute_amd import ops
+    for target, dtype in (("labels", torch.bfloat16), ("profile", torch.float32)):
+        def both(x, kernel, t, b, dloss):
+            loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+            return (loss, lse) + ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+        args = _problem(200, 100, 1500, dtype, "in_out", target)
+        other = _problem(200, 100, 1500, dtype, "in_out", target, seed=3)
+        want, want2 = both(*args), both(*other)
+        for u, v in zip(both(*args), want):
+            assert torch.equal(u, v)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        got = []
+        for s, a in zip(streams, (args, other)):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(both(*a))
+        torch.cuda.synchronize()
+        for g, w in zip(got, (want, want2)):
+            for u, v in zip(g, w):
+                assert torch.equal(u, v)
+        held = [a.clone() for a in args]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(*held)
+        for k in range(4):
+            new = _problem(200, 100, 1500, dtype, "in_out", target, seed=10 + k)
+            for a, v in zip(held, new):
+                a.copy_(v)
+            graph.replay()
+            torch.cuda.synchronize()
+            for u, v in zip(out, both(*new)):
+                assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+def test_norm_and_loss_together():
+    """A normalised hidden layer in front of the output layer, forward and back through both operators, against autograd in float64."""
+    from deepimpute_amd import ops
+    x, kernel, t, b, dloss = _problem(150, 96, 777, torch.float32, "in_out", "labels")
+    x = 3 * x + 1
+    gamma, beta = torch.linspace(0.5, 1.5, 96, device="cuda"), torch.linspace(-1, 1, 96, device="cuda")
+    y, mean, rstd = ops.layer_norm(x, gamma, beta)
+    loss, lse = ops.linear_cross_entropy(y, kernel, t, b)
+    dy, dk, db = ops.linear_cross_entropy_grad(dloss, y, kernel, t, lse, b)
+    dx, dgamma, dbeta = ops.layer_norm_grad(dy, x, mean, rstd, gamma)
+    leaves = [v.double().cpu().requires_grad_() for v in (x, gamma, beta, kernel, b)]
+    X, g, c, K, B = leaves
+    m = X.mean(1, keepdim=True)
+    hat = (X - m) / torch.sqrt(((X - m) ** 2).mean(1, keepdim=True) + 1e-3)
+    z = (hat * g + c) @ K + B
+    T = _target64(t, 777).cpu()
+    total = (dloss.double().cpu() * (T.sum(1) * torch.logsumexp(z, 1) - (T * z).sum(1))).sum()
+    total.backward()
+    for got, leaf in zip((dx, dgamma, dbeta, dk, db), leaves):
+        w = leaf.grad
+        assert float((got.double().cpu() - w).norm()) <= 2e-5 * float(w.norm())      # 1e-6 of the operands' errors, amplified by at most 10 on either way
+
+
+def _describe(**kw):
+    base = dict(device_id=0, type=0, rows=4, width=8, classes=16, x=4096, x_row=8, kernel=4096, kernel_in=16, kernel_out=1, bias=None, target=4096,
+                target_row=0, target_kind=0)
+    base.update(kw)
+    return _cabi.OutputLoss(**base)
+
+
+def test_refusals_on_the_host():
+    """Refused before anything reaches a GPU (no GPU needed)."""
+    fns = _lib.load()
+    n = C.c_int64()
+
+    def refused(what, **kw):
+        d = _describe(**kw)
+        assert fns["linear_cross_entropy"](d, None, 4096, 4096, 4096, 1 << 40) < 0
+        assert what in fns["last_error"]().decode()
+        assert fns["linear_cross_entropy_grad"](d, None, 4096, 4096, 4096, 8, 4096, 16, 1, None, 4096, 1 << 40) < 0
+        assert what in fns["last_error"]().decode()
+        assert fns["linear_cross_entropy_workspace"](d, 1, n) < 0
+    refused("element type", type=5)
+    refused("target kind", target_kind=9)
+    refused("width 0", width=0)
+    refused("0 classes", classes=0)
+    refused("rows", rows=-1)
+    refused("rows", rows=1 << 30)
+    refused("strides", kernel_in=16, kernel_out=2)
+    refused("null", x=None)
+    refused("null", kernel=None)
+    refused("null", target=None)
+    refused("tiles", rows=1 << 22, classes=1 << 22)
+    assert fns["linear_cross_entropy"](None, None, 4096, 4096, 4096, 1) < 0
+    assert fns["linear_cross_entropy"](_describe(), None, None, 4096, 4096, 1) < 0 and b"null" in fns["last_error"]()
+    assert fns["linear_cross_entropy_grad"](_describe(), None, None, 4096, 4096, 8, 4096, 16, 1, None, 4096, 1) < 0 and b"null" in fns["last_error"]()
+    assert fns["linear_cross_entropy_grad"](_describe(), None, 4096, 4096, 4096, 8, 4096, 16, 3, None, 4096, 1) < 0 and b"dkernel" in fns["last_error"]()
+    assert fns["linear_cross_entropy"](_describe(rows=0), None, 4096, 4096, None, 0) == 0
+
+
+def test_refusals_of_tensors():
+    from deepimpute_amd import ops
+    x, k, t = torch.zeros((4, 8)), torch.zeros((8, 16)), torch.zeros(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.linear_cross_entropy(x, k, t)
+    with pytest.raises(ValueError, match="float32 or bfloat16"):
+        ops.linear_cross_entropy(x.half(), k.half(), t)
+    with pytest.raises(ValueError, match="the kernel"):
+        ops.linear_cross_entropy(x, k.bfloat16(), t)
+    with pytest.raises(ValueError, match="expected, got"):
+        ops.linear_cross_entropy(x, k.t(), t)
+    with pytest.raises(ValueError, match="bias has shape"):
+        ops.linear_cross_entropy(x, k, t, torch.zeros(15))
+    for bad in (torch.zeros(3, dtype=torch.int32), torch.zeros(4), torch.zeros((4, 15)), torch.zeros(4, dtype=torch.int16), torch.zeros((4, 16), dtype=torch.int32)):
+        with pytest.raises(ValueError, match="target must be"):
+            ops.linear_cross_entropy(x, k, bad)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    from deepimpute_amd import ops
+    fns = _lib.load()
+    x, kernel, t, b, dloss = _problem(8, 16, 20, torch.float32, "in_out")
+    out = torch.zeros((2, 8), device="cuda")
+    d, keep = ops._output_loss("test", x, kernel, t, b)
+    n = C.c_int64()
+    assert fns["linear_cross_entropy_workspace"](d, 0, n) == 0
+    work = torch.empty(n.value + 512, dtype=torch.uint8, device="cuda")
+    assert fns["linear_cross_entropy"](d, None, out[0].data_ptr(), out[1].data_ptr(), work.data_ptr(), n.value - 1) == -1 and b"workspace" in fns["last_error"]()
+    assert fns["linear_cross_entropy"](d, None, out[0].data_ptr(), out[1].data_ptr(), work.data_ptr() + 16, n.value) == -1
+    with pytest.raises(ValueError, match="lse has shape"):
+        ops.linear_cross_entropy_grad(dloss, x, kernel, t, dloss[:5], b)
+    with pytest.raises(ValueError, match="dloss must be float32"):
+        ops.linear_cross_entropy_grad(dloss.double(), x, kernel, t, dloss, b)
+    empty = ops.linear_cross_entropy(x[:0], kernel, t[:0], b)
+    assert empty[0].shape == (0,)
+    g = ops.linear_cross_entropy_grad(dloss[:0], x[:0], kernel, t[:0], dloss[:0], b)
+    assert g[0].shape == (0, 16) and not bool(g[1].any()) and not bool(g[2].any())
