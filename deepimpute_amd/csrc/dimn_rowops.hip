@@ -5,9 +5,11 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "dimn_norm.h"
 #include "dimn_xent.h"
+#include "dimn_xent_thin.h"
 
 #define HIPCHK(expr)                                                                            \
     do {                                                                                        \
@@ -29,8 +31,12 @@ int64_t ceil_div64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 struct OnDevice {
     int before = -1, now = -1;
     int enter(const char* who, int32_t device) {
-        int n = 0;
-        if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return dimn_fail(DIMN_ERR_HIP, "%s: no HIP device visible", who);
+        static std::atomic<int> known{0};                        // (a query of ~0.5 us per call; the number does not change while a process lives)
+        int n = known.load(std::memory_order_relaxed);
+        if (n == 0) {
+            if (hipGetDeviceCount(&n) != hipSuccess || n < 1) return dimn_fail(DIMN_ERR_HIP, "%s: no HIP device visible", who);
+            known.store(n, std::memory_order_relaxed);
+        }
         if (device < 0 || device >= n) return dimn_fail(DIMN_ERR_ARG, "%s: device_id %d out of range (%d devices)", who, device, n);
         HIPCHK(hipGetDevice(&before));
         now = device;
@@ -242,6 +248,7 @@ struct XentPlan {
     int t_logits;
     int64_t tiles_m, tiles_n;                 // logits
     int t_dx, splits;
+    bool thin; int nf; int64_t blocks;        // few rows: dimn_xent_thin.h; 16 nf rows per block
     size_t x, xt, w, wt, g, gt, part, part_t, picked, scale, tsum, dbias, acc, bytes;
 
     size_t take(int64_t n) { const size_t at = bytes; bytes += (size_t)up(n, 256); return at; }
@@ -270,6 +277,27 @@ struct XentPlan {
         tiles_m = ceil_div64(N, kTiles[t_logits].bm);
         tiles_n = ceil_div64(V, kTiles[t_logits].bn);
         bytes = 0;
+        // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.
+        thin = N <= 64 && V >= 4 && H >= 4;
+        if (thin) {
+            nf = N <= 16 ? 1 : (N <= 32 ? 2 : 4);
+            blocks = ceil_div64(N, 16 * nf);
+            tiles_n = ceil_div64(V, out_in ? 32 : 64);
+            if (!grad) {
+                part = take(8 * tiles_n * N);
+                part_t = labels ? 0 : take(8 * tiles_n * N);
+                picked = take(4 * N);
+                return;
+            }
+            g = take((f32 ? 4 : 2) * N * V);
+            scale = take(4 * N);
+            tsum = take(4 * N);
+            dbias = take(4 * blocks * V);
+            const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
+            splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, 2 * ncu / wgs, chunks / 2}));
+            acc = take(4 * (int64_t)splits * N * H);
+            return;
+        }
         x = x_direct ? 0 : take(2 * planes * N * Hp);
         w = w_direct ? 0 : take(2 * planes * P * Hp);
         if (!grad) {
@@ -340,6 +368,58 @@ void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& 
     p.class0 = c0; p.classes = q.V;
 }
 
+template <typename T, int EPI>
+void xent_thin(const XentPlan& q, bool vc, int64_t n, int splits, const rowops::Thin& p, hipStream_t st) {
+    const dim3 grid((unsigned)ceil_div64(n, vc ? 64 : 32), (unsigned)splits, (unsigned)q.blocks);
+#define THIN(NF)                                                                                                  \
+    do {                                                                                                          \
+        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin<T, true, NF, EPI>), grid, dim3(256), 0, st, p);           \
+        else hipLaunchKernelGGL((rowops::k_xent_thin<T, false, NF, EPI>), grid, dim3(256), 0, st, p);             \
+    } while (0)
+    if (q.nf == 1) THIN(1);
+    else if (q.nf == 2) THIN(2);
+    else THIN(4);
+#undef THIN
+}
+rowops::Thin xent_thin_logits(const XentPlan& q) {
+    const dimn_output_loss* d = q.d;
+    rowops::Thin p{};
+    p.A = d->x; p.lda = d->x_row;
+    p.B = d->kernel; p.ldb = q.out_in ? d->kernel_out : d->kernel_in;
+    p.M = q.N; p.N = q.V; p.K = q.H;
+    p.bias = d->bias; p.target = d->target; p.target_row = d->target_row; p.target_kind = d->target_kind;
+    return p;
+}
+// scale (and the sums of profiles) of every row
+void xent_rows(const XentPlan& q, const float* dloss, float* scale, float* tsum, hipStream_t st) {
+    const dimn_output_loss* d = q.d;
+    hipLaunchKernelGGL(rowops::k_xent_rows, dim3((unsigned)(q.labels ? ceil_div64(q.N, 1024) : q.N)), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.N, q.V, dloss, scale, tsum);
+}
+template <typename T>
+void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
+    const dimn_output_loss* d = q.d;
+    float *scale = (float*)(ws + q.scale), *tsum = (float*)(ws + q.tsum), *dbias_part = (float*)(ws + q.dbias), *acc = (float*)(ws + q.acc);
+    T* G = (T*)(ws + q.g);
+    xent_rows(q, dloss, scale, tsum, st);
+    rowops::Thin p = xent_thin_logits(q);
+    p.lse = lse; p.scale = scale; p.tsum = tsum;
+    p.G = G; p.ldg = q.V;
+    p.dbias_part = dbias ? (q.blocks == 1 ? dbias : dbias_part) : nullptr;
+    xent_thin<T, rowops::XE_GRAD>(q, !q.out_in, q.V, 1, p, st);
+    if (dbias && q.blocks > 1) hipLaunchKernelGGL(rowops::k_xent_dbias, dim3((unsigned)ceil_div64(q.V, 256)), dim3(256), 0, st, dbias_part, q.V, (int)q.blocks, q.V, dbias);
+    // dx[n][h] = sum over the classes: the classes are the inner dimension now
+    rowops::Thin a{};
+    a.A = G; a.lda = q.V; a.B = d->kernel; a.ldb = p.ldb;
+    a.M = q.N; a.N = q.H; a.K = q.V; a.acc = acc;
+    xent_thin<T, rowops::XE_ADD>(q, q.out_in, q.H, q.splits, a, st);
+    hipLaunchKernelGGL(rowops::k_xent_finish<T>, dim3((unsigned)ceil_div64(q.N * q.H, 256)), dim3(256), 0, st, acc, q.N * q.H, q.splits, q.N, q.H, (T*)dx, dx_row);
+    const bool oi = dk_in == 1;
+    const int64_t na = oi ? q.V : q.H, nb = oi ? q.H : q.V;
+    const dim3 grid((unsigned)ceil_div64(nb, 256), (unsigned)ceil_div64(na, 64));
+    if (oi) hipLaunchKernelGGL(rowops::k_xent_thin_dw<T>, grid, dim3(256), 0, st, G, q.V, (const T*)d->x, d->x_row, q.N, na, nb, (T*)dkernel, dk_out);
+    else hipLaunchKernelGGL(rowops::k_xent_thin_dw<T>, grid, dim3(256), 0, st, (const T*)d->x, d->x_row, G, q.V, q.N, na, nb, (T*)dkernel, dk_in);
+}
+
 int xent_check(const char* who, const dimn_output_loss* d) {
     if (!d) return dimn_fail(DIMN_ERR_ARG, "%s: null description", who);
     if (d->type != DIMN_TYPE_F32 && d->type != DIMN_TYPE_BF16) return dimn_fail(DIMN_ERR_UNSUP, "%s: element type %d (DIMN_TYPE_F32 or DIMN_TYPE_BF16)", who, d->type);
@@ -385,7 +465,14 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
     const Tile& t = kTiles[q.t_logits];
-    for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
+    if (q.thin) {
+        rowops::Thin p = xent_thin_logits(q);
+        p.part = (float2*)(ws + q.part);
+        p.part_t = q.labels ? nullptr : (float2*)(ws + q.part_t);
+        p.picked = (float*)(ws + q.picked);
+        if (q.f32) xent_thin<float, rowops::XE_LSE>(q, !q.out_in, q.V, 1, p, st);
+        else xent_thin<bf16_t, rowops::XE_LSE>(q, !q.out_in, q.V, 1, p, st);
+    } else for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
         XentGemm p;
         xent_logits(q, ws, c0, std::min(q.P, q.V - c0), p, st);
         p.part = (float2*)(ws + q.part) + c0 / t.bn * q.N;
@@ -400,7 +487,9 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     r.tiles = q.tiles_n; r.rows = q.N; r.classes = q.V;
     r.target = d->target; r.target_kind = d->target_kind;
     r.loss = loss; r.lse = lse;
-    hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, 64)), dim3(1024), 0, st, r);
+    r.per = 1;                                                   // few rows: more strands over the tiles each
+    while (r.per < 64 && 2 * r.per <= q.N) r.per *= 2;
+    hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, r.per)), dim3(1024), 0, st, r);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
 }
@@ -419,9 +508,15 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
     if (d->rows == 0) return dimn_fail(DIMN_ERR_ARG, "%s: no rows", who);
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
+    if (q.thin) {
+        if (q.f32) xent_thin_backward<float>(q, ws, dloss, lse, dx, dx_row, dkernel, dkernel_in, dkernel_out, dbias, st);
+        else xent_thin_backward<bf16_t>(q, ws, dloss, lse, dx, dx_row, dkernel, dkernel_in, dkernel_out, dbias, st);
+        HIPCHK(hipGetLastError());
+        return DIMN_OK;
+    }
     float* scale = (float*)(ws + q.scale);
     float* tsum = (float*)(ws + q.tsum);
-    hipLaunchKernelGGL(rowops::k_xent_rows, dim3((unsigned)(q.labels ? ceil_div64(q.N, 256) : q.N)), dim3(256), 0, st, d->target, d->target_kind, d->target_row, q.N, q.V, dloss, scale, tsum);
+    xent_rows(q, dloss, scale, tsum, st);
     uint16_t* xt = (uint16_t*)(ws + q.xt);
     const int64_t xt_plane = q.H * q.Np;
     xent_lay(q.f32, true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane, st);
@@ -466,7 +561,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         }
         xent_gemm<rowops::XE_STORE>(pick_tile(w.M, w.N, q.ncu), 1, w, st);
     }
-    const unsigned blocks = (unsigned)ceil_div64(q.N * q.H, 1024);
+    const unsigned blocks = (unsigned)ceil_div64(q.N * q.H, 256);
     if (q.f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (float*)dx, dx_row);
     else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (bf16_t*)dx, dx_row);
     if (dbias)

@@ -408,47 +408,48 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
     }
 }
 
-// loss and lse of every row from the partial sums of the class tiles.  grid ceil(rows / 64), 1024 threads: 64 rows x 16 strands of tiles.
+// (maximum, sum) of two disjoint sets of classes.  A set of NaNs has no maximum: its sum says so.
+__device__ __forceinline__ float2 join_lse(float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x);
+    if (top == -INFINITY) return make_float2(top, a.y + b.y);
+    return make_float2(top, a.y * (a.x == -INFINITY ? 1.f : __expf(a.x - top)) + b.y * (b.x == -INFINITY ? 1.f : __expf(b.x - top)));
+}
+
+// loss and lse of every row from the partial sums of the class tiles: 1024 threads, `per` rows (a power of two up to 64) x 1024 / per strands of tiles
 struct XentRows {
     const float2* part; const float2* part_t; const float* picked;
     int64_t tiles, rows, classes;
+    int32_t per;
     const void* target; int32_t target_kind;
     float* loss; float* lse;
 };
 __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
-    __shared__ float2 red[16][64];
-    __shared__ float2 red_t[16][64];
-    const int c = threadIdx.x & 63, strand = threadIdx.x >> 6;
-    const int64_t row = (int64_t)blockIdx.x * 64 + c;
-    float top = -INFINITY, s = 0.f;
-    float2 t = make_float2(0.f, 0.f);
+    __shared__ float2 red[1024], red_t[1024];
+    const int c = threadIdx.x & (p.per - 1), strands = 1024 / p.per, strand = threadIdx.x / p.per;
+    const int64_t row = (int64_t)blockIdx.x * p.per + c;
+    float2 v = make_float2(-INFINITY, 0.f), t = make_float2(0.f, 0.f);
     if (row < p.rows) {
 #pragma unroll 4
-        for (int64_t k = strand; k < p.tiles; k += 16) {
-            const float2 v = p.part[k * p.rows + row];
-            const float m = fmaxf(top, v.x);
-            if (m > -INFINITY) { s = s * __expf(top - m) + v.y * __expf(v.x - m); top = m; }
-            else if (v.y != v.y || v.x != v.x) s = NAN;          // a tile of NaNs has no maximum: its sum says so
+        for (int64_t k = strand; k < p.tiles; k += strands) v = join_lse(v, p.part[k * p.rows + row]);
+        if (p.part_t) {
+#pragma unroll 4
+            for (int64_t k = strand; k < p.tiles; k += strands) { const float2 u = p.part_t[k * p.rows + row]; t.x += u.x; t.y += u.y; }
         }
-        if (p.part_t)
-            for (int64_t k = strand; k < p.tiles; k += 16) { const float2 v = p.part_t[k * p.rows + row]; t.x += v.x; t.y += v.y; }
     }
-    red[strand][c] = make_float2(top, s);
-    red_t[strand][c] = t;
-    __syncthreads();
+    red[threadIdx.x] = v;
+    red_t[threadIdx.x] = t;
+    for (int half = strands / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (strand < half) {
+            v = join_lse(v, red[threadIdx.x + half * p.per]);
+            const float2 u = red_t[threadIdx.x + half * p.per];
+            t.x += u.x; t.y += u.y;
+            red[threadIdx.x] = v;
+            red_t[threadIdx.x] = t;
+        }
+    }
     if (strand != 0 || row >= p.rows) return;
-    top = -INFINITY; s = 0.f; t = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 16; ++w) top = fmaxf(top, red[w][c].x);
-    const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        const float2 v = red[w][c];
-        s += v.y * (v.x == -INFINITY ? 1.f : __expf(v.x - ref));
-        t.x += red_t[w][c].x;
-        t.y += red_t[w][c].y;
-    }
-    const float lse = top == -INFINITY && s == 0.f ? -INFINITY : ref + __logf(s);
+    const float lse = v.x == -INFINITY ? (v.y == 0.f ? -INFINITY : v.y) : v.x + __logf(v.y);
     p.lse[row] = lse;
     float loss;
     if (p.target_kind <= XT_I64) {
@@ -461,37 +462,56 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
 }
 
 // Backward, per row: scale = dloss, or 0 for a row without a target (label negative or not a class); tsum = the sum of its profile.
-__global__ __launch_bounds__(256) void k_xent_rows(const void* target, int32_t kind, int64_t target_row, int64_t rows, int64_t classes, const float* __restrict__ dloss,
+__global__ __launch_bounds__(1024) void k_xent_rows(const void* target, int32_t kind, int64_t target_row, int64_t rows, int64_t classes, const float* __restrict__ dloss,
                                                    float* __restrict__ scale, float* __restrict__ tsum) {
     if (kind <= XT_I64) {
-        const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        const int64_t row = (int64_t)blockIdx.x * 1024 + threadIdx.x;
         if (row >= rows) return;
         const int64_t y = kind == XT_I64 ? ((const int64_t*)target)[row] : (int64_t)((const int32_t*)target)[row];
         scale[row] = y >= 0 && y < classes ? dloss[row] : 0.f;
         return;
     }
     const int64_t row = blockIdx.x;                              // one workgroup per row
-    __shared__ float red[4];
+    __shared__ float red[16];
     float s = 0.f;
-    if (kind == XT_F32) { const float* t = (const float*)target + row * target_row; for (int64_t c = threadIdx.x; c < classes; c += 256) s += t[c]; }
-    else { const uint16_t* t = (const uint16_t*)target + row * target_row; for (int64_t c = threadIdx.x; c < classes; c += 256) s += from_bf16(t[c]); }
+    if (kind == XT_F32) {
+        const float* t = (const float*)target + row * target_row;
+#pragma unroll 4
+        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += 4096) {
+            if (c + 4 <= classes) { const f32x4u v = *(const f32x4u*)(t + c); s += (v[0] + v[1]) + (v[2] + v[3]); }
+            else for (int64_t k = c; k < classes; ++k) s += t[k];
+        }
+    } else {
+        const uint16_t* t = (const uint16_t*)target + row * target_row;
+#pragma unroll 4
+        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += 4096) {
+            if (c + 4 <= classes) { const u16x4u v = *(const u16x4u*)(t + c); s += (from_bf16(v[0]) + from_bf16(v[1])) + (from_bf16(v[2]) + from_bf16(v[3])); }
+            else for (int64_t k = c; k < classes; ++k) s += from_bf16(t[k]);
+        }
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    if (threadIdx.x == 0) { tsum[row] = (red[0] + red[1]) + (red[2] + red[3]); scale[row] = dloss[row]; }
+    if (threadIdx.x == 0) {
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) s += red[w];
+        tsum[row] = s;
+        scale[row] = dloss[row];
+    }
 }
 
-// out[m][n] = sum of the splits' float32 sums, rounded once.  256 threads, four elements each.
+// out[m][n] = sum of the splits' float32 sums, in order, rounded once.  A thread takes one element: neighbours are neighbours in every split.
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ acc, int64_t split, int splits, int64_t rows, int64_t cols, T* __restrict__ out, int64_t ld) {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, total = rows * cols;
-    for (int r = 0; r < 4 && e + r < total; ++r) {
-        float s = 0.f;
-        for (int k = 0; k < splits; ++k) s += acc[k * split + e + r];
-        const int64_t m = (e + r) / cols, n = e + r - m * cols;
-        if constexpr (sizeof(T) == 4) out[m * ld + n] = s; else out[m * ld + n] = to_bf16(s);
-    }
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= rows * cols) return;
+    float s = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += acc[k * split + e];
+    const int64_t m = e / cols, n = e - m * cols;
+    if constexpr (sizeof(T) == 4) out[m * ld + n] = s; else out[m * ld + n] = to_bf16(s);
 }
 
 // dbias = the partial column sums, added in order

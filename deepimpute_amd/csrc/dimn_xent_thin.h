@@ -1,0 +1,333 @@
+// dimn_xent_thin.h -- the products of dimn_xent.h for few rows (gfx950): one pass over the kernel, operands in the caller's own layout.
+//
+// With few rows the logits, dx and dW are bound by reading (or writing) the kernel once, and what dimn_xent.h does first -- laying the operands
+// out as k-contiguous bfloat16 planes -- costs more than the products: for float32 it moves 16 bytes per weight where 4 have to be read.  Here
+// the matrix instructions take their operands straight from global memory, in whichever order the caller holds the kernel:
+//   * k-contiguous (KC): a lane loads 16 bytes of one class row; float32: element r feeds instruction r (any assignment of k's to the slots of
+//     v_mfma_f32_16x16x4_f32 gives the same sum as long as the rows' operand follows it); bfloat16: the eight k's of one 16x16x32 instruction.
+//   * class-contiguous (VC): a lane loads four consecutive classes of one k; element j belongs to class set j, whose sixteen classes lie four
+//     apart -- a permutation of the classes inside the workgroup's 64 that the epilogue undoes.
+// float32 runs on the exact float32 matrix instructions: at 64 rows their rate (154 TFLOP/s measured) and the HBM's meet.
+// A workgroup owns 32 (KC) / 64 (VC) classes x up to 64 rows; its four waves take every fourth chunk of k and are added through LDS in the
+// fixed order (w0 + w2) + (w1 + w3), so also a small problem keeps four waves per 32 classes busy.
+#pragma once
+#include "dimn_xent.h"
+
+namespace rowops {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x8u __attribute__((ext_vector_type(8), aligned(2)));
+
+struct Thin {
+    const void* A; int64_t lda;                // [M][K], k-contiguous
+    const void* B; int64_t ldb;                // KC: [N][K]; VC: [K][N]
+    int64_t M, N, K;
+    const float* bias;                         // [N] or NULL
+    const void* target; int64_t target_row; int32_t target_kind;
+    float2* part; float2* part_t; float* picked;          // as XentGemm (a tile: 32 / 64 classes)
+    const float* lse; const float* scale; const float* tsum;
+    void* G; int64_t ldg;                      // [M][ldg] of T
+    float* dbias_part;                         // [gridDim.z][N]
+    float* acc;                                // XE_ADD: [gridDim.y][M][N] float32
+};
+
+template <typename T> struct Four;             // four consecutive elements of a class row (VC)
+template <> struct Four<float> { typedef f32x4u vec; };
+template <> struct Four<bf16_t> { typedef u16x4u vec; };
+
+template <typename T, bool VC, int NF, int EPI>
+__global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
+    constexpr bool BF = sizeof(T) == 2, WIDE = BF && !VC;      // WIDE: the 16x16x32 instruction, eight k's per lane
+    constexpr int EL = WIDE ? 8 : 4, KS = 4 * EL, NS = VC ? 4 : 2, CW = VC ? 64 : 32, ROWS = 16 * NF, LD = CW + 4;
+    constexpr int U = NF > 2 ? 2 : 4;                           // chunks requested together
+    __shared__ __attribute__((aligned(16))) float red[2][ROWS][LD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lj = lane >> 4;
+    const int64_t c0 = (int64_t)blockIdx.x * CW, m0 = (int64_t)blockIdx.z * ROWS;
+    const T* A = (const T*)p.A;
+    const T* B = (const T*)p.B;
+    const T* arow[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        int64_t m = m0 + 16 * f + li;
+        m = m < p.M ? m : p.M - 1;                              // rows and classes past the end repeat the last one: never stored
+        arow[f] = A + m * p.lda;
+    }
+    const T* bptr[VC ? 1 : 2];
+    if constexpr (VC) {
+        const int64_t c = c0 + 4 * li;
+        bptr[0] = B + (c < p.N - 4 ? c : p.N - 4);              // (N >= 4: the caller's rule)
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int64_t c = c0 + 16 * s + li;
+            bptr[s] = B + (c < p.N ? c : p.N - 1) * p.ldb;
+        }
+    }
+    typedef typename std::conditional<BF, typename std::conditional<WIDE, u16x8u, u16x4u>::type, f32x4u>::type avec;
+    typedef typename std::conditional<VC, typename Four<T>::vec, avec>::type bvec;
+    constexpr int NB = VC ? 4 : 2;
+    avec a[U][NF];
+    bvec b[U][NB];
+    f32x4 acc[NF][NS];
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) acc[f][s] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto request = [&](int64_t k, avec (&ra)[NF], bvec (&rb)[NB]) {
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+            if constexpr (VC) rb[q] = *(const bvec*)(bptr[0] + (k + 4 * lj + q) * p.ldb);
+            else rb[q] = *(const bvec*)(bptr[q] + k + EL * lj);
+        }
+#pragma unroll
+        for (int f = 0; f < NF; ++f) ra[f] = *(const avec*)(arow[f] + k + EL * lj);
+    };
+    auto multiply = [&](const avec (&ra)[NF], const bvec (&rb)[NB]) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+                    acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, rb[s]), __builtin_bit_cast(bf8, ra[f]), acc[f][s], 0, 0, 0);
+        } else if constexpr (BF) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const s16x4 w = {(short)rb[0][s], (short)rb[1][s], (short)rb[2][s], (short)rb[3][s]};
+#pragma unroll
+                for (int f = 0; f < NF; ++f) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(w, __builtin_bit_cast(s16x4, ra[f]), acc[f][s], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int f = 0; f < NF; ++f)
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) acc[f][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(VC ? rb[r][s] : rb[s][r], ra[f][r], acc[f][s], 0, 0, 0);
+        }
+    };
+    // this workgroup's range of whole chunks; the chunk that crosses K belongs to the last range
+    const int64_t whole = p.K / KS, S = gridDim.y;
+    const int64_t cbeg = whole * blockIdx.y / S, cend = whole * (blockIdx.y + 1) / S;
+    int64_t c = cbeg + wave;
+    for (; c + 4 * (U - 1) < cend; c += 4 * U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) request((c + 4 * u) * KS, a[u], b[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
+    }
+    for (; c < cend; c += 4) { request(c * KS, a[0], b[0]); multiply(a[0], b[0]); }
+    if (whole * KS < p.K && blockIdx.y == S - 1 && wave == (whole & 3)) {
+        const int64_t k = whole * KS;
+#pragma unroll
+        for (int q = 0; q < NB; ++q)
+#pragma unroll
+            for (int i = 0; i < (VC ? 4 : EL); ++i) {
+                if constexpr (VC) b[0][q][i] = k + 4 * lj + q < p.K ? bptr[0][(k + 4 * lj + q) * p.ldb + i] : (T)0;
+                else b[0][q][i] = k + EL * lj + i < p.K ? bptr[q][k + EL * lj + i] : (T)0;
+            }
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int i = 0; i < EL; ++i) a[0][f][i] = k + EL * lj + i < p.K ? arow[f][k + EL * lj + i] : (T)0;
+        multiply(a[0], b[0]);
+    }
+    // element r of acc[f][s]: row 16 f + li, position 16 s + 4 lj + r (KC) / 4 (4 lj + r) + s (VC) of the workgroup's classes
+    auto put = [&](int slot) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int q = 0; q < NS; ++q) {
+                if constexpr (VC) *(f32x4*)&red[slot][16 * f + li][16 * lj + 4 * q] = (f32x4){acc[f][0][q], acc[f][1][q], acc[f][2][q], acc[f][3][q]};
+                else *(f32x4*)&red[slot][16 * f + li][16 * q + 4 * lj] = acc[f][q];
+            }
+    };
+    if (wave >= 2) put(wave - 2);
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int f = 0; f < NF; ++f)
+#pragma unroll
+            for (int q = 0; q < NS; ++q) {
+                if constexpr (VC) {
+                    const f32x4 t = *(const f32x4*)&red[wave][16 * f + li][16 * lj + 4 * q];
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) acc[f][s][q] += t[s];
+                } else acc[f][q] += *(const f32x4*)&red[wave][16 * f + li][16 * q + 4 * lj];
+            }
+    }
+    __syncthreads();
+    if (wave < 2) put(wave);
+    __syncthreads();
+    // PT threads per row, CPT consecutive positions each
+    constexpr int PT = 256 / ROWS, CPT = CW / PT;
+    const int row = tid / PT, pos0 = (tid % PT) * CPT;
+    const int64_t m = m0 + row;
+    const bool have = m < p.M;
+    // class of a position, and whether this workgroup answers for it
+    auto cls = [&](int pos, bool& mine) -> int64_t {
+        if constexpr (VC) {
+            const int64_t from = c0 + (pos & ~3), start = from < p.N - 4 ? from : p.N - 4, k = start + (pos & 3);
+            mine = k >= from;
+            return k;
+        } else { mine = c0 + pos < p.N; return c0 + pos; }
+    };
+    if constexpr (EPI == XE_ADD) {
+        if (!have) return;
+        float* to = p.acc + ((int64_t)blockIdx.y * p.M + m) * p.N;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+            bool mine;
+            const int64_t k = cls(pos0 + i, mine);
+            if (mine) to[k] = red[0][row][pos0 + i] + red[1][row][pos0 + i];
+        }
+        return;
+    }
+    const bool labels = p.target_kind <= XT_I64;
+    int64_t y = -1;
+    if (labels && have) y = p.target_kind == XT_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
+    float z[CPT], t[CPT];
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+        bool mine;
+        const int64_t k = cls(pos0 + i, mine);
+        z[i] = red[0][row][pos0 + i] + red[1][row][pos0 + i] + (p.bias && mine ? p.bias[k] : 0.f);
+        t[i] = 0.f;
+        if (!labels && have && mine)
+            t[i] = p.target_kind == XT_F32 ? ((const float*)p.target)[m * p.target_row + k] : from_bf16(((const uint16_t*)p.target)[m * p.target_row + k]);
+    }
+    if constexpr (EPI == XE_LSE) {
+        float top = -INFINITY, s = 0.f, st = 0.f, stz = 0.f;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+            bool mine;
+            const int64_t k = cls(pos0 + i, mine);
+            if (mine) top = fmaxf(top, z[i]);
+            if (labels && mine && k == y) p.picked[m] = z[i];
+            st += t[i];
+            stz += t[i] != 0.f ? t[i] * z[i] : 0.f;
+        }
+#pragma unroll
+        for (int o = 1; o < PT; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+            bool mine;
+            cls(pos0 + i, mine);
+            if (mine) s += BF ? __expf(z[i] - ref) : expf(z[i] - ref);
+        }
+#pragma unroll
+        for (int o = 1; o < PT; o <<= 1) { s += __shfl_xor(s, o); st += __shfl_xor(st, o); stz += __shfl_xor(stz, o); }
+        if (have && tid % PT == 0) {
+            const int64_t at = (int64_t)blockIdx.x * p.M + m;
+            p.part[at] = make_float2(top, s);
+            if (!labels) p.part_t[at] = make_float2(st, stz);
+        }
+    } else {
+        const float lse = have ? p.lse[m] : 0.f, d = have ? p.scale[m] : 0.f, ts = labels ? 1.f : (have ? p.tsum[m] : 0.f);
+        T* G = (T*)p.G + m * p.ldg;
+        __syncthreads();                                        // the products have been read: the first slot takes G for the sums over the rows
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+            bool mine;
+            const int64_t k = cls(pos0 + i, mine);
+            const float e = z[i] == -INFINITY ? 0.f : (BF ? __expf(z[i] - lse) : expf(z[i] - lse));
+            const float hot = labels ? (k == y ? 1.f : 0.f) : t[i];
+            const float g = d != 0.f ? d * (ts * e - hot) : 0.f;
+            red[0][row][pos0 + i] = g;
+            if (have && mine) { if constexpr (BF) G[k] = to_bf16(g); else G[k] = g; }
+        }
+        if (!p.dbias_part) return;
+        __syncthreads();
+        constexpr int ST = 256 / CW;                            // strands of rows per class
+        const int pos = tid % CW, strand = tid / CW;
+        float s = 0.f;
+        for (int r = strand; r < ROWS; r += ST) s += red[0][r][pos];
+        __syncthreads();
+        red[1][strand][pos] = s;
+        __syncthreads();
+        if (strand == 0) {
+            bool mine;
+            const int64_t k = cls(pos, mine);
+#pragma unroll
+            for (int w = 1; w < ST; ++w) s += red[1][w][pos];
+            if (mine) p.dbias_part[(int64_t)blockIdx.z * p.N + k] = s;
+        }
+    }
+}
+
+// dW for few rows: C[a][b] = sum_n P[n][a] Q[n][b], both operands with their output index contiguous, C's b contiguous (Keras order: P = x, Q = G;
+// the transposed order: P = G, Q = x).  Writing C bounds it.  A wave owns 64 x 64 of C: a lane loads four consecutive a's and b's of one n, element
+// j belongs to set j (sixteen indices four apart) -- sixteen instructions per pair of 16-byte loads, and a lane ends up with four consecutive b's.
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_thin_dw(const T* __restrict__ P, int64_t ldp, const T* __restrict__ Q, int64_t ldq, int64_t n, int64_t na, int64_t nb,
+                                                      T* __restrict__ C, int64_t ldc) {
+    constexpr bool BF = sizeof(T) == 2;
+    typedef typename Four<T>::vec vec;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lj = lane >> 4;
+    const int64_t a0 = (int64_t)blockIdx.y * 64, b0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
+    if (b0 >= nb) return;
+    auto start = [](int64_t from, int64_t end) { return from < end - 4 ? from : end - 4; };      // (na, nb >= 4: the caller's rule)
+    const int64_t ca = start(a0 + 4 * li, na), cb = start(b0 + 4 * li, nb);
+    f32x4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const vec zero = {0, 0, 0, 0};
+    if constexpr (BF) {
+        for (int64_t k = 0; k < n; k += 16) {
+            vec a[4], b[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t row = k + 4 * lj + r;
+                a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
+                b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const s16x4 u = {(short)a[0][i], (short)a[1][i], (short)a[2][i], (short)a[3][i]};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const s16x4 v = {(short)b[0][j], (short)b[1][j], (short)b[2][j], (short)b[3][j]};
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(u, v, acc[i][j], 0, 0, 0);
+                }
+            }
+        }
+    } else {
+        for (int64_t k = 0; k < n; k += 16) {
+            vec a[4], b[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t row = k + 4 * r + lj;
+                a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
+                b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][i], b[r][j], acc[i][j], 0, 0, 0);
+        }
+    }
+    // acc[i][j][r]: a = set i of lane 4 lj + r, b = set j of lane li
+    const bool whole = cb == b0 + 4 * li;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int64_t from = a0 + 4 * (4 * lj + r), at = start(from, na);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (at + i < from) continue;
+            T* to = C + (at + i) * ldc + cb;
+            vec o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { if constexpr (BF) o[j] = to_bf16(acc[i][j][r]); else o[j] = acc[i][j][r]; }
+            if (whole) *(vec*)to = o;
+            else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (cb + j >= b0 + 4 * li) to[j] = o[j];
+        }
+    }
+}
+
+}  // namespace rowops

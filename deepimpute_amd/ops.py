@@ -46,8 +46,8 @@ def _device(what, x, *others):
     return dev.index
 
 
-def _stream(index):
-    return torch.cuda.current_stream(index).cuda_stream
+# handle of torch's current stream on a device; the raw query when torch has it (0.1 us instead of 1.1 us per call)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _type(what, x):
@@ -109,7 +109,7 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-3):
     if not eps >= 0:
         raise ValueError("layer_norm: eps %r is negative or not a number" % (eps,))
     shape, width = x.shape, x.shape[-1]
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = torch.empty((2,) + shape[:-1], dtype=torch.float32, device=x.device)
     mean, rstd = stats.unbind(0)
     x, groups, rows, xg, xr = _planes(x, grouped)
@@ -131,7 +131,7 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None):
     shape, width = x.shape, x.shape[-1]
     mean, rstd = _f32(what, "mean", mean, shape[:-1]), _f32(what, "rstd", rstd, shape[:-1])
     dev = _device(what, x, dy, mean, rstd, gamma)
-    dx = torch.empty(shape, dtype=x.dtype, device=x.device)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     x, groups, rows, xg, xr = _planes(x, grouped)
     dy, _, _, dg, dr = _planes(dy, grouped)
     key = (dev, kind, groups, rows, width)

@@ -143,29 +143,32 @@ def test_large(dtype, rows, width, classes, order, target):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [50, 150])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-def test_strides(dtype):
+def test_strides(dtype, rows):
     """Row strides and base addresses of every remainder, a kernel that is a slice of a larger one in either order, a strided profile: the
-    values of contiguous copies."""
+    bits of contiguous copies in the same memory order (the two orders may add in another order: test_sizes bounds both)."""
     from deepimpute_amd import ops
     dt = DTYPES[dtype]
-    x, kernel, t, b, dloss = _problem(50, 72, 333, dt, "in_out", "profile")
-    want = ops.linear_cross_entropy(x, kernel, t, b)
-    wgrad = ops.linear_cross_entropy_grad(dloss, x, kernel, t, want[1], b)
+    x, kernel, t, b, dloss = _problem(rows, 72, 333, dt, "in_out", "profile")
+    wants = []
+    for k in (kernel, kernel.t().contiguous().t()):
+        want = ops.linear_cross_entropy(x, k, t, b)
+        wants.append(want + ops.linear_cross_entropy_grad(dloss, x, k, t, want[1], b))
     for pad, first in ((1, 0), (3, 1), (8, 5), (56, 8)):
-        xs = torch.full((50, 72 + pad + first), float("nan"), dtype=dt, device="cuda")
+        xs = torch.full((rows, 72 + pad + first), float("nan"), dtype=dt, device="cuda")
         xs[:, first:first + 72] = x
         ks = torch.full((72 + 2, 333 + pad + first), float("nan"), dtype=dt, device="cuda")
         ks[1:73, first:first + 333] = kernel
         kt = torch.full((333 + 1, 72 + pad + first), float("nan"), dtype=dt, device="cuda")
         kt[1:, first:first + 72] = kernel.t()
-        ts = torch.full((50, 333 + pad + first), float("nan"), device="cuda")
+        ts = torch.full((rows, 333 + pad + first), float("nan"), device="cuda")
         ts[:, first:first + 333] = t
-        for k in (ks[1:73, first:first + 333], kt[1:, first:first + 72].t()):
+        for k, want in zip((ks[1:73, first:first + 333], kt[1:, first:first + 72].t()), wants):
             a, tt = xs[:, first:first + 72], ts[:, first:first + 333]
             got = ops.linear_cross_entropy(a, k, tt, b)
             grad = ops.linear_cross_entropy_grad(dloss, a, k, tt, got[1], b)
-            for u, v in zip(got + grad, want + wgrad):
+            for u, v in zip(got + grad, want):
                 assert torch.equal(u, v)
 
 
