@@ -249,8 +249,39 @@ struct XentPlan {
     int64_t tiles_m, tiles_n;                 // logits
     int t_dx, splits;
     bool thin; int nf; int64_t blocks;        // few rows: dimn_xent_thin.h; 16 nf rows per block
-    size_t x, xt, w, wt, g, gt, part, part_t, picked, scale, tsum, dbias, acc, bytes;
+    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, dbias, acc, bytes;
 
+    // The largest piece allowed, or a smaller one whose 256 x 256 tiles fill the device in whole rounds: a piece of 84 class tiles at 16 row tiles
+    // takes 6 rounds of 256 workgroups where 96 class tiles take the same six (64000 classes: 16 rounds instead of 18, 8 instead of 9 for dW).
+    int64_t best_piece(int64_t most) const {
+        const int64_t tm = ceil_div64(N, 256), th = ceil_div64(H, 256);
+        auto rounds = [&](int64_t tiles) { return ceil_div64(tiles, ncu); };
+        auto cost = [&](int64_t tiles_v) { return (double)rounds(tiles_v * tm) * H + (grad ? (double)rounds(tiles_v * th) * N : 0.0); };
+        const int64_t all = ceil_div64(V, 256), top = most / 256;
+        int64_t best = top;
+        double least = 1e300;
+        for (int64_t t = top; t >= 1 && t >= top / 4; --t) {
+            const int64_t full = all / t, rest = all - full * t;
+            const double c = full * cost(t) + (rest ? cost(rest) : 0.0) + 2e-3 * (double)ncu * (full + (rest ? 1 : 0));
+            if (c < least) { least = c; best = t; }
+        }
+        return best * 256;
+    }
+    // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 256 .. 4096 and 300 .. 32000
+    // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles)
+    bool prefers_thin() const {
+        const double hv = (double)H * (double)V, work = hv * (double)N, steps = 0.5 * segments * (double)(Hp / 64);
+        double t, g;
+        if (!grad) {
+            t = work * (f32 ? 25e-6 : 10.5e-6) * 1e-3;
+            g = (x_direct ? 0 : 5) + (w_direct ? 0 : 5 + hv * (f32 ? 3.9e-6 : 0.9e-6));
+            g += std::max(work * (f32 ? 8e-6 : 2.1e-6) * 1e-3, steps) - 4;
+        } else {
+            t = work * (f32 ? 68e-6 : 24e-6) * 1e-3 + 0.03 * (double)N;
+            g = 30 + hv * (f32 ? 10e-6 : 2e-6) + std::max(work * (f32 ? 40e-6 : 8.6e-6) * 1e-3, steps);
+        }
+        return t < g;
+    }
     size_t take(int64_t n) { const size_t at = bytes; bytes += (size_t)up(n, 256); return at; }
     void make(const dimn_output_loss* desc, bool with_grad, int compute_units) {
         d = desc; grad = with_grad; ncu = compute_units;
@@ -271,18 +302,20 @@ struct XentPlan {
         const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0));
         const int64_t budget = (int64_t)512 << 20;
         P = per_class ? std::max<int64_t>(256, budget / per_class / 256 * 256) : up(V, 256);
-        P = std::min(P, far);
-        P = up(ceil_div64(V, ceil_div64(V, P)), 256);
+        P = std::min(std::min(P, far), up(V, 256));
+        if (P < V && !w_direct) P = best_piece(P);
+        else if (P < V && grad) P = best_piece(P);
         t_logits = pick_tile(N, std::min(P, V), ncu);
         tiles_m = ceil_div64(N, kTiles[t_logits].bm);
         tiles_n = ceil_div64(V, kTiles[t_logits].bn);
         bytes = 0;
         // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.
-        thin = N <= 64 && V >= 4 && H >= 4;
+        thin = V >= 4 && H >= 4 && prefers_thin();
         if (thin) {
-            nf = N <= 16 ? 1 : (N <= 32 ? 2 : 4);
-            blocks = ceil_div64(N, 16 * nf);
+            // 64 rows per block read the kernel least often, 32 give twice the workgroups (and, class-contiguous float32, half the registers)
             tiles_n = ceil_div64(V, out_in ? 32 : 64);
+            nf = N <= 16 ? 1 : (N <= 32 || (f32 && !out_in) || tiles_n * ceil_div64(N, 64) < 2 * ncu ? 2 : 4);
+            blocks = ceil_div64(N, 16 * nf);
             if (!grad) {
                 part = take(8 * tiles_n * N);
                 part_t = labels ? 0 : take(8 * tiles_n * N);
@@ -290,7 +323,6 @@ struct XentPlan {
                 return;
             }
             g = take((f32 ? 4 : 2) * N * V);
-            scale = take(4 * N);
             tsum = take(4 * N);
             dbias = take(4 * blocks * V);
             const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
@@ -310,12 +342,20 @@ struct XentPlan {
         wt = wt_direct ? 0 : take(2 * planes * H * P);
         g = take(2 * planes * N * P);
         gt = take(2 * planes * P * Np);
-        scale = take(4 * N);
         tsum = take(4 * N);
         dbias = take(4 * tiles_m * kTiles[t_logits].wm * V);
-        t_dx = pick_tile(N, H, ncu);
+        // dx has few tiles and a long inner dimension: ranges of it, each with float32 sums of its own
         const int64_t steps = ceil_div64(std::min(P, V), 64) * segments;
-        splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)16, ncu / tile_count(kTiles[t_dx], N, H), steps / 8}));
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, steps / 8));
+        t_dx = N <= 64 ? 2 : (tile_count(kTiles[0], N, H) * std::min<int64_t>(most, 4) >= ncu * 3 / 4 ? 0 : 1);
+        const int64_t tiles = tile_count(kTiles[t_dx], N, H);
+        // a split's rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.3 per step of a 256 / 128 tile, 4 TB/s)
+        double least = 1e300;
+        splits = 1;
+        for (int64_t k = 1; k <= most; ++k) {
+            const double c = (double)ceil_div64(tiles * k, ncu) * (double)steps / (double)k * (t_dx == 0 ? 0.9 : 0.3) + (double)(k * N * H) * 8 / 4e6;
+            if (c < least) { least = c; splits = (int)k; }
+        }
         acc = take(4 * (int64_t)splits * N * H);
     }
 };
@@ -326,20 +366,26 @@ void xent_gemm(int tile, int splits, XentGemm& p, hipStream_t st) {
     p.tiles_m = (int)ceil_div64(p.M, t.bm);
     p.tiles_n = (int)ceil_div64(p.N, t.bn);
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)splits);
-    if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 256, 2, 4, EPI>), grid, dim3(512), 0, st, p);
-    else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI>), grid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI>), grid, dim3(256), 0, st, p);
+#define GEMM(PL)                                                                                                                  \
+    do {                                                                                                                          \
+        if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 256, 2, 4, EPI, PL>), grid, dim3(512), 0, st, p);             \
+        else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI, PL>), grid, dim3(256), 0, st, p);        \
+        else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI, PL>), grid, dim3(256), 0, st, p);                        \
+    } while (0)
+    if (p.segments > 1) GEMM(3);
+    else GEMM(1);
+#undef GEMM
 }
 
 // to[plane][rows][ldk] from a plane of the caller; transposed: the caller's memory runs along the rows
 void xent_lay(bool f32, bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane, hipStream_t st) {
-    const dim3 grid((unsigned)(ceil_div64(rows, 64) * (ldk / 64)));
+    const dim3 tiles((unsigned)(ceil_div64(rows, 64) * (ldk / 64))), flat((unsigned)ceil_div64(rows * ldk, 2048));
     if (f32) {
-        if (transposed) hipLaunchKernelGGL((rowops::k_xent_lay<float, true>), grid, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
-        else hipLaunchKernelGGL((rowops::k_xent_lay<float, false>), grid, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
+        if (transposed) hipLaunchKernelGGL(rowops::k_xent_lay_t<float>, tiles, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
+        else hipLaunchKernelGGL(rowops::k_xent_lay<float>, flat, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
     } else {
-        if (transposed) hipLaunchKernelGGL((rowops::k_xent_lay<bf16_t, true>), grid, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
-        else hipLaunchKernelGGL((rowops::k_xent_lay<bf16_t, false>), grid, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
+        if (transposed) hipLaunchKernelGGL(rowops::k_xent_lay_t<bf16_t>, tiles, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
+        else hipLaunchKernelGGL(rowops::k_xent_lay<bf16_t>, flat, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
     }
 }
 
@@ -390,19 +436,18 @@ rowops::Thin xent_thin_logits(const XentPlan& q) {
     p.bias = d->bias; p.target = d->target; p.target_row = d->target_row; p.target_kind = d->target_kind;
     return p;
 }
-// scale (and the sums of profiles) of every row
-void xent_rows(const XentPlan& q, const float* dloss, float* scale, float* tsum, hipStream_t st) {
+void xent_tsum(const XentPlan& q, float* tsum, hipStream_t st) {
     const dimn_output_loss* d = q.d;
-    hipLaunchKernelGGL(rowops::k_xent_rows, dim3((unsigned)(q.labels ? ceil_div64(q.N, 1024) : q.N)), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.N, q.V, dloss, scale, tsum);
+    if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
 }
 template <typename T>
 void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
     const dimn_output_loss* d = q.d;
-    float *scale = (float*)(ws + q.scale), *tsum = (float*)(ws + q.tsum), *dbias_part = (float*)(ws + q.dbias), *acc = (float*)(ws + q.acc);
+    float *tsum = (float*)(ws + q.tsum), *dbias_part = (float*)(ws + q.dbias), *acc = (float*)(ws + q.acc);
     T* G = (T*)(ws + q.g);
-    xent_rows(q, dloss, scale, tsum, st);
+    xent_tsum(q, tsum, st);
     rowops::Thin p = xent_thin_logits(q);
-    p.lse = lse; p.scale = scale; p.tsum = tsum;
+    p.lse = lse; p.dloss = dloss; p.tsum = tsum;
     p.G = G; p.ldg = q.V;
     p.dbias_part = dbias ? (q.blocks == 1 ? dbias : dbias_part) : nullptr;
     xent_thin<T, rowops::XE_GRAD>(q, !q.out_in, q.V, 1, p, st);
@@ -411,8 +456,13 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     rowops::Thin a{};
     a.A = G; a.lda = q.V; a.B = d->kernel; a.ldb = p.ldb;
     a.M = q.N; a.N = q.H; a.K = q.V; a.acc = acc;
-    xent_thin<T, rowops::XE_ADD>(q, q.out_in, q.H, q.splits, a, st);
-    hipLaunchKernelGGL(rowops::k_xent_finish<T>, dim3((unsigned)ceil_div64(q.N * q.H, 256)), dim3(256), 0, st, acc, q.N * q.H, q.splits, q.N, q.H, (T*)dx, dx_row);
+    if (q.splits == 1) {
+        a.C = dx; a.ldc = dx_row;
+        xent_thin<T, rowops::XE_STORE>(q, q.out_in, q.H, 1, a, st);
+    } else {
+        xent_thin<T, rowops::XE_ADD>(q, q.out_in, q.H, q.splits, a, st);
+        hipLaunchKernelGGL(rowops::k_xent_finish<T>, dim3((unsigned)ceil_div64(q.N * q.H, 256)), dim3(256), 0, st, acc, q.N * q.H, q.splits, q.N, q.H, (T*)dx, dx_row);
+    }
     const bool oi = dk_in == 1;
     const int64_t na = oi ? q.V : q.H, nb = oi ? q.H : q.V;
     const dim3 grid((unsigned)ceil_div64(nb, 256), (unsigned)ceil_div64(na, 64));
@@ -487,8 +537,8 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     r.tiles = q.tiles_n; r.rows = q.N; r.classes = q.V;
     r.target = d->target; r.target_kind = d->target_kind;
     r.loss = loss; r.lse = lse;
-    r.per = 1;                                                   // few rows: more strands over the tiles each
-    while (r.per < 64 && 2 * r.per <= q.N) r.per *= 2;
+    r.per = 1;                                                   // rows per workgroup: fewer, with more strands over the tiles each, while a strand has more than two
+    while (r.per < 64 && 2 * r.per <= q.N && (r.per < 4 || 1024 / (2 * r.per) * 2 >= q.tiles_n)) r.per *= 2;
     hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, r.per)), dim3(1024), 0, st, r);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
@@ -514,9 +564,8 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         HIPCHK(hipGetLastError());
         return DIMN_OK;
     }
-    float* scale = (float*)(ws + q.scale);
     float* tsum = (float*)(ws + q.tsum);
-    xent_rows(q, dloss, scale, tsum, st);
+    xent_tsum(q, tsum, st);
     uint16_t* xt = (uint16_t*)(ws + q.xt);
     const int64_t xt_plane = q.H * q.Np;
     xent_lay(q.f32, true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane, st);
@@ -525,7 +574,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         const int64_t pv = std::min(q.P, q.V - c0), ldg = up(pv, 64);
         XentGemm p;
         xent_logits(q, ws, c0, pv, p, st);
-        p.lse = lse; p.scale = scale; p.tsum = tsum;
+        p.lse = lse; p.dloss = dloss; p.tsum = tsum;
         p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
         p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
         p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = q.V;
@@ -547,7 +596,6 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         // dW of the piece
         XentGemm w{};
         w.ksteps = (int)(q.Np / 64); w.segments = q.segments; w.a_of = q.a_of; w.b_of = q.b_of;
-        w.c_type = d->type;
         const uint16_t *gt = p.GT, *xa = xt;
         if (dk_out_in) {
             w.A = gt; w.lda = q.Np; w.a_plane = p.gt_plane; w.M = (int)pv;

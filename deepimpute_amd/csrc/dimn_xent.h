@@ -42,52 +42,79 @@ __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
 
 // ---- operand layout -----------------------------------------------------------------------------------------------------------
 // to[plane][r][k] = bfloat16 term `plane` of from[r][k], zero for cols <= k < ldk (ldk: a multiple of 64).  T = float: three planes, T = bf16_t: one.
-// TRANSPOSED: from is [k][r] with r contiguous (row stride `ld` along k).  64 x 64 tiles, through LDS when transposed.
-template <typename T, bool TRANSPOSED>
-__global__ __launch_bounds__(256) void k_xent_lay(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
+// Copying bounds both; everything moves in 16-byte pieces.
+template <typename T> struct Eight { typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Eight<float> { typedef float vec __attribute__((ext_vector_type(8), aligned(4))); };
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+__device__ __forceinline__ void lay_store(const T (&v)[8], uint16_t* to, int64_t plane) {
     constexpr int PL = sizeof(T) == 4 ? 3 : 1;
+    u16x8 o[PL];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if constexpr (PL == 3) {
+            uint16_t b[3];
+            split3(v[j], b);
+            o[0][j] = b[0]; o[1][j] = b[1]; o[2][j] = b[2];
+        } else o[0][j] = v[j];
+    }
+#pragma unroll
+    for (int pl = 0; pl < PL; ++pl) *(u16x8*)(to + pl * plane) = o[pl];
+}
+// from: [r][k], k contiguous.  One thread per eight k's.
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_lay(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
+    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (e >= rows * ldk) return;
+    const int64_t r = e / ldk, k = e - r * ldk;
+    const T* p = from + r * ld + k;
+    T v[8];
+    if (k + 8 <= cols) {
+        const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = x[j];
+    } else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? p[j] : (T)0;
+    lay_store<T>(v, to + e, plane);
+}
+// from: [k][r], r contiguous (row stride `ld` along k).  64 x 64 tiles through LDS; a line of 65 (float) / 66 (bfloat16) elements spreads a column
+// over the banks.
+template <typename T>
+__global__ __launch_bounds__(256) void k_xent_lay_t(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
+    constexpr int LD = sizeof(T) == 4 ? 65 : 66;
+    __shared__ T tile[64][LD];
     const int64_t tiles_k = ldk >> 6;
     const int64_t tr = blockIdx.x / tiles_k, tk = blockIdx.x - tr * tiles_k;
     const int64_t r0 = tr * 64, k0 = tk * 64;
-    const int q = threadIdx.x & 15, s = threadIdx.x >> 4;        // 16 pieces of four x 16 lines
-    __shared__ T tile[TRANSPOSED ? 64 : 1][TRANSPOSED ? 66 : 1];
-    if constexpr (TRANSPOSED) {
+    const int q = threadIdx.x & 7, s = threadIdx.x >> 3;         // 8 pieces of eight x 32 lines
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t k = k0 + s + 16 * i;
-            T v[4] = {0, 0, 0, 0};
-            if (k < cols) {
-                const T* p = from + k * ld + r0 + 4 * q;
+    for (int i = 0; i < 2; ++i) {
+        const int64_t k = k0 + s + 32 * i, r = r0 + 8 * q;
+        const T* p = from + k * ld + r;
+        T v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (k < cols) {
+            if (r + 8 <= rows) {
+                const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)p;
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (r0 + 4 * q + j < rows) v[j] = p[j];
-            }
+                for (int j = 0; j < 8; ++j) v[j] = x[j];
+            } else
 #pragma unroll
-            for (int j = 0; j < 4; ++j) tile[s + 16 * i][4 * q + j] = v[j];
+                for (int j = 0; j < 8; ++j) if (r + j < rows) v[j] = p[j];
         }
-        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[s + 32 * i][8 * q + j] = v[j];
     }
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = r0 + s + 16 * i;
+    for (int i = 0; i < 2; ++i) {
+        const int64_t r = r0 + s + 32 * i;
         if (r >= rows) continue;
-        T v[4] = {0, 0, 0, 0};
+        T v[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (TRANSPOSED) v[j] = tile[4 * q + j][s + 16 * i];
-            else if (k0 + 4 * q + j < cols) v[j] = from[r * ld + k0 + 4 * q + j];
-        }
-        u16x4 o[PL];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (PL == 3) {
-                uint16_t b[3];
-                split3(v[j], b);
-                o[0][j] = b[0]; o[1][j] = b[1]; o[2][j] = b[2];
-            } else o[0][j] = v[j];
-        }
-#pragma unroll
-        for (int pl = 0; pl < PL; ++pl) *(u16x4*)(to + pl * plane + r * ldk + k0 + 4 * q) = o[pl];
+        for (int j = 0; j < 8; ++j) v[j] = tile[8 * q + j][s + 32 * i];
+        lay_store<T>(v, to + r * ldk + k0 + 8 * q, plane);
     }
 }
 
@@ -110,13 +137,13 @@ struct XentGemm {
     float2* part_t;                            // profile: [tiles_n][M]: (sum of t, sum of t z)
     float* picked;                             // labels: [M], z of the label, written by the workgroup that holds it
     // G
-    const float* lse; const float* scale;      // [M]: dloss (0 for a row without a target)
+    const float* lse; const float* dloss;      // [M]
     const float* tsum;                         // profile: [M]
     uint16_t* G; int64_t ldg, g_plane;         // [plane][M][ldg], columns N .. ldg zero
     uint16_t* GT; int64_t ldgt, gt_plane;      // [plane][N][ldgt], columns M .. ldgt zero
     float* dbias_part; int64_t dbias_ld;       // [2 tiles_m][dbias_ld]: column sums of G over the rows of one wave row
     // result
-    void* C; int64_t ldc; int32_t c_type;      // epilogue 2: C[m][n], DIMN_TYPE_*
+    void* C; int64_t ldc;                      // epilogue 2: C[m][n], float32 (three planes) or bfloat16 (one)
     float* acc; int64_t acc_split; int32_t acc_first;   // epilogue 3: acc[split][M][N] (+)= C
 };
 enum { XE_LSE = 0, XE_GRAD = 1, XE_STORE = 2, XE_ADD = 3 };
@@ -126,16 +153,16 @@ __device__ __forceinline__ int64_t xent_label(const XentGemm& p, int64_t row) {
     return p.target_kind == XT_I64 ? ((const int64_t*)p.target)[row] : (int64_t)((const int32_t*)p.target)[row];
 }
 // four consecutive entries of a profile row, 0 from `n` on
-__device__ __forceinline__ f32x4 xent_profile4(const XentGemm& p, int64_t row, int col, int n) {
+__device__ __forceinline__ f32x4 xent_profile4(const void* target, int32_t kind, int64_t ld, int64_t row, int64_t col, int64_t n) {
     f32x4 t = {0.f, 0.f, 0.f, 0.f};
-    if (p.target_kind == XT_F32) {
-        const float* q = (const float*)p.target + row * p.target_row + col;
+    if (kind == XT_F32) {
+        const float* q = (const float*)target + row * ld + col;
         if (col + 4 <= n) t = *(const f32x4u*)q;
         else
 #pragma unroll
             for (int r = 0; r < 4; ++r) if (col + r < n) t[r] = q[r];
     } else {
-        const uint16_t* q = (const uint16_t*)p.target + row * p.target_row + col;
+        const uint16_t* q = (const uint16_t*)target + row * ld + col;
         if (col + 4 <= n) {
             const u16x4u v = *(const u16x4u*)q;
 #pragma unroll
@@ -151,11 +178,15 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 
 // Tile BM x BN per workgroup, WM x WN waves; k in steps of 64, two stages of LDS filled by 16-byte DMA while the other one is multiplied, one
-// barrier per step.  A row of a tile is 128 bytes; its eight 16-byte pieces are stored at piece ^ (row & 7), so that the sixteen rows a
-// fragment reads spread over all banks (the DMA writes LDS in lane order: the permutation is made on the global side).
-// The matrix instruction takes B's rows as its rows and A's as its columns: a lane then holds four consecutive n of one m, so that
-// sums along n are mostly inside a lane and results leave in pieces of four.
-template <int BM, int BN, int WM, int WN, int EPI>
+// barrier per step.  The matrix instruction takes B's rows as its rows and A's as its columns, and fragment i / j of a wave holds rows
+// FM li + i of A, 4 FN (q >> 2) + 4 j + (q & 3) of B (q: the instruction's row): a lane then owns FM consecutive m's x 4 FN consecutive n's of C.
+// Sums along n are mostly inside a lane, results leave in 16-byte pieces in BOTH memory orders, and G needs no transposition.
+// A row of a tile is 128 bytes; its eight 16-byte pieces are stored at piece ^ bank_turn(row): the rows a fragment reads at once (FM or 4 FN
+// apart) then fall on different banks.  The DMA writes LDS in lane order, so the turn is made on the global side.
+__device__ __forceinline__ int bank_turn(int row) {
+    return ((row ^ (row >> 3)) & 1) | ((((row >> 1) ^ (row >> 2) ^ (row >> 5)) & 1) << 1) | (((row >> 4) & 1) << 2);
+}
+template <int BM, int BN, int WM, int WN, int EPI, int PL>
 __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
     constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
     constexpr int LOADS = (BM + BN) / 8 / NW;
@@ -183,9 +214,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
 #pragma unroll
     for (int c = 0; c < LOADS; ++c) {
         const int row = (wave * LOADS + c) * 8 + (lane >> 3);
-        const int piece = (lane & 7) ^ (row & 7);
         const bool isA = (wave * LOADS + c) * 8 < BM;
         int r = isA ? row : row - BM;
+        const int piece = (lane & 7) ^ bank_turn(r);
         const int lim = isA ? p.M - 1 - m0 : p.N - 1 - n0;       // rows past the end read the last one: their results are never used
         r = r < lim ? r : lim;
         off[c] = (uint32_t)((int64_t)r * (isA ? p.lda : p.ldb) * 2 + piece * 16);
@@ -217,13 +248,13 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
             bf8 a[FM], b[FN];
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const int row = BM + wn * TN + 16 * j + li;
-                b[j] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ (row & 7)) << 3)];
+                const int row = wn * TN + (li >> 2) * 4 * FN + 4 * j + (li & 3);
+                b[j] = *(const bf8*)&lds[stage][(BM + row) * 64 + (((kk * 4 + lj) ^ bank_turn(row)) << 3)];
             }
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const int row = wm * TM + 16 * i + li;
-                a[i] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ (row & 7)) << 3)];
+                const int row = wm * TM + li * FM + i;
+                a[i] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ bank_turn(row)) << 3)];
             }
 #pragma unroll
             for (int i = 0; i < FM; ++i)
@@ -232,22 +263,36 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
         }
     };
     if (tbeg < tend) request(0);
-    for (int t = tbeg; t < tend; ++t) {
-        const int stage = (t - tbeg) & 1;
+    int stage = 0;
+    for (int t = tbeg; t + 1 < tend; ++t) {
         __syncthreads();                                         // the stage's bytes have landed (the barrier waits for this wave's requests first) and
-        if (t + 1 < tend) request(stage ^ 1);                    // everybody is done with the other stage
+        request(stage ^ 1);                                      // everybody is done with the other stage
+        multiply(stage);
+        stage ^= 1;
+        // Fragments are read one group of 2 FN products ahead of their use: left alone, the compiler reads two, waits, and multiplies (4-6 % slower)
+        constexpr int GROUP = (2 * FM + FN - 2) / (FM - 2);
+        __builtin_amdgcn_sched_group_barrier(0x100, FN + 2, 0);
+#pragma unroll
+        for (int q = 0; q < FM - 2; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x100, GROUP, 0);
+            __builtin_amdgcn_sched_group_barrier(0x8, 2 * FN, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4 * FN, 0);
+    }
+    if (tbeg < tend) {
+        __syncthreads();
         multiply(stage);
     }
-    // a lane's results: C[m0 + wm TM + 16 i + li][n0 + wn TN + 16 j + 4 lj + r] in acc[i][j][r]
-    const int nb = n0 + wn * TN + 4 * lj;
+    // this lane's results: C[mb + i][nb + 4 j + r] in acc[i][j][r]
+    const int mb = m0 + wm * TM + li * FM, nb = n0 + wn * TN + lj * 4 * FN;
     if constexpr (EPI == XE_STORE || EPI == XE_ADD) {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const int64_t m = m0 + wm * TM + 16 * i + li;
+            const int64_t m = mb + i;
             if (m >= p.M) continue;
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const int n = nb + 16 * j;
+                const int n = nb + 4 * j;
                 if (n >= p.N) continue;
                 const f32x4 v = acc[i][j];
                 if constexpr (EPI == XE_ADD) {
@@ -256,7 +301,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                     else
 #pragma unroll
                         for (int r = 0; r < 4; ++r) if (n + r < p.N) q[r] = p.acc_first ? v[r] : q[r] + v[r];
-                } else if (p.c_type == DIMN_TYPE_F32) {
+                } else if constexpr (PL == 3) {
                     float* q = (float*)p.C + m * p.ldc + n;
                     if (n + 4 <= p.N) *(f32x4u*)q = v;
                     else
@@ -277,44 +322,54 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
         return;
     }
     if constexpr (EPI == XE_LSE || EPI == XE_GRAD) {
-        const bool labels = p.target_kind <= XT_I64, split = p.segments > 1;
-        f32x4 bias[FN];
+        // (__expf rounds its scaled argument, 2^-24 |d| of the result: far below a bfloat16 operand's half step, too much for float32 results)
+        auto power = [](float d) { if constexpr (PL == 1) return __expf(d); else return expf(d); };
+        const bool labels = p.target_kind <= XT_I64;
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
-            const int n = nb + 16 * j;
+            f32x4 b = {0.f, 0.f, 0.f, 0.f};
+            const int n = nb + 4 * j;
+            if (p.bias) {
+                if (n + 4 <= p.N) b = *(const f32x4u*)(p.bias + n);
+                else
 #pragma unroll
-            for (int r = 0; r < 4; ++r) bias[j][r] = p.bias && n + r < p.N ? p.bias[n + r] : 0.f;
+                    for (int r = 0; r < 4; ++r) if (n + r < p.N) b[r] = p.bias[n + r];
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (n + r >= p.N) b[r] = -INFINITY;              // no class: no probability
+#pragma unroll
+                for (int i = 0; i < FM; ++i) acc[i][j][r] += b[r];
+            }
         }
         if constexpr (EPI == XE_LSE) {
             float2* red = (float2*)&lds[0][0];                   // [WN][BM] (maximum, sum), then [WN][BM] (sum t, sum t z)
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const int mr = wm * TM + 16 * i + li;
+                const int mr = wm * TM + li * FM + i;
                 const int64_t m = m0 + mr;
                 const bool mine = m < p.M;
-                float top = -INFINITY;
+                float top = -INFINITY, s = 0.f;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        acc[i][j][r] += bias[j][r];
-                        if (nb + 16 * j + r < p.N) top = fmaxf(top, acc[i][j][r]);
-                    }
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
                 if (labels) {
                     const int64_t y = mine ? xent_label(p, m) - p.class0 - nb : -1;
-                    if (y >= 0 && y < TN && (y & 15) < 4 && nb + y < p.N) {
+                    if (y >= 0 && y < 4 * FN && nb + y < p.N) {
 #pragma unroll
                         for (int j = 0; j < FN; ++j)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) if (y == 16 * j + r) p.picked[m] = acc[i][j][r];
+                            for (int r = 0; r < 4; ++r) if (y == 4 * j + r) p.picked[m] = acc[i][j][r];
                     }
                 } else {
                     float st = 0.f, stz = 0.f;
                     if (mine)
 #pragma unroll
                         for (int j = 0; j < FN; ++j) {
-                            const f32x4 t = xent_profile4(p, m, nb + 16 * j, p.N);
+                            if (nb + 4 * j >= p.N) continue;
+                            const f32x4 t = xent_profile4(p.target, p.target_kind, p.target_row, m, nb + 4 * j, p.N);
 #pragma unroll
                             for (int r = 0; r < 4; ++r) { st += t[r]; stz += t[r] != 0.f ? t[r] * acc[i][j][r] : 0.f; }
                         }
@@ -325,11 +380,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 const float ref = top == -INFINITY ? 0.f : top;
-                float s = 0.f;
 #pragma unroll
                 for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) if (nb + 16 * j + r < p.N) s += split ? expf(acc[i][j][r] - ref) : __expf(acc[i][j][r] - ref);
+                    for (int r = 0; r < 4; ++r) s += power(acc[i][j][r] - ref);
                 s += __shfl_xor(s, 16);
                 s += __shfl_xor(s, 32);
                 if (lj == 0) red[wn * BM + mr] = make_float2(top, s);
@@ -342,7 +396,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                 for (int w = 0; w < WN; ++w) top = fmaxf(top, red[w * BM + mr].x);
                 const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                for (int w = 0; w < WN; ++w) { const float2 v = red[w * BM + mr]; s += v.y * __expf((v.x == -INFINITY ? ref : v.x) - ref); }
+                for (int w = 0; w < WN; ++w) { const float2 v = red[w * BM + mr]; s += v.y * power((v.x == -INFINITY ? ref : v.x) - ref); }
                 const int64_t at = (int64_t)tn * p.M + m0 + mr;
                 p.part[at] = make_float2(top, s);
                 if (!labels) {
@@ -353,45 +407,35 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                 }
             }
         } else {
-            float col[FN][4];
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) col[j][r] = 0.f;
+            // G in place of the logits: d ts exp(z - lse), minus d t or, at the label, d.  Rows without a target (d = 0) are 0 whatever they hold.
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const int64_t m = m0 + wm * TM + 16 * i + li;
+                const int64_t m = mb + i;
                 const bool mine = m < p.M;
-                const float lse = mine ? p.lse[m] : 0.f, d = mine ? p.scale[m] : 0.f;
-                const float ts = labels ? 1.f : (mine ? p.tsum[m] : 0.f);
-                const int64_t y = labels && mine ? xent_label(p, m) - p.class0 - nb : -1;
+                const int64_t label = labels && mine ? xent_label(p, m) : -1;
+                const float d = mine && (!labels || (label >= 0 && label < p.classes)) ? p.dloss[m] : 0.f;     // a label that is no class: no gradient
+                float lse = mine ? p.lse[m] : 0.f;
+                lse = lse == -INFINITY ? 0.f : lse;              // (no class left: every exponential is 0)
+                const float scale = labels ? d : (mine ? d * p.tsum[m] : 0.f);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) {
-                    const int n = nb + 16 * j;
-                    f32x4 t = {0.f, 0.f, 0.f, 0.f};
-                    if (!labels && mine && n < p.N) t = xent_profile4(p, m, n, p.N);
-                    float g[4];
+                for (int j = 0; j < FN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float z = acc[i][j][r] + bias[j][r];
-                        const float e = z == -INFINITY ? 0.f : (split ? expf(z - lse) : __expf(z - lse));   // (__expf: 2^-24 |z - lse| off, too much only for float32 results)
-                        const float hot = labels ? (y == 16 * j + r ? 1.f : 0.f) : t[r];
-                        g[r] = d != 0.f && n + r < p.N ? d * (ts * e - hot) : 0.f;
-                        col[j][r] += g[r];
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = d != 0.f ? scale * power(acc[i][j][r] - lse) : 0.f;
+                if (labels) {
+                    const int64_t y = label - p.class0 - nb;
+                    if (d != 0.f && y >= 0 && y < 4 * FN) {
+#pragma unroll
+                        for (int j = 0; j < FN; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[i][j][r] -= y == 4 * j + r ? d : 0.f;
                     }
+                } else if (d != 0.f) {
 #pragma unroll
-                    for (int pl = 0; pl < 3; ++pl) {
-                        if (pl > 0 && !split) break;
-                        u16x4 o;
+                    for (int j = 0; j < FN; ++j) {
+                        if (nb + 4 * j >= p.N) continue;
+                        const f32x4 t = xent_profile4(p.target, p.target_kind, p.target_row, m, nb + 4 * j, p.N);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            o[r] = to_bf16(g[r]);
-                            g[r] -= from_bf16(o[r]);
-                        }
-                        if (mine && n < p.ldg) *(u16x4*)(p.G + pl * p.g_plane + m * p.ldg + n) = o;
-                        if (m < p.ldgt)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) if (n + r < p.N) p.GT[pl * p.gt_plane + (int64_t)(n + r) * p.ldgt + m] = o[r];
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] -= d * t[r];
                     }
                 }
             }
@@ -399,11 +443,50 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
             for (int j = 0; j < FN; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    float s = col[j][r];
+                    float s = 0.f;
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) s += acc[i][j][r];
 #pragma unroll
                     for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-                    if (li == 0 && nb + 16 * j + r < p.N) p.dbias_part[(int64_t)(tm * WM + wm) * p.dbias_ld + p.class0 + nb + 16 * j + r] = s;
+                    if (li == 0 && nb + 4 * j + r < p.N) p.dbias_part[(int64_t)(tm * WM + wm) * p.dbias_ld + p.class0 + nb + 4 * j + r] = s;
                 }
+            typedef uint16_t rowvec __attribute__((ext_vector_type(4 * FN)));
+            typedef uint16_t colvec __attribute__((ext_vector_type(FM)));
+#pragma unroll
+            for (int pl = 0; pl < PL; ++pl) {
+                uint16_t o[FM][4 * FN];
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            o[i][4 * j + r] = to_bf16(acc[i][j][r]);
+                            if (pl + 1 < PL) acc[i][j][r] -= from_bf16(o[i][4 * j + r]);
+                        }
+                uint16_t* G = p.G + pl * p.g_plane;
+                uint16_t* GT = p.GT + pl * p.gt_plane;
+                if (nb < p.ldg) {                                // (ldg is a multiple of 64, a lane's 4 FN columns lie inside or outside of it)
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) {
+                        if (mb + i >= p.M) continue;
+                        rowvec v;
+#pragma unroll
+                        for (int k = 0; k < 4 * FN; ++k) v[k] = o[i][k];
+                        *(rowvec*)(G + (int64_t)(mb + i) * p.ldg + nb) = v;
+                    }
+                }
+                if (mb < p.ldgt) {                               // (so is ldgt)
+#pragma unroll
+                    for (int k = 0; k < 4 * FN; ++k) {
+                        if (nb + k >= p.N) continue;
+                        colvec v;
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) v[i] = o[i][k];
+                        *(colvec*)(GT + (int64_t)(nb + k) * p.ldgt + mb) = v;
+                    }
+                }
+            }
         }
     }
 }
@@ -461,17 +544,9 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
     p.loss[row] = loss;
 }
 
-// Backward, per row: scale = dloss, or 0 for a row without a target (label negative or not a class); tsum = the sum of its profile.
-__global__ __launch_bounds__(1024) void k_xent_rows(const void* target, int32_t kind, int64_t target_row, int64_t rows, int64_t classes, const float* __restrict__ dloss,
-                                                   float* __restrict__ scale, float* __restrict__ tsum) {
-    if (kind <= XT_I64) {
-        const int64_t row = (int64_t)blockIdx.x * 1024 + threadIdx.x;
-        if (row >= rows) return;
-        const int64_t y = kind == XT_I64 ? ((const int64_t*)target)[row] : (int64_t)((const int32_t*)target)[row];
-        scale[row] = y >= 0 && y < classes ? dloss[row] : 0.f;
-        return;
-    }
-    const int64_t row = blockIdx.x;                              // one workgroup per row
+// tsum = the sum of every row of a profile; one workgroup per row
+__global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t kind, int64_t target_row, int64_t classes, float* __restrict__ tsum) {
+    const int64_t row = blockIdx.x;
     __shared__ float red[16];
     float s = 0.f;
     if (kind == XT_F32) {
@@ -498,7 +573,6 @@ __global__ __launch_bounds__(1024) void k_xent_rows(const void* target, int32_t 
 #pragma unroll
         for (int w = 0; w < 16; ++w) s += red[w];
         tsum[row] = s;
-        scale[row] = dloss[row];
     }
 }
 
@@ -519,6 +593,7 @@ __global__ __launch_bounds__(256) void k_xent_dbias(const float* __restrict__ pa
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= classes) return;
     float s = 0.f;
+#pragma unroll 8
     for (int k = 0; k < parts; ++k) s += part[k * ld + c];
     dbias[c] = s;
 }

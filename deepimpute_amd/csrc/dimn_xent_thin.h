@@ -25,10 +25,11 @@ struct Thin {
     const float* bias;                         // [N] or NULL
     const void* target; int64_t target_row; int32_t target_kind;
     float2* part; float2* part_t; float* picked;          // as XentGemm (a tile: 32 / 64 classes)
-    const float* lse; const float* scale; const float* tsum;
+    const float* lse; const float* dloss; const float* tsum;
     void* G; int64_t ldg;                      // [M][ldg] of T
     float* dbias_part;                         // [gridDim.z][N]
     float* acc;                                // XE_ADD: [gridDim.y][M][N] float32
+    void* C; int64_t ldc;                      // XE_STORE: [M][N] of T
 };
 
 template <typename T> struct Four;             // four consecutive elements of a class row (VC)
@@ -108,14 +109,16 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
     // this workgroup's range of whole chunks; the chunk that crosses K belongs to the last range
     const int64_t whole = p.K / KS, S = gridDim.y;
     const int64_t cbeg = whole * blockIdx.y / S, cend = whole * (blockIdx.y + 1) / S;
-    int64_t c = cbeg + wave;
-    for (; c + 4 * (U - 1) < cend; c += 4 * U) {
+    // whole rounds of U consecutive chunks per wave (256 bytes of a class row at a time), then single chunks
+    const int64_t rounds = (cend - cbeg) / (4 * U);
+    for (int64_t i = 0; i < rounds; ++i) {
+        const int64_t c = cbeg + (4 * i + wave) * U;
 #pragma unroll
-        for (int u = 0; u < U; ++u) request((c + 4 * u) * KS, a[u], b[u]);
+        for (int u = 0; u < U; ++u) request((c + u) * KS, a[u], b[u]);
 #pragma unroll
         for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
     }
-    for (; c < cend; c += 4) { request(c * KS, a[0], b[0]); multiply(a[0], b[0]); }
+    for (int64_t c = cbeg + rounds * 4 * U + wave; c < cend; c += 4) { request(c * KS, a[0], b[0]); multiply(a[0], b[0]); }
     if (whole * KS < p.K && blockIdx.y == S - 1 && wave == (whole & 3)) {
         const int64_t k = whole * KS;
 #pragma unroll
@@ -158,99 +161,151 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
     __syncthreads();
     if (wave < 2) put(wave);
     __syncthreads();
-    // PT threads per row, CPT consecutive positions each
-    constexpr int PT = 256 / ROWS, CPT = CW / PT;
+    // PT threads per row, CPT consecutive positions each, in groups of four whose classes are consecutive
+    constexpr int CPT = CW * ROWS / 256 < 4 ? 4 : CW * ROWS / 256, PT = CW / CPT, NG = CPT / 4;
     const int row = tid / PT, pos0 = (tid % PT) * CPT;
     const int64_t m = m0 + row;
-    const bool have = m < p.M;
-    // class of a position, and whether this workgroup answers for it
-    auto cls = [&](int pos, bool& mine) -> int64_t {
+    const bool have = row < ROWS && m < p.M;
+    // first class of a group, and how many of its four classes belong to another group (VC: the last one is moved back to end with the classes) or are none
+    auto group = [&](int pos, int& before, int& upto) -> int64_t {
+        const int64_t from = c0 + pos;
         if constexpr (VC) {
-            const int64_t from = c0 + (pos & ~3), start = from < p.N - 4 ? from : p.N - 4, k = start + (pos & 3);
-            mine = k >= from;
-            return k;
-        } else { mine = c0 + pos < p.N; return c0 + pos; }
+            const int64_t start = from < p.N - 4 ? from : p.N - 4;
+            before = from - start < 4 ? (int)(from - start) : 4;
+            upto = 4;
+            return start;
+        } else {
+            before = 0;
+            upto = from + 4 <= p.N ? 4 : (from < p.N ? (int)(p.N - from) : 0);
+            return from;
+        }
     };
-    if constexpr (EPI == XE_ADD) {
-        if (!have) return;
-        float* to = p.acc + ((int64_t)blockIdx.y * p.M + m) * p.N;
+    f32x4 z[NG];
+    if (row < ROWS) {
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            bool mine;
-            const int64_t k = cls(pos0 + i, mine);
-            if (mine) to[k] = red[0][row][pos0 + i] + red[1][row][pos0 + i];
+        for (int q = 0; q < NG; ++q) z[q] = *(const f32x4*)&red[0][row][pos0 + 4 * q] + *(const f32x4*)&red[1][row][pos0 + 4 * q];
+    }
+    if constexpr (EPI == XE_ADD || EPI == XE_STORE) {
+        if (!have) return;
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+            int before, upto;
+            const int64_t k = group(pos0 + 4 * q, before, upto);
+            if constexpr (EPI == XE_ADD) {
+                float* to = p.acc + ((int64_t)blockIdx.y * p.M + m) * p.N + k;
+                if (before == 0 && upto == 4) *(f32x4u*)to = z[q];
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (i >= before && i < upto) to[i] = z[q][i];
+            } else {
+                T* to = (T*)p.C + m * p.ldc + k;
+                typename Four<T>::vec o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { if constexpr (BF) o[i] = to_bf16(z[q][i]); else o[i] = z[q][i]; }
+                if (before == 0 && upto == 4) *(typename Four<T>::vec*)to = o;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (i >= before && i < upto) to[i] = o[i];
+            }
         }
         return;
     }
-    const bool labels = p.target_kind <= XT_I64;
-    int64_t y = -1;
-    if (labels && have) y = p.target_kind == XT_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
-    float z[CPT], t[CPT];
+    if constexpr (EPI == XE_LSE || EPI == XE_GRAD) {
+        const bool labels = p.target_kind <= XT_I64;
+        int64_t y = -1;
+        if (labels && have) y = p.target_kind == XT_I64 ? ((const int64_t*)p.target)[m] : (int64_t)((const int32_t*)p.target)[m];
+        f32x4 t[NG];
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-        bool mine;
-        const int64_t k = cls(pos0 + i, mine);
-        z[i] = red[0][row][pos0 + i] + red[1][row][pos0 + i] + (p.bias && mine ? p.bias[k] : 0.f);
-        t[i] = 0.f;
-        if (!labels && have && mine)
-            t[i] = p.target_kind == XT_F32 ? ((const float*)p.target)[m * p.target_row + k] : from_bf16(((const uint16_t*)p.target)[m * p.target_row + k]);
-    }
-    if constexpr (EPI == XE_LSE) {
-        float top = -INFINITY, s = 0.f, st = 0.f, stz = 0.f;
+        for (int q = 0; q < NG; ++q) {
+            t[q] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            int before, upto;
+            const int64_t k = group(pos0 + 4 * q, before, upto);
+            if (!have || upto == 0) continue;
+            if (p.bias) {
+                f32x4 b4 = {0.f, 0.f, 0.f, 0.f};
+                if (upto == 4) b4 = *(const f32x4u*)(p.bias + k);
+                else
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            bool mine;
-            const int64_t k = cls(pos0 + i, mine);
-            if (mine) top = fmaxf(top, z[i]);
-            if (labels && mine && k == y) p.picked[m] = z[i];
-            st += t[i];
-            stz += t[i] != 0.f ? t[i] * z[i] : 0.f;
+                    for (int i = 0; i < 4; ++i) if (i < upto) b4[i] = p.bias[k + i];
+                z[q] += b4;
+            }
+            if (!labels) t[q] = xent_profile4(p.target, p.target_kind, p.target_row, m, k, p.N);
         }
+        if constexpr (EPI == XE_LSE) {
+            float top = -INFINITY, s = 0.f, st = 0.f, stz = 0.f;
 #pragma unroll
-        for (int o = 1; o < PT; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float ref = top == -INFINITY ? 0.f : top;
+            for (int q = 0; q < NG; ++q) {
+                int before, upto;
+                const int64_t k = group(pos0 + 4 * q, before, upto);
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            bool mine;
-            cls(pos0 + i, mine);
-            if (mine) s += BF ? __expf(z[i] - ref) : expf(z[i] - ref);
-        }
+                for (int i = 0; i < 4; ++i) {
+                    if (i < before || i >= upto) continue;
+                    top = fmaxf(top, z[q][i]);
+                    if (have && labels && k + i == y) p.picked[m] = z[q][i];
+                    st += t[q][i];
+                    stz += t[q][i] != 0.f ? t[q][i] * z[q][i] : 0.f;
+                }
+            }
 #pragma unroll
-        for (int o = 1; o < PT; o <<= 1) { s += __shfl_xor(s, o); st += __shfl_xor(st, o); stz += __shfl_xor(stz, o); }
-        if (have && tid % PT == 0) {
-            const int64_t at = (int64_t)blockIdx.x * p.M + m;
-            p.part[at] = make_float2(top, s);
-            if (!labels) p.part_t[at] = make_float2(st, stz);
-        }
-    } else {
-        const float lse = have ? p.lse[m] : 0.f, d = have ? p.scale[m] : 0.f, ts = labels ? 1.f : (have ? p.tsum[m] : 0.f);
-        T* G = (T*)p.G + m * p.ldg;
-        __syncthreads();                                        // the products have been read: the first slot takes G for the sums over the rows
+            for (int o = 1; o < PT; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+            const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int i = 0; i < CPT; ++i) {
-            bool mine;
-            const int64_t k = cls(pos0 + i, mine);
-            const float e = z[i] == -INFINITY ? 0.f : (BF ? __expf(z[i] - lse) : expf(z[i] - lse));
-            const float hot = labels ? (k == y ? 1.f : 0.f) : t[i];
-            const float g = d != 0.f ? d * (ts * e - hot) : 0.f;
-            red[0][row][pos0 + i] = g;
-            if (have && mine) { if constexpr (BF) G[k] = to_bf16(g); else G[k] = g; }
-        }
-        if (!p.dbias_part) return;
-        __syncthreads();
-        constexpr int ST = 256 / CW;                            // strands of rows per class
-        const int pos = tid % CW, strand = tid / CW;
-        float s = 0.f;
-        for (int r = strand; r < ROWS; r += ST) s += red[0][r][pos];
-        __syncthreads();
-        red[1][strand][pos] = s;
-        __syncthreads();
-        if (strand == 0) {
-            bool mine;
-            const int64_t k = cls(pos, mine);
+            for (int q = 0; q < NG; ++q) {
+                int before, upto;
+                group(pos0 + 4 * q, before, upto);
 #pragma unroll
-            for (int w = 1; w < ST; ++w) s += red[1][w][pos];
-            if (mine) p.dbias_part[(int64_t)blockIdx.z * p.N + k] = s;
+                for (int i = 0; i < 4; ++i)
+                    if (i >= before && i < upto) s += BF ? __expf(z[q][i] - ref) : expf(z[q][i] - ref);
+            }
+#pragma unroll
+            for (int o = 1; o < PT; o <<= 1) { s += __shfl_xor(s, o); st += __shfl_xor(st, o); stz += __shfl_xor(stz, o); }
+            if (have && tid % PT == 0) {
+                const int64_t at = (int64_t)blockIdx.x * p.M + m;
+                p.part[at] = make_float2(top, s);
+                if (!labels) p.part_t[at] = make_float2(st, stz);
+            }
+        } else {
+            const float lse = have ? p.lse[m] : 0.f, d = have && (!labels || (y >= 0 && y < p.N)) ? p.dloss[m] : 0.f, ts = labels ? 1.f : (have ? p.tsum[m] : 0.f);     // (a label that is no class: no gradient)
+            __syncthreads();                                    // the products have been read: the first slot takes G for the sums over the rows
+#pragma unroll
+            for (int q = 0; q < NG; ++q) {
+                int before, upto;
+                const int64_t k = group(pos0 + 4 * q, before, upto);
+                f32x4 g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float e = z[q][i] == -INFINITY ? 0.f : (BF ? __expf(z[q][i] - lse) : expf(z[q][i] - lse));
+                    const float hot = labels ? (k + i == y ? 1.f : 0.f) : t[q][i];
+                    g[i] = d != 0.f ? d * (ts * e - hot) : 0.f;
+                }
+                if (row < ROWS) *(f32x4*)&red[0][row][pos0 + 4 * q] = g;
+                if (!have) continue;
+                T* to = (T*)p.G + m * p.ldg + k;
+                typename Four<T>::vec o;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { if constexpr (BF) o[i] = to_bf16(g[i]); else o[i] = g[i]; }
+                if (before == 0 && upto == 4) *(typename Four<T>::vec*)to = o;
+                else
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) if (i >= before && i < upto) to[i] = o[i];
+            }
+            if (!p.dbias_part) return;
+            __syncthreads();
+            constexpr int ST = 256 / CW;                        // strands of rows per class
+            const int pos = tid % CW, strand = tid / CW;
+            float s = 0.f;
+#pragma unroll 8
+            for (int r = strand; r < ROWS; r += ST) s += red[0][r][pos];
+            __syncthreads();
+            red[1][strand][pos] = s;
+            __syncthreads();
+            if (strand == 0) {
+                int before, upto;
+                const int64_t k = group(pos & ~3, before, upto);
+#pragma unroll
+                for (int w = 1; w < ST; ++w) s += red[1][w][pos];
+                if ((pos & 3) >= before && (pos & 3) < upto) p.dbias_part[(int64_t)blockIdx.z * p.N + k + (pos & 3)] = s;
+            }
         }
     }
 }

@@ -210,6 +210,11 @@ def test_masks_and_odd_labels(dtype):
         assert bool((lse4 == -inf).all()) and bool((loss4 == inf).all())
         g = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse4, none)
         assert all(bool(torch.isfinite(v).all()) for v in g)
+        # every class masked by the lowest float32: all of them equally likely, not none
+        loss6, lse6 = ops.linear_cross_entropy(x, kernel, t, torch.full_like(b, torch.finfo(torch.float32).min))
+        assert bool((lse6 == torch.finfo(torch.float32).min).all()) and bool((loss6 == 0).all())
+        loss7, _ = ops.linear_cross_entropy(x, kernel, odd, low)
+        assert bool(torch.isfinite(loss7).all()) and float(loss7.min()) > 3.4e38
         # labels that are no classes: a loss that says so, no gradient, nothing out of bounds
         bad = t.clone()
         bad[3], bad[7], bad[9] = classes, 2 ** 31 - 1, -(2 ** 31)
