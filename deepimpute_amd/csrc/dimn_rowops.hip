@@ -46,17 +46,21 @@ struct OnDevice {
     ~OnDevice() { if (now >= 0 && before != now) (void)hipSetDevice(before); }
 };
 
-// compute units of the current device (256 on MI355X), asked once per device
-int compute_units() {
+// compute units of a device (256 on MI355X), asked once per device
+int compute_units(int dev) {
     static std::atomic<int> known[64];
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (dev < 0 || dev >= 64) return 256;
     int n = known[dev].load(std::memory_order_relaxed);
     if (n == 0) {
         if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n < 1) n = 256;
         known[dev].store(n, std::memory_order_relaxed);
     }
     return n;
+}
+
+int current_device() {
+    int dev = 0;
+    return hipGetDevice(&dev) == hipSuccess ? dev : 0;
 }
 
 // ---- layer normalisation: which kernel a width takes -----------------------------------------------------------------------
@@ -82,7 +86,7 @@ int64_t norm_blocks(const NormForm& f, bool grad, int64_t groups, int64_t rows) 
     if (rows == 0) return 1;
     const int sets = f.tpr == 0 ? 1 : std::max(1, 256 / f.tpr);
     const int64_t per_cu = grad ? 2 : 4;
-    const int64_t budget = std::max<int64_t>(1, per_cu * compute_units() / (f.tpr == 1024 || f.tpr == 0 ? 2 : 1) / std::max<int64_t>(1, groups));
+    const int64_t budget = std::max<int64_t>(1, per_cu * compute_units(current_device()) / (f.tpr == 1024 || f.tpr == 0 ? 2 : 1) / std::max<int64_t>(1, groups));
     const int64_t all = ceil_div64(rows, sets);
     const int64_t each = ceil_div64(all, budget);
     return std::max<int64_t>(1, ceil_div64(all, each));
@@ -232,9 +236,11 @@ int64_t up(int64_t a, int64_t b) { return ceil_div64(a, b) * b; }
 struct Tile { int bm, bn, wm; };
 constexpr Tile kTiles[3] = {{256, 256, 2}, {128, 128, 2}, {64, 128, 1}};
 int64_t tile_count(const Tile& t, int64_t M, int64_t N) { return ceil_div64(M, t.bm) * ceil_div64(N, t.bn); }
+// 256 tiles (one workgroup per CU) unless 128 tiles (two per CU, a quarter of the work each, 15 % more time for it) need fewer rounds
 int pick_tile(int64_t M, int64_t N, int ncu) {
     if (M <= 64) return 2;
-    return tile_count(kTiles[0], M, N) >= ncu * 3 / 4 ? 0 : 1;
+    const double t256 = (double)ceil_div64(tile_count(kTiles[0], M, N), ncu), t128 = 0.29 * (double)ceil_div64(tile_count(kTiles[1], M, N), ncu);
+    return t256 <= t128 ? 0 : 1;
 }
 
 // what a call needs: operand forms, pieces of the classes, and where everything lies in the workspace
@@ -346,14 +352,15 @@ struct XentPlan {
         dbias = take(4 * tiles_m * kTiles[t_logits].wm * V);
         // dx has few tiles and a long inner dimension: ranges of it, each with float32 sums of its own
         const int64_t steps = ceil_div64(std::min(P, V), 64) * segments;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(16, steps / 8));
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32, steps / 8));
         t_dx = N <= 64 ? 2 : (tile_count(kTiles[0], N, H) * std::min<int64_t>(most, 4) >= ncu * 3 / 4 ? 0 : 1);
+        const int64_t slots = t_dx == 0 ? ncu : 2 * ncu;
         const int64_t tiles = tile_count(kTiles[t_dx], N, H);
-        // a split's rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.3 per step of a 256 / 128 tile, 4 TB/s)
+        // a split's rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.6 per step of a 256 tile / two 128 tiles, 4 TB/s)
         double least = 1e300;
         splits = 1;
         for (int64_t k = 1; k <= most; ++k) {
-            const double c = (double)ceil_div64(tiles * k, ncu) * (double)steps / (double)k * (t_dx == 0 ? 0.9 : 0.3) + (double)(k * N * H) * 8 / 4e6;
+            const double c = (double)ceil_div64(tiles * k, slots) * (double)steps / (double)k * (t_dx == 0 ? 0.9 : 0.6) + (double)(k * N * H) * 8 / 4e6;
             if (c < least) { least = c; splits = (int)k; }
         }
         acc = take(4 * (int64_t)splits * N * H);
@@ -377,34 +384,39 @@ void xent_gemm(int tile, int splits, XentGemm& p, hipStream_t st) {
 #undef GEMM
 }
 
-// to[plane][rows][ldk] from a plane of the caller; transposed: the caller's memory runs along the rows
-void xent_lay(bool f32, bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane, hipStream_t st) {
-    const dim3 tiles((unsigned)(ceil_div64(rows, 64) * (ldk / 64))), flat((unsigned)ceil_div64(rows * ldk, 2048));
-    if (f32) {
-        if (transposed) hipLaunchKernelGGL(rowops::k_xent_lay_t<float>, tiles, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
-        else hipLaunchKernelGGL(rowops::k_xent_lay<float>, flat, dim3(256), 0, st, (const float*)from, ld, rows, cols, to, ldk, plane);
-    } else {
-        if (transposed) hipLaunchKernelGGL(rowops::k_xent_lay_t<bf16_t>, tiles, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
-        else hipLaunchKernelGGL(rowops::k_xent_lay<bf16_t>, flat, dim3(256), 0, st, (const bf16_t*)from, ld, rows, cols, to, ldk, plane);
+// Operands to lay out, gathered and launched together
+struct Lay {
+    rowops::LayJobs jobs{};
+    void add(bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane) {
+        rowops::LayJob& j = jobs.job[jobs.n++];
+        j = {from, ld, rows, cols, to, ldk, plane, transposed, (int32_t)(transposed ? ceil_div64(rows, 64) * (ldk / 64) : ceil_div64(rows * ldk, 2048))};
     }
-}
+    void launch(bool f32, hipStream_t st) {
+        int64_t blocks = 0;
+        for (int i = 0; i < jobs.n; ++i) blocks += jobs.job[i].blocks;
+        if (blocks == 0) return;
+        if (f32) hipLaunchKernelGGL(rowops::k_xent_lay<float>, dim3((unsigned)blocks), dim3(256), 0, st, jobs);
+        else hipLaunchKernelGGL(rowops::k_xent_lay<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, st, jobs);
+        jobs.n = 0;
+    }
+};
 
 const void* at(const dimn_output_loss* d, const void* base, int64_t elements) { return (const char*)base + elements * (d->type == DIMN_TYPE_F32 ? 4 : 2); }
 
 // the logits' operands of the piece that starts at class c0 and has pv classes
-void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& p, hipStream_t st) {
+void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& p, Lay& lay) {
     const dimn_output_loss* d = q.d;
     p = XentGemm{};
     if (q.x_direct) { p.A = (const uint16_t*)d->x; p.lda = d->x_row; }
     else {
         p.A = (const uint16_t*)(ws + q.x); p.lda = q.Hp; p.a_plane = q.N * q.Hp;
-        if (c0 == 0) xent_lay(q.f32, false, d->x, d->x_row, q.N, q.H, (uint16_t*)(ws + q.x), q.Hp, p.a_plane, st);
+        if (c0 == 0) lay.add(false, d->x, d->x_row, q.N, q.H, (uint16_t*)(ws + q.x), q.Hp, p.a_plane);
     }
     if (q.w_direct) { p.B = (const uint16_t*)at(d, d->kernel, c0 * d->kernel_out); p.ldb = d->kernel_out; }
     else {
         p.B = (const uint16_t*)(ws + q.w); p.ldb = q.Hp; p.b_plane = q.P * q.Hp;
-        if (q.out_in) xent_lay(q.f32, false, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane, st);
-        else xent_lay(q.f32, true, at(d, d->kernel, c0), d->kernel_in, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane, st);
+        if (q.out_in) lay.add(false, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane);
+        else lay.add(true, at(d, d->kernel, c0), d->kernel_in, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane);
     }
     p.M = (int)q.N; p.N = (int)pv;
     p.ksteps = (int)(q.Hp / 64); p.segments = q.segments; p.a_of = q.a_of; p.b_of = q.b_of;
@@ -440,34 +452,51 @@ void xent_tsum(const XentPlan& q, float* tsum, hipStream_t st) {
     const dimn_output_loss* d = q.d;
     if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
 }
+// dx from `splits` float32 sums (0: it is there already) and dbias from `parts` partial sums (0: likewise)
+void xent_finish(const XentPlan& q, char* ws, int splits, int parts, void* dx, int64_t dx_row, float* dbias, hipStream_t st) {
+    rowops::XentFinish f{};
+    f.acc = (const float*)(ws + q.acc); f.split = q.N * q.H; f.splits = splits; f.rows = q.N; f.cols = q.H; f.out = dx; f.ld = dx_row;
+    f.blocks = splits ? (int)ceil_div64(q.N * q.H, 256) : 0;
+    f.part = (const float*)(ws + q.dbias); f.part_ld = q.V; f.parts = parts; f.classes = q.V; f.dbias = dbias;
+    const unsigned blocks = (unsigned)(f.blocks + (dbias && parts ? ceil_div64(q.V, 256) : 0));
+    if (blocks == 0) return;
+    if (q.f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, f);
+    else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, f);
+}
 template <typename T>
 void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
     const dimn_output_loss* d = q.d;
-    float *tsum = (float*)(ws + q.tsum), *dbias_part = (float*)(ws + q.dbias), *acc = (float*)(ws + q.acc);
+    float* tsum = (float*)(ws + q.tsum);
     T* G = (T*)(ws + q.g);
     xent_tsum(q, tsum, st);
     rowops::Thin p = xent_thin_logits(q);
     p.lse = lse; p.dloss = dloss; p.tsum = tsum;
     p.G = G; p.ldg = q.V;
-    p.dbias_part = dbias ? (q.blocks == 1 ? dbias : dbias_part) : nullptr;
+    p.dbias_part = dbias ? (q.blocks == 1 ? dbias : (float*)(ws + q.dbias)) : nullptr;
     xent_thin<T, rowops::XE_GRAD>(q, !q.out_in, q.V, 1, p, st);
-    if (dbias && q.blocks > 1) hipLaunchKernelGGL(rowops::k_xent_dbias, dim3((unsigned)ceil_div64(q.V, 256)), dim3(256), 0, st, dbias_part, q.V, (int)q.blocks, q.V, dbias);
     // dx[n][h] = sum over the classes: the classes are the inner dimension now
     rowops::Thin a{};
     a.A = G; a.lda = q.V; a.B = d->kernel; a.ldb = p.ldb;
-    a.M = q.N; a.N = q.H; a.K = q.V; a.acc = acc;
-    if (q.splits == 1) {
-        a.C = dx; a.ldc = dx_row;
-        xent_thin<T, rowops::XE_STORE>(q, q.out_in, q.H, 1, a, st);
-    } else {
-        xent_thin<T, rowops::XE_ADD>(q, q.out_in, q.H, q.splits, a, st);
-        hipLaunchKernelGGL(rowops::k_xent_finish<T>, dim3((unsigned)ceil_div64(q.N * q.H, 256)), dim3(256), 0, st, acc, q.N * q.H, q.splits, q.N, q.H, (T*)dx, dx_row);
-    }
-    const bool oi = dk_in == 1;
-    const int64_t na = oi ? q.V : q.H, nb = oi ? q.H : q.V;
-    const dim3 grid((unsigned)ceil_div64(nb, 256), (unsigned)ceil_div64(na, 64));
-    if (oi) hipLaunchKernelGGL(rowops::k_xent_thin_dw<T>, grid, dim3(256), 0, st, G, q.V, (const T*)d->x, d->x_row, q.N, na, nb, (T*)dkernel, dk_out);
-    else hipLaunchKernelGGL(rowops::k_xent_thin_dw<T>, grid, dim3(256), 0, st, (const T*)d->x, d->x_row, G, q.V, q.N, na, nb, (T*)dkernel, dk_in);
+    a.M = q.N; a.N = q.H; a.K = q.V; a.acc = (float*)(ws + q.acc);
+    a.C = dx; a.ldc = dx_row;
+    rowops::ThinDw w{};
+    w.n = q.N;
+    if (dk_in == 1) { w.P = G; w.ldp = q.V; w.Q = d->x; w.ldq = d->x_row; w.na = q.V; w.nb = q.H; w.ldc = dk_out; }
+    else { w.P = d->x; w.ldp = d->x_row; w.Q = G; w.ldq = q.V; w.na = q.H; w.nb = q.V; w.ldc = dk_in; }
+    w.C = dkernel;
+    w.tiles_b = (int)ceil_div64(w.nb, 256);
+    const bool vc = q.out_in;
+    const int tiles = (int)ceil_div64(q.H, vc ? 64 : 32), dx_blocks = tiles * q.splits * (int)q.blocks;
+    const dim3 grid((unsigned)(dx_blocks + w.tiles_b * ceil_div64(w.na, 64)));
+#define BOTH(NF, EPI)                                                                                                                                      \
+    do {                                                                                                                                                   \
+        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin_both<T, true, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_blocks, tiles, q.splits);                \
+        else hipLaunchKernelGGL((rowops::k_xent_thin_both<T, false, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_blocks, tiles, q.splits);                  \
+    } while (0)
+    if (q.splits == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(4, rowops::XE_STORE); }
+    else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
+#undef BOTH
+    xent_finish(q, ws, q.splits == 1 ? 0 : q.splits, q.blocks == 1 ? 0 : (int)q.blocks, dx, dx_row, dbias, st);
 }
 
 int xent_check(const char* who, const dimn_output_loss* d) {
@@ -497,7 +526,7 @@ extern "C" int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, in
     OnDevice on;
     CHK(on.enter(who, d->device_id));
     XentPlan q;
-    q.make(d, grad != 0, compute_units());
+    q.make(d, grad != 0, compute_units(d->device_id));
     *bytes = (int64_t)q.bytes;
     return DIMN_OK;
 }
@@ -511,7 +540,7 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     CHK(on.enter(who, d->device_id));
     hipStream_t st = (hipStream_t)stream;
     XentPlan q;
-    q.make(d, false, compute_units());
+    q.make(d, false, compute_units(d->device_id));
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
     const Tile& t = kTiles[q.t_logits];
@@ -524,7 +553,9 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
         else xent_thin<bf16_t, rowops::XE_LSE>(q, !q.out_in, q.V, 1, p, st);
     } else for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
         XentGemm p;
-        xent_logits(q, ws, c0, std::min(q.P, q.V - c0), p, st);
+        Lay lay;
+        xent_logits(q, ws, c0, std::min(q.P, q.V - c0), p, lay);
+        lay.launch(q.f32, st);
         p.part = (float2*)(ws + q.part) + c0 / t.bn * q.N;
         if (!q.labels) p.part_t = (float2*)(ws + q.part_t) + c0 / t.bn * q.N;
         p.picked = (float*)(ws + q.picked);
@@ -554,7 +585,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
     CHK(on.enter(who, d->device_id));
     hipStream_t st = (hipStream_t)stream;
     XentPlan q;
-    q.make(d, true, compute_units());
+    q.make(d, true, compute_units(d->device_id));
     if (d->rows == 0) return dimn_fail(DIMN_ERR_ARG, "%s: no rows", who);
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
@@ -566,14 +597,22 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
     }
     float* tsum = (float*)(ws + q.tsum);
     xent_tsum(q, tsum, st);
+    Lay lay;
     uint16_t* xt = (uint16_t*)(ws + q.xt);
     const int64_t xt_plane = q.H * q.Np;
-    xent_lay(q.f32, true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane, st);
+    lay.add(true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane);
     const bool dk_out_in = dkernel_in == 1;
     for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
         const int64_t pv = std::min(q.P, q.V - c0), ldg = up(pv, 64);
         XentGemm p;
-        xent_logits(q, ws, c0, pv, p, st);
+        xent_logits(q, ws, c0, pv, p, lay);
+        uint16_t* wt = (uint16_t*)(ws + q.wt);
+        const int64_t wt_plane = q.H * ldg;
+        if (!q.wt_direct) {
+            if (q.out_in) lay.add(true, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, q.H, pv, wt, ldg, wt_plane);
+            else lay.add(false, at(d, d->kernel, c0), d->kernel_in, q.H, pv, wt, ldg, wt_plane);
+        }
+        lay.launch(q.f32, st);
         p.lse = lse; p.dloss = dloss; p.tsum = tsum;
         p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
         p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
@@ -583,12 +622,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         XentGemm a{};
         a.A = p.G; a.lda = ldg; a.a_plane = p.g_plane;
         if (q.wt_direct) { a.B = (const uint16_t*)at(d, d->kernel, c0); a.ldb = d->kernel_in; }
-        else {
-            uint16_t* wt = (uint16_t*)(ws + q.wt);
-            a.B = wt; a.ldb = ldg; a.b_plane = q.H * ldg;
-            if (q.out_in) xent_lay(q.f32, true, at(d, d->kernel, c0 * d->kernel_out), d->kernel_out, q.H, pv, wt, ldg, a.b_plane, st);
-            else xent_lay(q.f32, false, at(d, d->kernel, c0), d->kernel_in, q.H, pv, wt, ldg, a.b_plane, st);
-        }
+        else { a.B = wt; a.ldb = ldg; a.b_plane = wt_plane; }
         a.M = (int)q.N; a.N = (int)q.H;
         a.ksteps = (int)(ldg / 64); a.segments = q.segments; a.a_of = q.a_of; a.b_of = q.b_of;
         a.acc = (float*)(ws + q.acc); a.acc_split = q.N * q.H; a.acc_first = c0 == 0;
@@ -609,12 +643,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         }
         xent_gemm<rowops::XE_STORE>(pick_tile(w.M, w.N, q.ncu), 1, w, st);
     }
-    const unsigned blocks = (unsigned)ceil_div64(q.N * q.H, 256);
-    if (q.f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (float*)dx, dx_row);
-    else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, (const float*)(ws + q.acc), q.N * q.H, q.splits, q.N, q.H, (bf16_t*)dx, dx_row);
-    if (dbias)
-        hipLaunchKernelGGL(rowops::k_xent_dbias, dim3((unsigned)ceil_div64(q.V, 256)), dim3(256), 0, st, (const float*)(ws + q.dbias), q.V,
-                           (int)(q.tiles_m * kTiles[q.t_logits].wm), q.V, dbias);
+    xent_finish(q, ws, q.splits, (int)(q.tiles_m * kTiles[q.t_logits].wm), dx, dx_row, dbias, st);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
 }

@@ -62,46 +62,55 @@ __device__ __forceinline__ void lay_store(const T (&v)[8], uint16_t* to, int64_t
 #pragma unroll
     for (int pl = 0; pl < PL; ++pl) *(u16x8*)(to + pl * plane) = o[pl];
 }
-// from: [r][k], k contiguous.  One thread per eight k's.
+// One operand to lay out.  Not transposed: from is [r][k] with k contiguous, a thread takes eight k's.  Transposed: from is [k][r] with r contiguous
+// (row stride `ld` along k), 64 x 64 tiles through LDS, whose line of 65 (float) / 66 (bfloat16) elements spreads a column over the banks.
+struct LayJob {
+    const void* from; int64_t ld, rows, cols;
+    uint16_t* to; int64_t ldk, plane;
+    int32_t transposed, blocks;
+};
+struct LayJobs { LayJob job[4]; int32_t n; };                    // (one launch for everything a piece needs: each is a few microseconds of copying)
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_lay(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
-    if (e >= rows * ldk) return;
-    const int64_t r = e / ldk, k = e - r * ldk;
-    const T* p = from + r * ld + k;
-    T v[8];
-    if (k + 8 <= cols) {
-        const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = x[j];
-    } else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < cols ? p[j] : (T)0;
-    lay_store<T>(v, to + e, plane);
-}
-// from: [k][r], r contiguous (row stride `ld` along k).  64 x 64 tiles through LDS; a line of 65 (float) / 66 (bfloat16) elements spreads a column
-// over the banks.
-template <typename T>
-__global__ __launch_bounds__(256) void k_xent_lay_t(const T* __restrict__ from, int64_t ld, int64_t rows, int64_t cols, uint16_t* __restrict__ to, int64_t ldk, int64_t plane) {
+__global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
     constexpr int LD = sizeof(T) == 4 ? 65 : 66;
     __shared__ T tile[64][LD];
-    const int64_t tiles_k = ldk >> 6;
-    const int64_t tr = blockIdx.x / tiles_k, tk = blockIdx.x - tr * tiles_k;
+    int block = blockIdx.x, w = 0;
+    while (w + 1 < all.n && block >= all.job[w].blocks) { block -= all.job[w].blocks; ++w; }
+    const LayJob& p = all.job[w];
+    const T* from = (const T*)p.from;
+    if (!p.transposed) {
+        const int64_t e = ((int64_t)block * 256 + threadIdx.x) * 8;
+        if (e >= p.rows * p.ldk) return;
+        const int64_t r = e / p.ldk, k = e - r * p.ldk;
+        const T* q = from + r * p.ld + k;
+        T v[8];
+        if (k + 8 <= p.cols) {
+            const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)q;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = x[j];
+        } else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = k + j < p.cols ? q[j] : (T)0;
+        lay_store<T>(v, p.to + e, p.plane);
+        return;
+    }
+    const int64_t tiles_k = p.ldk >> 6;
+    const int64_t tr = block / tiles_k, tk = block - tr * tiles_k;
     const int64_t r0 = tr * 64, k0 = tk * 64;
     const int q = threadIdx.x & 7, s = threadIdx.x >> 3;         // 8 pieces of eight x 32 lines
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int64_t k = k0 + s + 32 * i, r = r0 + 8 * q;
-        const T* p = from + k * ld + r;
+        const T* f = from + k * p.ld + r;
         T v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (k < cols) {
-            if (r + 8 <= rows) {
-                const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)p;
+        if (k < p.cols) {
+            if (r + 8 <= p.rows) {
+                const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] = x[j];
             } else
 #pragma unroll
-                for (int j = 0; j < 8; ++j) if (r + j < rows) v[j] = p[j];
+                for (int j = 0; j < 8; ++j) if (r + j < p.rows) v[j] = f[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) tile[s + 32 * i][8 * q + j] = v[j];
@@ -110,11 +119,11 @@ __global__ __launch_bounds__(256) void k_xent_lay_t(const T* __restrict__ from, 
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int64_t r = r0 + s + 32 * i;
-        if (r >= rows) continue;
+        if (r >= p.rows) continue;
         T v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = tile[8 * q + j][s + 32 * i];
-        lay_store<T>(v, to + r * ldk + k0 + 8 * q, plane);
+        lay_store<T>(v, p.to + r * p.ldk + k0 + 8 * q, p.plane);
     }
 }
 
@@ -576,26 +585,35 @@ __global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t 
     }
 }
 
-// out[m][n] = sum of the splits' float32 sums, in order, rounded once.  A thread takes one element: neighbours are neighbours in every split.
+// What is left of a backward pass, in one launch: out[m][n] = the sum of the splits' float32 sums (splits = 0: nothing), dbias = the sum of the
+// partial column sums (dbias = NULL: nothing), each added in order and rounded once.  A thread takes one element: neighbours are neighbours in
+// every split.
+struct XentFinish {
+    const float* acc; int64_t split; int32_t splits, blocks;     // blocks: workgroups of the first part
+    int64_t rows, cols;
+    void* out; int64_t ld;
+    const float* part; int64_t part_ld; int32_t parts;
+    int64_t classes;
+    float* dbias;
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_finish(const float* __restrict__ acc, int64_t split, int splits, int64_t rows, int64_t cols, T* __restrict__ out, int64_t ld) {
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= rows * cols) return;
+__global__ __launch_bounds__(256) void k_xent_finish(const XentFinish p) {
+    if ((int)blockIdx.x < p.blocks) {
+        const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (e >= p.rows * p.cols) return;
+        float s = 0.f;
+#pragma unroll 8
+        for (int k = 0; k < p.splits; ++k) s += p.acc[k * p.split + e];
+        const int64_t m = e / p.cols, n = e - m * p.cols;
+        if constexpr (sizeof(T) == 4) ((float*)p.out)[m * p.ld + n] = s; else ((uint16_t*)p.out)[m * p.ld + n] = to_bf16(s);
+        return;
+    }
+    const int64_t c = (int64_t)((int)blockIdx.x - p.blocks) * 256 + threadIdx.x;
+    if (c >= p.classes) return;
     float s = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < splits; ++k) s += acc[k * split + e];
-    const int64_t m = e / cols, n = e - m * cols;
-    if constexpr (sizeof(T) == 4) out[m * ld + n] = s; else out[m * ld + n] = to_bf16(s);
-}
-
-// dbias = the partial column sums, added in order
-__global__ __launch_bounds__(256) void k_xent_dbias(const float* __restrict__ part, int64_t ld, int parts, int64_t classes, float* __restrict__ dbias) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c >= classes) return;
-    float s = 0.f;
-#pragma unroll 8
-    for (int k = 0; k < parts; ++k) s += part[k * ld + c];
-    dbias[c] = s;
+    for (int k = 0; k < p.parts; ++k) s += p.part[k * p.part_ld + c];
+    p.dbias[c] = s;
 }
 
 }  // namespace rowops

@@ -27,8 +27,8 @@ struct Thin {
     float2* part; float2* part_t; float* picked;          // as XentGemm (a tile: 32 / 64 classes)
     const float* lse; const float* dloss; const float* tsum;
     void* G; int64_t ldg;                      // [M][ldg] of T
-    float* dbias_part;                         // [gridDim.z][N]
-    float* acc;                                // XE_ADD: [gridDim.y][M][N] float32
+    float* dbias_part;                         // [row blocks][N]
+    float* acc;                                // XE_ADD: [k-ranges][M][N] float32
     void* C; int64_t ldc;                      // XE_STORE: [M][N] of T
 };
 
@@ -36,14 +36,15 @@ template <typename T> struct Four;             // four consecutive elements of a
 template <> struct Four<float> { typedef f32x4u vec; };
 template <> struct Four<bf16_t> { typedef u16x4u vec; };
 
+// (class tile, k-range, row block) of one workgroup; `ranges` k-ranges in all
 template <typename T, bool VC, int NF, int EPI>
-__global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
+__device__ __forceinline__ void thin_product(const Thin& p, int tile, int range, int ranges, int block) {
     constexpr bool BF = sizeof(T) == 2, WIDE = BF && !VC;      // WIDE: the 16x16x32 instruction, eight k's per lane
     constexpr int EL = WIDE ? 8 : 4, KS = 4 * EL, NS = VC ? 4 : 2, CW = VC ? 64 : 32, ROWS = 16 * NF, LD = CW + 4;
     constexpr int U = NF > 2 ? 2 : 4;                           // chunks requested together
     __shared__ __attribute__((aligned(16))) float red[2][ROWS][LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lj = lane >> 4;
-    const int64_t c0 = (int64_t)blockIdx.x * CW, m0 = (int64_t)blockIdx.z * ROWS;
+    const int64_t c0 = (int64_t)tile * CW, m0 = (int64_t)block * ROWS;
     const T* A = (const T*)p.A;
     const T* B = (const T*)p.B;
     const T* arow[NF];
@@ -107,8 +108,8 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
         }
     };
     // this workgroup's range of whole chunks; the chunk that crosses K belongs to the last range
-    const int64_t whole = p.K / KS, S = gridDim.y;
-    const int64_t cbeg = whole * blockIdx.y / S, cend = whole * (blockIdx.y + 1) / S;
+    const int64_t whole = p.K / KS;
+    const int64_t cbeg = whole * range / ranges, cend = whole * (range + 1) / ranges;
     // whole rounds of U consecutive chunks per wave (256 bytes of a class row at a time), then single chunks
     const int64_t rounds = (cend - cbeg) / (4 * U);
     for (int64_t i = 0; i < rounds; ++i) {
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
         for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
     }
     for (int64_t c = cbeg + rounds * 4 * U + wave; c < cend; c += 4) { request(c * KS, a[0], b[0]); multiply(a[0], b[0]); }
-    if (whole * KS < p.K && blockIdx.y == S - 1 && wave == (whole & 3)) {
+    if (whole * KS < p.K && range == ranges - 1 && wave == (whole & 3)) {
         const int64_t k = whole * KS;
 #pragma unroll
         for (int q = 0; q < NB; ++q)
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
             int before, upto;
             const int64_t k = group(pos0 + 4 * q, before, upto);
             if constexpr (EPI == XE_ADD) {
-                float* to = p.acc + ((int64_t)blockIdx.y * p.M + m) * p.N + k;
+                float* to = p.acc + ((int64_t)range * p.M + m) * p.N + k;
                 if (before == 0 && upto == 4) *(f32x4u*)to = z[q];
                 else
 #pragma unroll
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
 #pragma unroll
             for (int o = 1; o < PT; o <<= 1) { s += __shfl_xor(s, o); st += __shfl_xor(st, o); stz += __shfl_xor(stz, o); }
             if (have && tid % PT == 0) {
-                const int64_t at = (int64_t)blockIdx.x * p.M + m;
+                const int64_t at = (int64_t)tile * p.M + m;
                 p.part[at] = make_float2(top, s);
                 if (!labels) p.part_t[at] = make_float2(st, stz);
             }
@@ -304,7 +305,7 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
                 const int64_t k = group(pos & ~3, before, upto);
 #pragma unroll
                 for (int w = 1; w < ST; ++w) s += red[1][w][pos];
-                if ((pos & 3) >= before && (pos & 3) < upto) p.dbias_part[(int64_t)blockIdx.z * p.N + k + (pos & 3)] = s;
+                if ((pos & 3) >= before && (pos & 3) < upto) p.dbias_part[(int64_t)block * p.N + k + (pos & 3)] = s;
             }
         }
     }
@@ -313,13 +314,21 @@ __global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
 // dW for few rows: C[a][b] = sum_n P[n][a] Q[n][b], both operands with their output index contiguous, C's b contiguous (Keras order: P = x, Q = G;
 // the transposed order: P = G, Q = x).  Writing C bounds it.  A wave owns 64 x 64 of C: a lane loads four consecutive a's and b's of one n, element
 // j belongs to set j (sixteen indices four apart) -- sixteen instructions per pair of 16-byte loads, and a lane ends up with four consecutive b's.
+struct ThinDw {
+    const void* P; int64_t ldp; const void* Q; int64_t ldq;
+    int64_t n, na, nb;
+    void* C; int64_t ldc;
+    int32_t tiles_b;                           // workgroups along b (256 columns each)
+};
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_thin_dw(const T* __restrict__ P, int64_t ldp, const T* __restrict__ Q, int64_t ldq, int64_t n, int64_t na, int64_t nb,
-                                                      T* __restrict__ C, int64_t ldc) {
+__device__ __forceinline__ void thin_dw(const ThinDw& p, int tile) {
+    const T *P = (const T*)p.P, *Q = (const T*)p.Q;
+    T* C = (T*)p.C;
+    const int64_t ldp = p.ldp, ldq = p.ldq, n = p.n, na = p.na, nb = p.nb, ldc = p.ldc;
     constexpr bool BF = sizeof(T) == 2;
     typedef typename Four<T>::vec vec;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lj = lane >> 4;
-    const int64_t a0 = (int64_t)blockIdx.y * 64, b0 = ((int64_t)blockIdx.x * 4 + wave) * 64;
+    const int64_t a0 = (int64_t)(tile / p.tiles_b) * 64, b0 = ((int64_t)(tile % p.tiles_b) * 4 + wave) * 64;
     if (b0 >= nb) return;
     auto start = [](int64_t from, int64_t end) { return from < end - 4 ? from : end - 4; };      // (na, nb >= 4: the caller's rule)
     const int64_t ca = start(a0 + 4 * li, na), cb = start(b0 + 4 * li, nb);
@@ -383,6 +392,24 @@ __global__ __launch_bounds__(256) void k_xent_thin_dw(const T* __restrict__ P, i
                 for (int j = 0; j < 4; ++j) if (cb + j >= b0 + 4 * li) to[j] = o[j];
         }
     }
+}
+
+// grid (class tiles, k-ranges, row blocks)
+template <typename T, bool VC, int NF, int EPI>
+__global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
+    thin_product<T, VC, NF, EPI>(p, blockIdx.x, blockIdx.y, gridDim.y, blockIdx.z);
+}
+
+// dx and dW in one launch: both read G and neither waits for the other, and with few rows each is mostly latency.  The first `dx_blocks` workgroups
+// multiply for dx (tiles x ranges x row blocks, flattened), the others for dW.
+template <typename T, bool VC, int NF, int EPI>
+__global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const ThinDw w, int dx_blocks, int tiles, int ranges) {
+    int b = blockIdx.x;
+    if (b < dx_blocks) {
+        const int per = tiles * ranges, block = b / per;
+        b -= block * per;
+        thin_product<T, VC, NF, EPI>(a, b % tiles, b / tiles, ranges, block);
+    } else thin_dw<T>(w, b - dx_blocks);
 }
 
 }  // namespace rowops

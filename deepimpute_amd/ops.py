@@ -20,13 +20,13 @@ from . import _cabi, _lib
 from .engine import DimnError
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
-_f = None
+_f = {}
 
 
 def _fns():
-    global _f
-    if _f is None:
-        _f = _lib.load()
+    """The bound entry points (loaded at the first call)."""
+    if not _f:
+        _f.update(_lib.load())
     return _f
 
 
@@ -61,7 +61,7 @@ def _f32(what, name, t, shape):
     """A contiguous float32 tensor of exactly `shape`, or None."""
     if t is None:
         return None
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         raise ValueError("%s: %s must be float32, got %s" % (what, name, t.dtype))
     if t.shape != shape:
         raise ValueError("%s: %s has shape %s, expected %s" % (what, name, tuple(t.shape), tuple(shape)))
@@ -76,12 +76,14 @@ def _planes(x, grouped):
     """x as [groups][rows][width]: (tensor, groups, rows, group stride, row stride)."""
     if x.stride(-1) != 1 and x.shape[-1] > 1:
         x = x.contiguous()
+    shape = x.shape
     if grouped:
-        if x.dim() != 3:
-            x = x.reshape(x.shape[0], math.prod(x.shape[1:-1]), x.shape[-1])
-        return x, x.shape[0], x.shape[1], x.stride(0), x.stride(1)
-    if x.dim() != 2:
-        x = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+        if len(shape) != 3:
+            x = x.reshape(shape[0], math.prod(shape[1:-1]), shape[-1])
+        s = x.stride()
+        return x, shape[0], x.shape[1], s[0], s[1]
+    if len(shape) != 2:
+        x = x.reshape(math.prod(shape[:-1]), shape[-1])
     return x, 1, x.shape[0], 0, x.stride(0)
 
 
@@ -108,13 +110,15 @@ def layer_norm(x, gamma=None, beta=None, eps=1e-3):
     dev = _device("layer_norm", x, gamma, beta)
     if not eps >= 0:
         raise ValueError("layer_norm: eps %r is negative or not a number" % (eps,))
-    shape, width = x.shape, x.shape[-1]
+    shape = x.shape
+    width = shape[-1]
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    stats = torch.empty((2,) + shape[:-1], dtype=torch.float32, device=x.device)
-    mean, rstd = stats.unbind(0)
+    mean, rstd = y.new_empty((2,) + shape[:-1], dtype=torch.float32).unbind(0)
     x, groups, rows, xg, xr = _planes(x, grouped)
-    _check(_fns()["layer_norm"](dev, _stream(dev), kind, groups, rows, width, x.data_ptr(), xg, xr, _ptr(gamma), _ptr(beta), eps,
-                                y.data_ptr(), rows * width, width, mean.data_ptr(), rstd.data_ptr()))
+    rc = _fns()["layer_norm"](dev, _stream(dev), kind, groups, rows, width, x.data_ptr(), xg, xr, _ptr(gamma), _ptr(beta), eps,
+                              y.data_ptr(), rows * width, width, mean.data_ptr(), rstd.data_ptr())
+    if rc:
+        _check(rc)
     return y, mean, rstd
 
 
@@ -142,9 +146,8 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None):
         if len(_norm_space) > 4096:
             _norm_space.clear()
         need = _norm_space[key] = n.value
-    work = torch.empty(need, dtype=torch.uint8, device=x.device)
-    params = torch.empty((2,) + ((groups, width) if grouped else (width,)), dtype=torch.float32, device=x.device)
-    dgamma, dbeta = params.unbind(0)
+    work = dx.new_empty(need, dtype=torch.uint8)
+    dgamma, dbeta = dx.new_empty((2, groups, width) if grouped else (2, width), dtype=torch.float32).unbind(0)
     _check(_fns()["layer_norm_grad"](dev, _stream(dev), kind, groups, rows, width, dy.data_ptr(), dg, dr, x.data_ptr(), xg, xr,
                                      mean.data_ptr(), rstd.data_ptr(), _ptr(gamma), dx.data_ptr(), rows * width, width,
                                      dgamma.data_ptr(), dbeta.data_ptr(), work.data_ptr(), need))
