@@ -253,9 +253,9 @@ struct XentPlan {
     bool x_direct, w_direct, wt_direct;
     int t_logits;
     int64_t tiles_m, tiles_n;                 // logits
-    int t_dx, splits;
+    int t_dx, splits, t_dw, dw_splits;
     bool thin; int nf; int64_t blocks;        // few rows: dimn_xent_thin.h; 16 nf rows per block
-    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, dbias, acc, bytes;
+    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, dbias, acc, acc_w, bytes;
 
     // The largest piece allowed, or a smaller one whose 256 x 256 tiles fill the device in whole rounds: a piece of 84 class tiles at 16 row tiles
     // takes 6 rounds of 256 workgroups where 96 class tiles take the same six (64000 classes: 16 rounds instead of 18, 8 instead of 9 for dW).
@@ -273,6 +273,18 @@ struct XentPlan {
         }
         return best * 256;
     }
+    // Ranges of the inner dimension of an M x N product: its rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.6 per
+    // step of a 256 tile / two 128 tiles, 4 TB/s).
+    int split_count(int tile, int64_t M, int64_t N_, int64_t steps) const {
+        const int64_t tiles = tile_count(kTiles[tile], M, N_), slots = tile == 0 ? ncu : 2 * ncu, most = std::max<int64_t>(1, std::min<int64_t>(32, steps / 8));
+        double least = 1e300;
+        int best = 1;
+        for (int64_t k = 1; k <= most; ++k) {
+            const double c = (double)ceil_div64(tiles * k, slots) * (double)steps / (double)k * (tile == 0 ? 0.9 : 0.6) + (k > 1 ? 4.0 + (double)(k * M * N_) * 8 / 4e6 : 0.0);
+            if (c < least) { least = c; best = (int)k; }
+        }
+        return best;
+    }
     // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 256 .. 4096 and 300 .. 32000
     // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles)
     bool prefers_thin() const {
@@ -283,8 +295,9 @@ struct XentPlan {
             g = (x_direct ? 0 : 5) + (w_direct ? 0 : 5 + hv * (f32 ? 3.9e-6 : 0.9e-6));
             g += std::max(work * (f32 ? 8e-6 : 2.1e-6) * 1e-3, steps) - 4;
         } else {
-            t = work * (f32 ? 68e-6 : 24e-6) * 1e-3 + 0.03 * (double)N;
-            g = 30 + hv * (f32 ? 10e-6 : 2e-6) + std::max(work * (f32 ? 40e-6 : 8.6e-6) * 1e-3, steps);
+            const double nv = (double)N * (double)V * 1e-6 / 4;  // (G is written and read: 12 / 6 bytes an entry, laid out for the large products 24 / 8)
+            t = work * (f32 ? 62e-6 : 22e-6) * 1e-3 + 0.01 * (double)N + nv * (f32 ? 12 : 6);
+            g = 25 + hv * (f32 ? 10e-6 : 2e-6) + std::max(work * (f32 ? 30e-6 : 7e-6) * 1e-3, steps) + nv * (f32 ? 24 : 8);
         }
         return t < g;
     }
@@ -334,6 +347,9 @@ struct XentPlan {
             const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
             splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, 2 * ncu / wgs, chunks / 2}));
             acc = take(4 * (int64_t)splits * N * H);
+            const int64_t wt_wgs = ceil_div64(H, 64) * ceil_div64(V, 256);        // (dW: 64 x 256 of the product per workgroup, either way round)
+            dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)32, 2 * ncu / wt_wgs, N / 128}));
+            acc_w = dw_splits > 1 ? take(4 * (int64_t)dw_splits * H * V) : 0;
             return;
         }
         x = x_direct ? 0 : take(2 * planes * N * Hp);
@@ -350,19 +366,14 @@ struct XentPlan {
         gt = take(2 * planes * P * Np);
         tsum = take(4 * N);
         dbias = take(4 * tiles_m * kTiles[t_logits].wm * V);
-        // dx has few tiles and a long inner dimension: ranges of it, each with float32 sums of its own
-        const int64_t steps = ceil_div64(std::min(P, V), 64) * segments;
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(32, steps / 8));
+        // dx has few tiles and a long inner dimension, so has dW of a narrow layer: ranges of it, each with float32 sums of its own
+        const int64_t pv = std::min(P, V);
+        const int64_t steps = ceil_div64(pv, 64) * segments, most = std::min<int64_t>(32, steps / 8);
         t_dx = N <= 64 ? 2 : (tile_count(kTiles[0], N, H) * std::min<int64_t>(most, 4) >= ncu * 3 / 4 ? 0 : 1);
-        const int64_t slots = t_dx == 0 ? ncu : 2 * ncu;
-        const int64_t tiles = tile_count(kTiles[t_dx], N, H);
-        // a split's rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.6 per step of a 256 tile / two 128 tiles, 4 TB/s)
-        double least = 1e300;
-        splits = 1;
-        for (int64_t k = 1; k <= most; ++k) {
-            const double c = (double)ceil_div64(tiles * k, slots) * (double)steps / (double)k * (t_dx == 0 ? 0.9 : 0.6) + (double)(k * N * H) * 8 / 4e6;
-            if (c < least) { least = c; splits = (int)k; }
-        }
+        splits = split_count(t_dx, N, H, steps);
+        t_dw = pick_tile(d->kernel_in == 1 ? pv : H, d->kernel_in == 1 ? H : pv, ncu);
+        dw_splits = split_count(t_dw, d->kernel_in == 1 ? pv : H, d->kernel_in == 1 ? H : pv, Np / 64 * segments);
+        acc_w = dw_splits > 1 ? take(4 * (int64_t)dw_splits * H * pv) : 0;
         acc = take(4 * (int64_t)splits * N * H);
     }
 };
@@ -452,16 +463,18 @@ void xent_tsum(const XentPlan& q, float* tsum, hipStream_t st) {
     const dimn_output_loss* d = q.d;
     if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
 }
-// dx from `splits` float32 sums (0: it is there already) and dbias from `parts` partial sums (0: likewise)
-void xent_finish(const XentPlan& q, char* ws, int splits, int parts, void* dx, int64_t dx_row, float* dbias, hipStream_t st) {
-    rowops::XentFinish f{};
-    f.acc = (const float*)(ws + q.acc); f.split = q.N * q.H; f.splits = splits; f.rows = q.N; f.cols = q.H; f.out = dx; f.ld = dx_row;
-    f.blocks = splits ? (int)ceil_div64(q.N * q.H, 256) : 0;
-    f.part = (const float*)(ws + q.dbias); f.part_ld = q.V; f.parts = parts; f.classes = q.V; f.dbias = dbias;
-    const unsigned blocks = (unsigned)(f.blocks + (dbias && parts ? ceil_div64(q.V, 256) : 0));
+rowops::SplitSum split_sum(const float* acc, int splits, int64_t rows, int64_t cols, void* out, int64_t ld) {
+    return {acc, rows * cols, splits, (int32_t)ceil_div64(rows * cols, 256), rows, cols, out, ld};
+}
+void xent_finish(bool f32, const rowops::XentFinish& f, hipStream_t st) {
+    const unsigned blocks = (unsigned)(f.m[0].blocks + f.m[1].blocks + (f.dbias && f.parts ? ceil_div64(f.classes, 256) : 0));
     if (blocks == 0) return;
-    if (q.f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, f);
+    if (f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, f);
     else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, f);
+}
+// the bias gradient from `parts` partial sums in the workspace
+void finish_bias(rowops::XentFinish& f, const XentPlan& q, char* ws, int parts, float* dbias) {
+    f.part = (const float*)(ws + q.dbias); f.part_ld = q.V; f.parts = parts; f.classes = q.V; f.dbias = dbias;
 }
 template <typename T>
 void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
@@ -485,9 +498,12 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     else { w.P = d->x; w.ldp = d->x_row; w.Q = G; w.ldq = q.V; w.na = q.H; w.nb = q.V; w.ldc = dk_in; }
     w.C = dkernel;
     w.tiles_b = (int)ceil_div64(w.nb, 256);
+    w.tiles = w.tiles_b * (int)ceil_div64(w.na, 64);
+    w.ranges = q.dw_splits;
+    w.acc = (float*)(ws + q.acc_w);
     const bool vc = q.out_in;
     const int tiles = (int)ceil_div64(q.H, vc ? 64 : 32), dx_blocks = tiles * q.splits * (int)q.blocks;
-    const dim3 grid((unsigned)(dx_blocks + w.tiles_b * ceil_div64(w.na, 64)));
+    const dim3 grid((unsigned)(dx_blocks + w.tiles * w.ranges));
 #define BOTH(NF, EPI)                                                                                                                                      \
     do {                                                                                                                                                   \
         if (vc) hipLaunchKernelGGL((rowops::k_xent_thin_both<T, true, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_blocks, tiles, q.splits);                \
@@ -496,7 +512,11 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     if (q.splits == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(4, rowops::XE_STORE); }
     else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
 #undef BOTH
-    xent_finish(q, ws, q.splits == 1 ? 0 : q.splits, q.blocks == 1 ? 0 : (int)q.blocks, dx, dx_row, dbias, st);
+    rowops::XentFinish f{};
+    if (q.splits > 1) f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
+    if (w.ranges > 1) f.m[1] = split_sum(w.acc, w.ranges, w.na, w.nb, w.C, w.ldc);
+    if (q.blocks > 1) finish_bias(f, q, ws, (int)q.blocks, dbias);
+    xent_finish(q.f32, f, st);
 }
 
 int xent_check(const char* who, const dimn_output_loss* d) {
@@ -641,9 +661,18 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
             w.B = gt; w.ldb = q.Np; w.b_plane = p.gt_plane; w.N = (int)pv;
             w.C = const_cast<void*>(at(d, dkernel, c0)); w.ldc = dkernel_in;
         }
-        xent_gemm<rowops::XE_STORE>(pick_tile(w.M, w.N, q.ncu), 1, w, st);
+        if (q.dw_splits > 1) {
+            w.acc = (float*)(ws + q.acc_w); w.acc_split = (int64_t)w.M * w.N; w.acc_first = 1;
+            xent_gemm<rowops::XE_ADD>(q.t_dw, q.dw_splits, w, st);
+            rowops::XentFinish f{};
+            f.m[0] = split_sum(w.acc, q.dw_splits, w.M, w.N, w.C, w.ldc);
+            xent_finish(q.f32, f, st);
+        } else xent_gemm<rowops::XE_STORE>(q.t_dw, 1, w, st);
     }
-    xent_finish(q, ws, q.splits, (int)(q.tiles_m * kTiles[q.t_logits].wm), dx, dx_row, dbias, st);
+    rowops::XentFinish f{};
+    f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
+    finish_bias(f, q, ws, (int)(q.tiles_m * kTiles[q.t_logits].wm), dbias);
+    xent_finish(q.f32, f, st);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
 }

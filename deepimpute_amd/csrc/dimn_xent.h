@@ -585,30 +585,38 @@ __global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t 
     }
 }
 
-// What is left of a backward pass, in one launch: out[m][n] = the sum of the splits' float32 sums (splits = 0: nothing), dbias = the sum of the
-// partial column sums (dbias = NULL: nothing), each added in order and rounded once.  A thread takes one element: neighbours are neighbours in
-// every split.
-struct XentFinish {
-    const float* acc; int64_t split; int32_t splits, blocks;     // blocks: workgroups of the first part
+// What is left of a backward pass, in one launch: out[m][n] = the sum of the splits' float32 sums for up to two matrices (dx, dW), dbias = the sum of
+// the partial column sums, each added in order and rounded once.  A thread takes one element: neighbours are neighbours in every split.
+struct SplitSum {
+    const float* acc; int64_t split; int32_t splits, blocks;     // [splits][rows][cols], `split` elements apart; blocks = 0: nothing to do
     int64_t rows, cols;
     void* out; int64_t ld;
+};
+struct XentFinish {
+    SplitSum m[2];
     const float* part; int64_t part_ld; int32_t parts;
     int64_t classes;
     float* dbias;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_finish(const XentFinish p) {
-    if ((int)blockIdx.x < p.blocks) {
-        const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-        if (e >= p.rows * p.cols) return;
-        float s = 0.f;
+    int block = blockIdx.x;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if (block < p.m[w].blocks) {
+            const SplitSum& q = p.m[w];
+            const int64_t e = (int64_t)block * 256 + threadIdx.x;
+            if (e >= q.rows * q.cols) return;
+            float s = 0.f;
 #pragma unroll 8
-        for (int k = 0; k < p.splits; ++k) s += p.acc[k * p.split + e];
-        const int64_t m = e / p.cols, n = e - m * p.cols;
-        if constexpr (sizeof(T) == 4) ((float*)p.out)[m * p.ld + n] = s; else ((uint16_t*)p.out)[m * p.ld + n] = to_bf16(s);
-        return;
+            for (int k = 0; k < q.splits; ++k) s += q.acc[k * q.split + e];
+            const int64_t m = e / q.cols, n = e - m * q.cols;
+            if constexpr (sizeof(T) == 4) ((float*)q.out)[m * q.ld + n] = s; else ((uint16_t*)q.out)[m * q.ld + n] = to_bf16(s);
+            return;
+        }
+        block -= p.m[w].blocks;
     }
-    const int64_t c = (int64_t)((int)blockIdx.x - p.blocks) * 256 + threadIdx.x;
+    const int64_t c = (int64_t)block * 256 + threadIdx.x;
     if (c >= p.classes) return;
     float s = 0.f;
 #pragma unroll 8

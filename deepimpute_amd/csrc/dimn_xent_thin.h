@@ -318,13 +318,15 @@ struct ThinDw {
     const void* P; int64_t ldp; const void* Q; int64_t ldq;
     int64_t n, na, nb;
     void* C; int64_t ldc;
-    int32_t tiles_b;                           // workgroups along b (256 columns each)
+    int32_t tiles_b, tiles;                    // workgroups along b (256 columns each), in all
+    int32_t ranges; float* acc;                // ranges > 1: range r of the rows leaves its float32 sums in acc[r][na][nb]
 };
 template <typename T>
-__device__ __forceinline__ void thin_dw(const ThinDw& p, int tile) {
+__device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const T *P = (const T*)p.P, *Q = (const T*)p.Q;
     T* C = (T*)p.C;
-    const int64_t ldp = p.ldp, ldq = p.ldq, n = p.n, na = p.na, nb = p.nb, ldc = p.ldc;
+    const int64_t ldp = p.ldp, ldq = p.ldq, na = p.na, nb = p.nb, ldc = p.ldc;
+    const int64_t chunks = (p.n + 15) >> 4, beg = chunks * range / p.ranges * 16, end = chunks * (range + 1) / p.ranges * 16, n = end < p.n ? end : p.n;
     constexpr bool BF = sizeof(T) == 2;
     typedef typename Four<T>::vec vec;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lj = lane >> 4;
@@ -339,7 +341,7 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile) {
         for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const vec zero = {0, 0, 0, 0};
     if constexpr (BF) {
-        for (int64_t k = 0; k < n; k += 16) {
+        for (int64_t k = beg; k < n; k += 16) {
             vec a[4], b[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -358,7 +360,7 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile) {
             }
         }
     } else {
-        for (int64_t k = 0; k < n; k += 16) {
+        for (int64_t k = beg; k < n; k += 16) {
             vec a[4], b[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -382,6 +384,15 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (at + i < from) continue;
+            if (p.ranges > 1) {
+                float* to = p.acc + ((int64_t)range * na + at + i) * nb + cb;
+                const f32x4 o = {acc[i][0][r], acc[i][1][r], acc[i][2][r], acc[i][3][r]};
+                if (whole) *(f32x4u*)to = o;
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) if (cb + j >= b0 + 4 * li) to[j] = o[j];
+                continue;
+            }
             T* to = C + (at + i) * ldc + cb;
             vec o;
 #pragma unroll
@@ -409,7 +420,7 @@ __global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const Thin
         const int per = tiles * ranges, block = b / per;
         b -= block * per;
         thin_product<T, VC, NF, EPI>(a, b % tiles, b / tiles, ranges, block);
-    } else thin_dw<T>(w, b - dx_blocks);
+    } else thin_dw<T>(w, (b - dx_blocks) % w.tiles, (b - dx_blocks) / w.tiles);
 }
 
 }  // namespace rowops
