@@ -232,23 +232,24 @@ using rowops::XentGemm;
 
 int64_t up(int64_t a, int64_t b) { return ceil_div64(a, b) * b; }
 
-// tile shapes of k_xent_gemm: 256 x 256 (8 waves), 128 x 128 (4), 64 x 128 (4)
-struct Tile { int bm, bn, wm; };
-constexpr Tile kTiles[3] = {{256, 256, 2}, {128, 128, 2}, {64, 128, 1}};
+// tile shapes of k_xent_gemm: 256 x 256 (float32: 256 x 128; 8 waves), 128 x 128 (4), 64 x 128 (4); wm: waves along m; step: microseconds of one step
+// when every CU has a workgroup (128 x 128 bfloat16: two)
+struct Tile { int bm, bn, wm, per_cu; double step; };
+constexpr Tile kTiles[2][3] = {{{256, 256, 2, 1, 0.9}, {128, 128, 2, 2, 0.6}, {64, 128, 1, 2, 0.4}}, {{256, 128, 4, 1, 1.5}, {128, 128, 2, 1, 1.0}, {64, 128, 1, 2, 0.9}}};
 int64_t tile_count(const Tile& t, int64_t M, int64_t N) { return ceil_div64(M, t.bm) * ceil_div64(N, t.bn); }
-// 256 tiles (one workgroup per CU) unless 128 tiles (two per CU, a quarter of the work each, 15 % more time for it) need fewer rounds
-int pick_tile(int64_t M, int64_t N, int ncu) {
+// the large tile unless 128 x 128 tiles need less time in whole rounds
+int pick_tile(bool f32, int64_t M, int64_t N, int ncu) {
     if (M <= 64) return 2;
-    const double t256 = (double)ceil_div64(tile_count(kTiles[0], M, N), ncu), t128 = 0.29 * (double)ceil_div64(tile_count(kTiles[1], M, N), ncu);
-    return t256 <= t128 ? 0 : 1;
+    const Tile* t = kTiles[f32];
+    auto cost = [&](const Tile& x) { return (double)ceil_div64(tile_count(x, M, N), (int64_t)ncu * x.per_cu) * x.step; };
+    return cost(t[0]) <= cost(t[1]) ? 0 : 1;
 }
 
 // what a call needs: operand forms, pieces of the classes, and where everything lies in the workspace
 struct XentPlan {
     const dimn_output_loss* d;
     bool grad, f32, labels, out_in;           // out_in: the kernel is stored [classes][width]
-    int planes, segments, ncu;
-    uint32_t a_of, b_of;
+    int planes, deep, ncu;                    // deep: k's of one step
     int64_t N, H, V, Hp, Np, P;               // Hp, Np: width / rows rounded up to 64; P: classes per piece
     bool x_direct, w_direct, wt_direct;
     int t_logits;
@@ -260,7 +261,7 @@ struct XentPlan {
     // The largest piece allowed, or a smaller one whose 256 x 256 tiles fill the device in whole rounds: a piece of 84 class tiles at 16 row tiles
     // takes 6 rounds of 256 workgroups where 96 class tiles take the same six (64000 classes: 16 rounds instead of 18, 8 instead of 9 for dW).
     int64_t best_piece(int64_t most) const {
-        const int64_t tm = ceil_div64(N, 256), th = ceil_div64(H, 256);
+        const int64_t tm = ceil_div64(N, 256) * (f32 ? 2 : 1), th = ceil_div64(H, 256) * (f32 ? 2 : 1);
         auto rounds = [&](int64_t tiles) { return ceil_div64(tiles, ncu); };
         auto cost = [&](int64_t tiles_v) { return (double)rounds(tiles_v * tm) * H + (grad ? (double)rounds(tiles_v * th) * N : 0.0); };
         const int64_t all = ceil_div64(V, 256), top = most / 256;
@@ -273,14 +274,14 @@ struct XentPlan {
         }
         return best * 256;
     }
-    // Ranges of the inner dimension of an M x N product: its rounds get shorter, its sums are written and read once more (microseconds: 0.9 / 0.6 per
-    // step of a 256 tile / two 128 tiles, 4 TB/s).
+    // Ranges of the inner dimension of an M x N product: its rounds get shorter, its sums are written and read once more (at 4 TB/s).
     int split_count(int tile, int64_t M, int64_t N_, int64_t steps) const {
-        const int64_t tiles = tile_count(kTiles[tile], M, N_), slots = tile == 0 ? ncu : 2 * ncu, most = std::max<int64_t>(1, std::min<int64_t>(32, steps / 8));
+        const Tile& x = kTiles[f32][tile];
+        const int64_t tiles = tile_count(x, M, N_), slots = (int64_t)ncu * x.per_cu, most = std::max<int64_t>(1, std::min<int64_t>(32, steps / 8));
         double least = 1e300;
         int best = 1;
         for (int64_t k = 1; k <= most; ++k) {
-            const double c = (double)ceil_div64(tiles * k, slots) * (double)steps / (double)k * (tile == 0 ? 0.9 : 0.6) + (k > 1 ? 4.0 + (double)(k * M * N_) * 8 / 4e6 : 0.0);
+            const double c = (double)ceil_div64(tiles * k, slots) * (double)steps / (double)k * x.step + (k > 1 ? 4.0 + (double)(k * M * N_) * 8 / 4e6 : 0.0);
             if (c < least) { least = c; best = (int)k; }
         }
         return best;
@@ -288,7 +289,7 @@ struct XentPlan {
     // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 256 .. 4096 and 300 .. 32000
     // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles)
     bool prefers_thin() const {
-        const double hv = (double)H * (double)V, work = hv * (double)N, steps = 0.5 * segments * (double)(Hp / 64);
+        const double hv = (double)H * (double)V, work = hv * (double)N, steps = (f32 ? 2.0 : 0.5) * (double)(Hp / 64);
         double t, g;
         if (!grad) {
             t = work * (f32 ? 25e-6 : 10.5e-6) * 1e-3;
@@ -309,9 +310,7 @@ struct XentPlan {
         labels = d->target_kind <= DIMN_TARGET_I64;
         out_in = d->kernel_in == 1;
         planes = f32 ? 3 : 1;
-        segments = f32 ? 6 : 1;
-        a_of = f32 ? 0x001102u : 0;           // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), small terms first
-        b_of = f32 ? 0x010120u : 0;
+        deep = f32 ? 32 : 64;
         Hp = up(H, 64); Np = up(N, 64);
         const int64_t far = 1 << 22;          // (operand rows are reached by 32-bit offsets inside a tile of 256)
         auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
@@ -324,9 +323,9 @@ struct XentPlan {
         P = std::min(std::min(P, far), up(V, 256));
         if (P < V && !w_direct) P = best_piece(P);
         else if (P < V && grad) P = best_piece(P);
-        t_logits = pick_tile(N, std::min(P, V), ncu);
-        tiles_m = ceil_div64(N, kTiles[t_logits].bm);
-        tiles_n = ceil_div64(V, kTiles[t_logits].bn);
+        t_logits = pick_tile(f32, N, std::min(P, V), ncu);
+        tiles_m = ceil_div64(N, kTiles[f32][t_logits].bm);
+        tiles_n = ceil_div64(V, kTiles[f32][t_logits].bn);
         bytes = 0;
         // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.
         thin = V >= 4 && H >= 4 && prefers_thin();
@@ -365,34 +364,39 @@ struct XentPlan {
         g = take(2 * planes * N * P);
         gt = take(2 * planes * P * Np);
         tsum = take(4 * N);
-        dbias = take(4 * tiles_m * kTiles[t_logits].wm * V);
+        dbias = take(4 * tiles_m * kTiles[f32][t_logits].wm * V);
         // dx has few tiles and a long inner dimension, so has dW of a narrow layer: ranges of it, each with float32 sums of its own
         const int64_t pv = std::min(P, V);
-        const int64_t steps = ceil_div64(pv, 64) * segments, most = std::min<int64_t>(32, steps / 8);
-        t_dx = N <= 64 ? 2 : (tile_count(kTiles[0], N, H) * std::min<int64_t>(most, 4) >= ncu * 3 / 4 ? 0 : 1);
+        auto tile_for = [&](int64_t M, int64_t N_, int64_t steps) {        // (the large tile if a few ranges of k fill the device with it)
+            const int64_t most = std::min<int64_t>(4, std::max<int64_t>(1, steps / 8));
+            return M > 64 && tile_count(kTiles[f32][0], M, N_) * most >= ncu * 3 / 4 ? 0 : pick_tile(f32, M, N_, ncu);
+        };
+        const int64_t steps = up(pv, 64) / deep, steps_w = Np / deep;
+        t_dx = tile_for(N, H, steps);
         splits = split_count(t_dx, N, H, steps);
-        t_dw = pick_tile(d->kernel_in == 1 ? pv : H, d->kernel_in == 1 ? H : pv, ncu);
-        dw_splits = split_count(t_dw, d->kernel_in == 1 ? pv : H, d->kernel_in == 1 ? H : pv, Np / 64 * segments);
+        const int64_t wm = d->kernel_in == 1 ? pv : H, wn = d->kernel_in == 1 ? H : pv;
+        t_dw = pick_tile(f32, wm, wn, ncu);
+        dw_splits = split_count(t_dw, wm, wn, steps_w);
         acc_w = dw_splits > 1 ? take(4 * (int64_t)dw_splits * H * pv) : 0;
         acc = take(4 * (int64_t)splits * N * H);
     }
 };
 
 template <int EPI>
-void xent_gemm(int tile, int splits, XentGemm& p, hipStream_t st) {
-    const Tile& t = kTiles[tile];
+void xent_gemm(bool f32, int tile, int splits, XentGemm& p, hipStream_t st) {
+    const Tile& t = kTiles[f32][tile];
     p.tiles_m = (int)ceil_div64(p.M, t.bm);
     p.tiles_n = (int)ceil_div64(p.N, t.bn);
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)splits);
-#define GEMM(PL)                                                                                                                  \
-    do {                                                                                                                          \
-        if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 256, 2, 4, EPI, PL>), grid, dim3(512), 0, st, p);             \
-        else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI, PL>), grid, dim3(256), 0, st, p);        \
-        else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI, PL>), grid, dim3(256), 0, st, p);                        \
-    } while (0)
-    if (p.segments > 1) GEMM(3);
-    else GEMM(1);
-#undef GEMM
+    if (f32) {
+        if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 128, 4, 2, EPI, 3>), grid, dim3(512), 0, st, p);
+        else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI, 3>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI, 3>), grid, dim3(256), 0, st, p);
+    } else {
+        if (tile == 0) hipLaunchKernelGGL((rowops::k_xent_gemm<256, 256, 2, 4, EPI, 1>), grid, dim3(512), 0, st, p);
+        else if (tile == 1) hipLaunchKernelGGL((rowops::k_xent_gemm<128, 128, 2, 2, EPI, 1>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((rowops::k_xent_gemm<64, 128, 1, 4, EPI, 1>), grid, dim3(256), 0, st, p);
+    }
 }
 
 // Operands to lay out, gathered and launched together
@@ -430,7 +434,7 @@ void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& 
         else lay.add(true, at(d, d->kernel, c0), d->kernel_in, pv, q.H, (uint16_t*)(ws + q.w), q.Hp, p.b_plane);
     }
     p.M = (int)q.N; p.N = (int)pv;
-    p.ksteps = (int)(q.Hp / 64); p.segments = q.segments; p.a_of = q.a_of; p.b_of = q.b_of;
+    p.ksteps = (int)(q.Hp / q.deep);
     p.bias = d->bias ? d->bias + c0 : nullptr;
     p.target = d->target; p.target_row = d->target_row; p.target_kind = d->target_kind;
     if (!q.labels) p.target = (const char*)d->target + c0 * (d->target_kind == DIMN_TARGET_F32 ? 4 : 2);
@@ -563,7 +567,7 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     q.make(d, false, compute_units(d->device_id));
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
-    const Tile& t = kTiles[q.t_logits];
+    const Tile& t = kTiles[q.f32][q.t_logits];
     if (q.thin) {
         rowops::Thin p = xent_thin_logits(q);
         p.part = (float2*)(ws + q.part);
@@ -579,7 +583,7 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
         p.part = (float2*)(ws + q.part) + c0 / t.bn * q.N;
         if (!q.labels) p.part_t = (float2*)(ws + q.part_t) + c0 / t.bn * q.N;
         p.picked = (float*)(ws + q.picked);
-        xent_gemm<rowops::XE_LSE>(q.t_logits, 1, p, st);
+        xent_gemm<rowops::XE_LSE>(q.f32, q.t_logits, 1, p, st);
     }
     rowops::XentRows r{};
     r.part = (const float2*)(ws + q.part);
@@ -637,23 +641,22 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
         p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
         p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = q.V;
-        xent_gemm<rowops::XE_GRAD>(q.t_logits, 1, p, st);
+        xent_gemm<rowops::XE_GRAD>(q.f32, q.t_logits, 1, p, st);
         // dx += G W^T
         XentGemm a{};
         a.A = p.G; a.lda = ldg; a.a_plane = p.g_plane;
         if (q.wt_direct) { a.B = (const uint16_t*)at(d, d->kernel, c0); a.ldb = d->kernel_in; }
         else { a.B = wt; a.ldb = ldg; a.b_plane = wt_plane; }
         a.M = (int)q.N; a.N = (int)q.H;
-        a.ksteps = (int)(ldg / 64); a.segments = q.segments; a.a_of = q.a_of; a.b_of = q.b_of;
+        a.ksteps = (int)(ldg / q.deep);
         a.acc = (float*)(ws + q.acc); a.acc_split = q.N * q.H; a.acc_first = c0 == 0;
-        xent_gemm<rowops::XE_ADD>(q.t_dx, q.splits, a, st);
+        xent_gemm<rowops::XE_ADD>(q.f32, q.t_dx, q.splits, a, st);
         // dW of the piece
         XentGemm w{};
-        w.ksteps = (int)(q.Np / 64); w.segments = q.segments; w.a_of = q.a_of; w.b_of = q.b_of;
+        w.ksteps = (int)(q.Np / q.deep);
         const uint16_t *gt = p.GT, *xa = xt;
         if (dk_out_in) {
             w.A = gt; w.lda = q.Np; w.a_plane = p.gt_plane; w.M = (int)pv;
-            std::swap(w.a_of, w.b_of);           // the operands change sides: the same products in the same order, the same bits
             w.B = xa; w.ldb = q.Np; w.b_plane = xt_plane; w.N = (int)q.H;
             w.C = const_cast<void*>(at(d, dkernel, c0 * dkernel_out)); w.ldc = dkernel_out;
         } else {
@@ -663,15 +666,15 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         }
         if (q.dw_splits > 1) {
             w.acc = (float*)(ws + q.acc_w); w.acc_split = (int64_t)w.M * w.N; w.acc_first = 1;
-            xent_gemm<rowops::XE_ADD>(q.t_dw, q.dw_splits, w, st);
+            xent_gemm<rowops::XE_ADD>(q.f32, q.t_dw, q.dw_splits, w, st);
             rowops::XentFinish f{};
             f.m[0] = split_sum(w.acc, q.dw_splits, w.M, w.N, w.C, w.ldc);
             xent_finish(q.f32, f, st);
-        } else xent_gemm<rowops::XE_STORE>(q.t_dw, 1, w, st);
+        } else xent_gemm<rowops::XE_STORE>(q.f32, q.t_dw, 1, w, st);
     }
     rowops::XentFinish f{};
     f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
-    finish_bias(f, q, ws, (int)(q.tiles_m * kTiles[q.t_logits].wm), dbias);
+    finish_bias(f, q, ws, (int)(q.tiles_m * kTiles[q.f32][q.t_logits].wm), dbias);
     xent_finish(q.f32, f, st);
     HIPCHK(hipGetLastError());
     return DIMN_OK;

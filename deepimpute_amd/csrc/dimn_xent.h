@@ -132,9 +132,7 @@ struct XentGemm {
     const uint16_t* A; const uint16_t* B;      // [plane][m][lda], [plane][n][ldb]; 16-byte aligned, lda / ldb multiples of 8
     int64_t lda, ldb, a_plane, b_plane;
     int32_t M, N;                              // columns from N on are not classes / not stored
-    int32_t ksteps;                            // 64-deep steps of one plane
-    int32_t segments;                          // plane pairs (1 or 6): pair i multiplies plane (a_of >> 4 i) & 15 of A with plane (b_of >> 4 i) & 15 of B
-    uint32_t a_of, b_of;
+    int32_t ksteps;                            // steps of the inner dimension: 64 deep (one plane) / 32 deep (three)
     int32_t tiles_m, tiles_n;
     // epilogues over logits: z = C + bias
     const float* bias;                         // [N] or NULL
@@ -186,23 +184,24 @@ __device__ __forceinline__ f32x4 xent_profile4(const void* target, int32_t kind,
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 
-// Tile BM x BN per workgroup, WM x WN waves; k in steps of 64, two stages of LDS filled by 16-byte DMA while the other one is multiplied, one
-// barrier per step.  The matrix instruction takes B's rows as its rows and A's as its columns, and fragment i / j of a wave holds rows
-// FM li + i of A, 4 FN (q >> 2) + 4 j + (q & 3) of B (q: the instruction's row): a lane then owns FM consecutive m's x 4 FN consecutive n's of C.
-// Sums along n are mostly inside a lane, results leave in 16-byte pieces in BOTH memory orders, and G needs no transposition.
-// A row of a tile is 128 bytes; its eight 16-byte pieces are stored at piece ^ bank_turn(row): the rows a fragment reads at once (FM or 4 FN
-// apart) then fall on different banks.  The DMA writes LDS in lane order, so the turn is made on the global side.
-__device__ __forceinline__ int bank_turn(int row) {
-    return ((row ^ (row >> 3)) & 1) | ((((row >> 1) ^ (row >> 2) ^ (row >> 5)) & 1) << 1) | (((row >> 4) & 1) << 2);
-}
+// Tile BM x BN per workgroup, WM x WN waves; k in steps of 64 (PL = 1: bfloat16) or 32 (PL = 3: all three planes of both operands, six products), two
+// stages of LDS filled by 16-byte DMA while the other one is multiplied, one barrier per step.  The matrix instruction takes B's rows as its rows and
+// A's as its columns, and fragment i / j of a wave holds rows FM q + i of A, 4 FN (q >> 2) + 4 j + (q & 3) of B (q: the instruction's index): a lane
+// then owns FM consecutive m's x 4 FN consecutive n's of C.  Sums along n are mostly inside a lane, results leave in 16-byte pieces in BOTH memory
+// orders, and G needs no transposition.
+// LDS holds the rows in fragment order (row 16 f + q of a wave's part), 128 / 64 bytes each, the 16-byte pieces of a row turned by its number: the
+// rows a fragment reads at once are neighbours on different banks, and every address is one register plus a constant.  The DMA writes LDS in lane
+// order, so order and turn are made on the global side.
 template <int BM, int BN, int WM, int WN, int EPI, int PL>
 __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
-    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-    constexpr int LOADS = (BM + BN) / 8 / NW;
-    static_assert(LOADS * 8 * NW == BM + BN, "whole requests per wave");
-    __shared__ __attribute__((aligned(1024))) uint16_t lds[2][(BM + BN) * 64];
+    constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16, ROWS = BM + BN;
+    constexpr int DEEP = PL == 1 ? 64 : 32, PIECES = DEEP / 8, LINE = 64 / PIECES;      // k's per step; pieces per row; rows per request
+    constexpr int LOADS = PL * ROWS / LINE / NW;
+    static_assert(LOADS * LINE * NW == PL * ROWS && BM % LINE == 0, "whole requests per wave");
+    __shared__ __attribute__((aligned(1024))) uint16_t lds[2][PL * ROWS * DEEP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, li = lane & 15, lj = lane >> 4;
+    auto turn = [](int row) { return PL == 1 ? row & 7 : (row >> 2) & 3; };
     // Workgroup b runs on XCD b % 8: each XCD gets a consecutive range of the tiles, ordered in columns of eight m tiles, so that the 32
     // workgroups of an XCD at a time share eight A and four B tiles in its L2.
     int tile;
@@ -218,75 +217,107 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
         tm = grp * 8 + in - tn * h;
     }
     const int m0 = tm * BM, n0 = tn * BN;
-    // requests: request c of this wave brings rows 8 (wave LOADS + c) .. + 7 of the stacked [A; B] tile
+    // request c of this wave brings lines [LINE (wave LOADS + c), + LINE) of the stacked planes of [A; B]
     uint32_t off[LOADS];
+    auto line_of = [&](int c) { return (wave * LOADS + c) * LINE; };
 #pragma unroll
     for (int c = 0; c < LOADS; ++c) {
-        const int row = (wave * LOADS + c) * 8 + (lane >> 3);
-        const bool isA = (wave * LOADS + c) * 8 < BM;
-        int r = isA ? row : row - BM;
-        const int piece = (lane & 7) ^ bank_turn(r);
+        const int pos = line_of(c) % ROWS + lane / PIECES;
+        const bool isA = line_of(c) % ROWS < BM;
+        const int t = isA ? pos : pos - BM, q = t & 15, f = t >> 4;
+        int r = isA ? f / FM * TM + q * FM + f % FM : f / FN * TN + (q >> 2) * 4 * FN + 4 * (f % FN) + (q & 3);
+        const int piece = (lane % PIECES) ^ turn(t);
         const int lim = isA ? p.M - 1 - m0 : p.N - 1 - n0;       // rows past the end read the last one: their results are never used
         r = r < lim ? r : lim;
         off[c] = (uint32_t)((int64_t)r * (isA ? p.lda : p.ldb) * 2 + piece * 16);
     }
     const char* Abase = (const char*)(p.A + (int64_t)m0 * p.lda);
     const char* Bbase = (const char*)(p.B + (int64_t)n0 * p.ldb);
-    const int total = p.ksteps * p.segments;
     const int S = gridDim.y, sp = blockIdx.y;
-    const int tbeg = (int)((int64_t)total * sp / S), tend = (int)((int64_t)total * (sp + 1) / S);
-    int seg = tbeg / p.ksteps, ks = tbeg - seg * p.ksteps;       // of the next request
-    auto request = [&](int stage) {
-        const char* a = Abase + (int64_t)((p.a_of >> (4 * seg)) & 15) * p.a_plane * 2 + (int64_t)ks * 128;
-        const char* b = Bbase + (int64_t)((p.b_of >> (4 * seg)) & 15) * p.b_plane * 2 + (int64_t)ks * 128;
+    const int tbeg = (int)((int64_t)p.ksteps * sp / S), tend = (int)((int64_t)p.ksteps * (sp + 1) / S);
+    auto request = [&](int stage, int t) {
+        const char* a = Abase + (int64_t)t * (DEEP * 2);
+        const char* b = Bbase + (int64_t)t * (DEEP * 2);
 #pragma unroll
         for (int c = 0; c < LOADS; ++c) {
-            const bool isA = (wave * LOADS + c) * 8 < BM;
-            __builtin_amdgcn_global_load_lds((global_void*)((isA ? a : b) + off[c]), (lds_void*)&lds[stage][(wave * LOADS + c) * 512], 16, 0, 0);
+            const int plane = line_of(c) / ROWS;
+            const bool isA = line_of(c) % ROWS < BM;
+            const char* from = isA ? a + plane * p.a_plane * 2 : b + plane * p.b_plane * 2;
+            __builtin_amdgcn_global_load_lds((global_void*)(from + off[c]), (lds_void*)&lds[stage][line_of(c) * DEEP], 16, 0, 0);
         }
-        if (++ks == p.ksteps) { ks = 0; ++seg; }
     };
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    // fragment f of a part that starts at LDS row `row0` of `plane`, k's 32 kk ..
+    auto fragment = [&](int stage, int plane, int row0, int f, int kk) {
+        return *(const bf8*)&lds[stage][(plane * ROWS + row0 + 16 * f + li) * DEEP + (((kk * 4 + lj) ^ turn(li)) << 3)];
+    };
     auto multiply = [&](int stage) {
+        if constexpr (PL == 1) {
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf8 a[FM], b[FN];
+            for (int kk = 0; kk < 2; ++kk) {
+                bf8 a[FM], b[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int row = wn * TN + (li >> 2) * 4 * FN + 4 * j + (li & 3);
-                b[j] = *(const bf8*)&lds[stage][(BM + row) * 64 + (((kk * 4 + lj) ^ bank_turn(row)) << 3)];
+                for (int j = 0; j < FN; ++j) b[j] = fragment(stage, 0, BM + wn * TN, j, kk);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) a[i] = fragment(stage, 0, wm * TM, i, kk);
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
             }
+        } else {
+            bf8 a[PL][FM], b[PL][FN];
+            auto add = [&](const bf8 (&u)[FM], const bf8 (&v)[FN]) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                const int row = wm * TM + li * FM + i;
-                a[i] = *(const bf8*)&lds[stage][row * 64 + (((kk * 4 + lj) ^ bank_turn(row)) << 3)];
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[j], u[i], acc[i][j], 0, 0, 0);
+            };
+#pragma unroll
+            for (int s = 0; s < PL; ++s) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) b[s][j] = fragment(stage, s, BM + wn * TN, j, 0);
+#pragma unroll
+                for (int i = 0; i < FM; ++i) a[s][i] = fragment(stage, s, wm * TM, i, 0);
+                // (0,0); (0,1) (1,0) (1,1); (0,2) (2,0)
+                add(a[0], b[s]);
+                if (s > 0) add(a[s], b[0]);
+                if (s == 1) add(a[1], b[1]);
             }
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
         }
     };
-    if (tbeg < tend) request(0);
+    if (tbeg < tend) request(0, tbeg);
     int stage = 0;
     for (int t = tbeg; t + 1 < tend; ++t) {
         __syncthreads();                                         // the stage's bytes have landed (the barrier waits for this wave's requests first) and
-        request(stage ^ 1);                                      // everybody is done with the other stage
+        request(stage ^ 1, t + 1);                               // everybody is done with the other stage
         multiply(stage);
         stage ^= 1;
-        // Fragments are read one group of 2 FN products ahead of their use: left alone, the compiler reads two, waits, and multiplies (4-6 % slower)
-        constexpr int GROUP = (2 * FM + FN - 2) / (FM - 2);
-        __builtin_amdgcn_sched_group_barrier(0x100, FN + 2, 0);
+        // Fragments are read one group of products ahead of their use: left alone, the compiler reads two, waits, and multiplies (4-6 % slower)
+        if constexpr (PL == 1) {
+            constexpr int GROUP = (2 * FM + FN - 2) / (FM - 2);
+            __builtin_amdgcn_sched_group_barrier(0x100, FN + 2, 0);
 #pragma unroll
-        for (int q = 0; q < FM - 2; ++q) {
-            __builtin_amdgcn_sched_group_barrier(0x100, GROUP, 0);
-            __builtin_amdgcn_sched_group_barrier(0x8, 2 * FN, 0);
+            for (int q = 0; q < FM - 2; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, GROUP, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, 2 * FN, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, 4 * FN, 0);
+        } else {
+            __builtin_amdgcn_sched_group_barrier(0x100, FM + FN, 0);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, FN, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, FM * FN, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, FM, 0);
+                __builtin_amdgcn_sched_group_barrier(0x8, FM * FN, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x8, 2 * FM * FN, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x8, 4 * FN, 0);
     }
     if (tbeg < tend) {
         __syncthreads();
