@@ -344,7 +344,7 @@ struct XentPlan {
             tsum = take(4 * N);
             dbias = take(4 * blocks * V);
             const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
-            splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, 2 * ncu / wgs, chunks / 2}));
+            splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, ceil_div64(4 * ncu, wgs), chunks / 2}));
             acc = take(4 * (int64_t)splits * N * H);
             const int64_t wt_wgs = ceil_div64(H, 64) * ceil_div64(V, 256);        // (dW: 64 x 256 of the product per workgroup, either way round)
             dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)32, 2 * ncu / wt_wgs, N / 128}));
@@ -441,17 +441,22 @@ void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& 
     p.class0 = c0; p.classes = q.V;
 }
 
+// workgroups of `units` x the row blocks (thin_place)
+int64_t thin_groups(const XentPlan& q, int64_t units) { return (units < 64 ? units : up(units, 8)) * q.blocks; }
+// the logits' product: epilogue XE_LSE or XE_GRAD
 template <typename T, int EPI>
-void xent_thin(const XentPlan& q, bool vc, int64_t n, int splits, const rowops::Thin& p, hipStream_t st) {
-    const dim3 grid((unsigned)ceil_div64(n, vc ? 64 : 32), (unsigned)splits, (unsigned)q.blocks);
-#define THIN(NF)                                                                                                  \
-    do {                                                                                                          \
-        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin<T, true, NF, EPI>), grid, dim3(256), 0, st, p);           \
-        else hipLaunchKernelGGL((rowops::k_xent_thin<T, false, NF, EPI>), grid, dim3(256), 0, st, p);             \
+void xent_thin(const XentPlan& q, const rowops::Thin& p, hipStream_t st) {
+    const dim3 grid((unsigned)thin_groups(q, q.tiles_n));
+    const int tiles = (int)q.tiles_n, blocks = (int)q.blocks;
+    // sixteen waves per workgroup while that leaves CUs to spare and every wave still has chunks of k
+    const bool deep = q.nf <= 2 && q.tiles_n * q.blocks <= q.ncu && q.H >= 512;
+#define THIN(VC, NF)                                                                                                                              \
+    do {                                                                                                                                          \
+        if (NF <= 2 && deep) hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF <= 2 ? NF : 1, EPI, 16>), grid, dim3(1024), 0, st, p, tiles, 1, blocks);  \
+        else hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF, EPI, 4>), grid, dim3(256), 0, st, p, tiles, 1, blocks);                              \
     } while (0)
-    if (q.nf == 1) THIN(1);
-    else if (q.nf == 2) THIN(2);
-    else THIN(4);
+    if (q.out_in) { if (q.nf == 1) THIN(false, 1); else if (q.nf == 2) THIN(false, 2); else THIN(false, 4); }
+    else { if (q.nf == 1) THIN(true, 1); else if (q.nf == 2) THIN(true, 2); else THIN(true, 4); }
 #undef THIN
 }
 rowops::Thin xent_thin_logits(const XentPlan& q) {
@@ -490,7 +495,7 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     p.lse = lse; p.dloss = dloss; p.tsum = tsum;
     p.G = G; p.ldg = q.V;
     p.dbias_part = dbias ? (q.blocks == 1 ? dbias : (float*)(ws + q.dbias)) : nullptr;
-    xent_thin<T, rowops::XE_GRAD>(q, !q.out_in, q.V, 1, p, st);
+    xent_thin<T, rowops::XE_GRAD>(q, p, st);
     // dx[n][h] = sum over the classes: the classes are the inner dimension now
     rowops::Thin a{};
     a.A = G; a.lda = q.V; a.B = d->kernel; a.ldb = p.ldb;
@@ -506,16 +511,32 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     w.ranges = q.dw_splits;
     w.acc = (float*)(ws + q.acc_w);
     const bool vc = q.out_in;
-    const int tiles = (int)ceil_div64(q.H, vc ? 64 : 32), dx_blocks = tiles * q.splits * (int)q.blocks;
-    const dim3 grid((unsigned)(dx_blocks + w.tiles * w.ranges));
+    const int tiles = (int)ceil_div64(q.H, vc ? 64 : 32), dx_groups = (int)thin_groups(q, (int64_t)tiles * q.splits);
+    const dim3 grid((unsigned)(dx_groups + w.tiles * w.ranges));
+    const int ranges = q.splits, blocks = (int)q.blocks;
+    if (grid.x <= 8 * (unsigned)q.ncu) {
 #define BOTH(NF, EPI)                                                                                                                                      \
     do {                                                                                                                                                   \
-        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin_both<T, true, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_blocks, tiles, q.splits);                \
-        else hipLaunchKernelGGL((rowops::k_xent_thin_both<T, false, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_blocks, tiles, q.splits);                  \
+        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin_both<T, true, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_groups, tiles, ranges, blocks);          \
+        else hipLaunchKernelGGL((rowops::k_xent_thin_both<T, false, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_groups, tiles, ranges, blocks);            \
     } while (0)
-    if (q.splits == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(4, rowops::XE_STORE); }
-    else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
+        if (ranges == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(4, rowops::XE_STORE); }
+        else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
 #undef BOTH
+    } else {
+        const dim3 gx((unsigned)dx_groups);
+#define DX(NF, EPI)                                                                                                                                        \
+    do {                                                                                                                                                   \
+        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin<T, true, NF, EPI, 4>), gx, dim3(256), 0, st, a, tiles, ranges, blocks);                            \
+        else hipLaunchKernelGGL((rowops::k_xent_thin<T, false, NF, EPI, 4>), gx, dim3(256), 0, st, a, tiles, ranges, blocks);                              \
+    } while (0)
+        if (ranges == 1) { if (q.nf == 1) DX(1, rowops::XE_STORE); else if (q.nf == 2) DX(2, rowops::XE_STORE); else DX(4, rowops::XE_STORE); }
+        else { if (q.nf == 1) DX(1, rowops::XE_ADD); else if (q.nf == 2) DX(2, rowops::XE_ADD); else DX(4, rowops::XE_ADD); }
+#undef DX
+        const dim3 gw((unsigned)(w.tiles * w.ranges));
+        if (q.N > 64) hipLaunchKernelGGL((rowops::k_xent_thin_dw<T, 2>), gw, dim3(256), 0, st, w);
+        else hipLaunchKernelGGL((rowops::k_xent_thin_dw<T, 1>), gw, dim3(256), 0, st, w);
+    }
     rowops::XentFinish f{};
     if (q.splits > 1) f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
     if (w.ranges > 1) f.m[1] = split_sum(w.acc, w.ranges, w.na, w.nb, w.C, w.ldc);
@@ -573,8 +594,8 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
         p.part = (float2*)(ws + q.part);
         p.part_t = q.labels ? nullptr : (float2*)(ws + q.part_t);
         p.picked = (float*)(ws + q.picked);
-        if (q.f32) xent_thin<float, rowops::XE_LSE>(q, !q.out_in, q.V, 1, p, st);
-        else xent_thin<bf16_t, rowops::XE_LSE>(q, !q.out_in, q.V, 1, p, st);
+        if (q.f32) xent_thin<float, rowops::XE_LSE>(q, p, st);
+        else xent_thin<bf16_t, rowops::XE_LSE>(q, p, st);
     } else for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
         XentGemm p;
         Lay lay;

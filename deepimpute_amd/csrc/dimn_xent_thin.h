@@ -8,8 +8,8 @@
 //   * class-contiguous (VC): a lane loads four consecutive classes of one k; element j belongs to class set j, whose sixteen classes lie four
 //     apart -- a permutation of the classes inside the workgroup's 64 that the epilogue undoes.
 // float32 runs on the exact float32 matrix instructions: at 64 rows their rate (154 TFLOP/s measured) and the HBM's meet.
-// A workgroup owns 32 (KC) / 64 (VC) classes x up to 64 rows; its four waves take every fourth chunk of k and are added through LDS in the
-// fixed order (w0 + w2) + (w1 + w3), so also a small problem keeps four waves per 32 classes busy.
+// A workgroup owns 32 (KC) / 64 (VC) classes x up to 64 rows; its waves (four, or sixteen where there are few workgroups and a long inner
+// dimension: 3840 x 222 float32 ran 45 us with four) share the chunks of k and are added through LDS, upper half onto lower half, in a fixed order.
 #pragma once
 #include "dimn_xent.h"
 
@@ -37,12 +37,14 @@ template <> struct Four<float> { typedef f32x4u vec; };
 template <> struct Four<bf16_t> { typedef u16x4u vec; };
 
 // (class tile, k-range, row block) of one workgroup; `ranges` k-ranges in all
-template <typename T, bool VC, int NF, int EPI>
+template <typename T, bool VC, int NF, int EPI, int NW>
 __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range, int ranges, int block) {
     constexpr bool BF = sizeof(T) == 2, WIDE = BF && !VC;      // WIDE: the 16x16x32 instruction, eight k's per lane
     constexpr int EL = WIDE ? 8 : 4, KS = 4 * EL, NS = VC ? 4 : 2, CW = VC ? 64 : 32, ROWS = 16 * NF, LD = CW + 4;
-    constexpr int U = NF > 2 ? 2 : 4;                           // chunks requested together
-    __shared__ __attribute__((aligned(16))) float red[2][ROWS][LD];
+    // Chunks requested together.  KC: two sets of them in registers, one in flight while the other is multiplied (3 x 1901 x 81826 float32: 145 ->
+    // 122 us, 5.1 TB/s).  VC needs twice the registers for that, and the workgroups a CU loses by it cost more (846 x 64 x 18203: 62 -> 91 us).
+    constexpr int SETS = VC ? 1 : 2, U = VC ? (NF > 2 || NW > 4 ? 2 : 4) : (NF > 1 || NW > 4 ? 2 : 4);
+    __shared__ __attribute__((aligned(16))) float red[NW / 2][ROWS][LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lj = lane >> 4;
     const int64_t c0 = (int64_t)tile * CW, m0 = (int64_t)block * ROWS;
     const T* A = (const T*)p.A;
@@ -68,8 +70,8 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
     typedef typename std::conditional<BF, typename std::conditional<WIDE, u16x8u, u16x4u>::type, f32x4u>::type avec;
     typedef typename std::conditional<VC, typename Four<T>::vec, avec>::type bvec;
     constexpr int NB = VC ? 4 : 2;
-    avec a[U][NF];
-    bvec b[U][NB];
+    avec a[SETS][U][NF];
+    bvec b[SETS][U][NB];
     f32x4 acc[NF][NS];
 #pragma unroll
     for (int f = 0; f < NF; ++f)
@@ -111,29 +113,48 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
     const int64_t whole = p.K / KS;
     const int64_t cbeg = whole * range / ranges, cend = whole * (range + 1) / ranges;
     // whole rounds of U consecutive chunks per wave (256 bytes of a class row at a time), then single chunks
-    const int64_t rounds = (cend - cbeg) / (4 * U);
-    for (int64_t i = 0; i < rounds; ++i) {
-        const int64_t c = cbeg + (4 * i + wave) * U;
+    const int64_t rounds = (cend - cbeg) / (NW * U);
+    auto fetch = [&](int64_t i, int set) {
+        const int64_t c = cbeg + (NW * (i < rounds ? i : rounds - 1) + wave) * U;
 #pragma unroll
-        for (int u = 0; u < U; ++u) request((c + u) * KS, a[u], b[u]);
+        for (int u = 0; u < U; ++u) request((c + u) * KS, a[set][u], b[set][u]);
+    };
+    auto consume = [&](int set) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) multiply(a[u], b[u]);
+        for (int u = 0; u < U; ++u) multiply(a[set][u], b[set][u]);
+    };
+    if constexpr (SETS == 1) {
+        for (int64_t i = 0; i < rounds; ++i) { fetch(i, 0); consume(0); }
+    } else if (rounds > 0) {
+        // (the barriers keep the compiler from moving every load down to its use)
+        fetch(0, 0);
+        for (int64_t i = 0; i + 1 < rounds; i += 2) {
+            fetch(i + 1, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(i + 2, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (rounds & 1) consume(0);
     }
-    for (int64_t c = cbeg + rounds * 4 * U + wave; c < cend; c += 4) { request(c * KS, a[0], b[0]); multiply(a[0], b[0]); }
-    if (whole * KS < p.K && range == ranges - 1 && wave == (whole & 3)) {
+    for (int64_t c = cbeg + rounds * NW * U + wave; c < cend; c += NW) { request(c * KS, a[0][0], b[0][0]); multiply(a[0][0], b[0][0]); }
+    if (whole * KS < p.K && range == ranges - 1 && wave == (int)(whole % NW)) {
         const int64_t k = whole * KS;
 #pragma unroll
         for (int q = 0; q < NB; ++q)
 #pragma unroll
             for (int i = 0; i < (VC ? 4 : EL); ++i) {
-                if constexpr (VC) b[0][q][i] = k + 4 * lj + q < p.K ? bptr[0][(k + 4 * lj + q) * p.ldb + i] : (T)0;
-                else b[0][q][i] = k + EL * lj + i < p.K ? bptr[q][k + EL * lj + i] : (T)0;
+                if constexpr (VC) b[0][0][q][i] = k + 4 * lj + q < p.K ? bptr[0][(k + 4 * lj + q) * p.ldb + i] : (T)0;
+                else b[0][0][q][i] = k + EL * lj + i < p.K ? bptr[q][k + EL * lj + i] : (T)0;
             }
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int i = 0; i < EL; ++i) a[0][f][i] = k + EL * lj + i < p.K ? arow[f][k + EL * lj + i] : (T)0;
-        multiply(a[0], b[0]);
+            for (int i = 0; i < EL; ++i) a[0][0][f][i] = k + EL * lj + i < p.K ? arow[f][k + EL * lj + i] : (T)0;
+        multiply(a[0][0], b[0][0]);
     }
     // element r of acc[f][s]: row 16 f + li, position 16 s + 4 lj + r (KC) / 4 (4 lj + r) + s (VC) of the workgroup's classes
     auto put = [&](int slot) {
@@ -145,25 +166,28 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
                 else *(f32x4*)&red[slot][16 * f + li][16 * q + 4 * lj] = acc[f][q];
             }
     };
-    if (wave >= 2) put(wave - 2);
-    __syncthreads();
-    if (wave < 2) {
 #pragma unroll
-        for (int f = 0; f < NF; ++f)
+    for (int half = NW / 2; half >= 2; half >>= 1) {
+        if (wave >= half && wave < 2 * half) put(wave - half);
+        __syncthreads();
+        if (wave < half) {
 #pragma unroll
-            for (int q = 0; q < NS; ++q) {
-                if constexpr (VC) {
-                    const f32x4 t = *(const f32x4*)&red[wave][16 * f + li][16 * lj + 4 * q];
+            for (int f = 0; f < NF; ++f)
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) acc[f][s][q] += t[s];
-                } else acc[f][q] += *(const f32x4*)&red[wave][16 * f + li][16 * q + 4 * lj];
-            }
+                for (int q = 0; q < NS; ++q) {
+                    if constexpr (VC) {
+                        const f32x4 t = *(const f32x4*)&red[wave][16 * f + li][16 * lj + 4 * q];
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) acc[f][s][q] += t[s];
+                    } else acc[f][q] += *(const f32x4*)&red[wave][16 * f + li][16 * q + 4 * lj];
+                }
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if (wave < 2) put(wave);
     __syncthreads();
     // PT threads per row, CPT consecutive positions each, in groups of four whose classes are consecutive
-    constexpr int CPT = CW * ROWS / 256 < 4 ? 4 : CW * ROWS / 256, PT = CW / CPT, NG = CPT / 4;
+    constexpr int CPT = CW * ROWS / (64 * NW) < 4 ? 4 : CW * ROWS / (64 * NW), PT = CW / CPT, NG = CPT / 4;
     const int row = tid / PT, pos0 = (tid % PT) * CPT;
     const int64_t m = m0 + row;
     const bool have = row < ROWS && m < p.M;
@@ -295,10 +319,11 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
             constexpr int ST = 256 / CW;                        // strands of rows per class
             const int pos = tid % CW, strand = tid / CW;
             float s = 0.f;
+            if (tid < 256)
 #pragma unroll 8
-            for (int r = strand; r < ROWS; r += ST) s += red[0][r][pos];
+                for (int r = strand; r < ROWS; r += ST) s += red[0][r][pos];
             __syncthreads();
-            red[1][strand][pos] = s;
+            if (tid < 256) red[1][strand][pos] = s;
             __syncthreads();
             if (strand == 0) {
                 int before, upto;
@@ -321,7 +346,9 @@ struct ThinDw {
     int32_t tiles_b, tiles;                    // workgroups along b (256 columns each), in all
     int32_t ranges; float* acc;                // ranges > 1: range r of the rows leaves its float32 sums in acc[r][na][nb]
 };
-template <typename T>
+// SETS = 2: sixteen rows in flight while sixteen are multiplied; for more than 64 rows (106 x 2922 x 25672 float32: 280 -> 233 us; with 12 rows the
+// registers it takes cost 56 -> 95 us)
+template <typename T, int SETS>
 __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const T *P = (const T*)p.P, *Q = (const T*)p.Q;
     T* C = (T*)p.C;
@@ -340,40 +367,48 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const vec zero = {0, 0, 0, 0};
-    if constexpr (BF) {
-        for (int64_t k = beg; k < n; k += 16) {
-            vec a[4], b[4];
+    vec a[SETS][4], b[SETS][4];
+    auto fetch = [&](int64_t k, int set) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = k + 4 * lj + r;
-                a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
-                b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int64_t row = BF ? k + 4 * lj + r : k + 4 * r + lj;       // bfloat16: four consecutive rows make one lane's operand
+            a[set][r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
+            b[set][r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
+        }
+    };
+    auto consume = [&](int set) {
+        if constexpr (BF) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const s16x4 u = {(short)a[0][i], (short)a[1][i], (short)a[2][i], (short)a[3][i]};
+                const s16x4 u = {(short)a[set][0][i], (short)a[set][1][i], (short)a[set][2][i], (short)a[set][3][i]};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const s16x4 v = {(short)b[0][j], (short)b[1][j], (short)b[2][j], (short)b[3][j]};
+                    const s16x4 v = {(short)b[set][0][j], (short)b[set][1][j], (short)b[set][2][j], (short)b[set][3][j]};
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(u, v, acc[i][j], 0, 0, 0);
                 }
             }
-        }
-    } else {
-        for (int64_t k = beg; k < n; k += 16) {
-            vec a[4], b[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int64_t row = k + 4 * r + lj;
-                a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
-                b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
-            }
+        } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][i], b[r][j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[set][r][i], b[set][r][j], acc[i][j], 0, 0, 0);
+        }
+    };
+    if constexpr (SETS == 1) {
+        for (int64_t k = beg; k < n; k += 16) { fetch(k, 0); consume(0); }
+    } else {
+        fetch(beg, 0);
+        for (int64_t k = beg; k < n; k += 32) {
+            fetch(k + 16, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(k + 32, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            consume(1);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     // acc[i][j][r]: a = set i of lane 4 lj + r, b = set j of lane li
@@ -405,22 +440,39 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     }
 }
 
-// grid (class tiles, k-ranges, row blocks)
-template <typename T, bool VC, int NF, int EPI>
-__global__ __launch_bounds__(256) void k_xent_thin(const Thin p) {
-    thin_product<T, VC, NF, EPI>(p, blockIdx.x, blockIdx.y, gridDim.y, blockIdx.z);
+// Workgroup b runs on XCD b % 8.  The row blocks of one class tile read the same part of the kernel: they are neighbours on one XCD, whose L2 then
+// holds it for all of them.  (unit, block) of workgroup b, units padded to a multiple of eight.  With few units that would leave XCDs idle
+// (three class tiles x 39 row blocks ran 43 us, 30 in plain order), and a small kernel sits in every L2 anyway.
+__device__ __forceinline__ void thin_place(int b, int units, int blocks, int& unit, int& block) {
+    if (units < 64) { unit = b % units; block = b / units; return; }
+    const int rest = b >> 3;
+    block = rest % blocks;
+    unit = rest / blocks * 8 + (b & 7);
+}
+template <typename T, bool VC, int NF, int EPI, int NW>
+__global__ __launch_bounds__(64 * NW) void k_xent_thin(const Thin p, int tiles, int ranges, int blocks) {
+    int unit, block;
+    thin_place(blockIdx.x, tiles * ranges, blocks, unit, block);
+    if (unit >= tiles * ranges) return;
+    thin_product<T, VC, NF, EPI, NW>(p, unit % tiles, unit / tiles, ranges, block);
+}
+template <typename T, int SETS>
+__global__ __launch_bounds__(256) void k_xent_thin_dw(const ThinDw w) {
+    thin_dw<T, SETS>(w, blockIdx.x % w.tiles, blockIdx.x / w.tiles);
 }
 
-// dx and dW in one launch: both read G and neither waits for the other, and with few rows each is mostly latency.  The first `dx_blocks` workgroups
-// multiply for dx (tiles x ranges x row blocks, flattened), the others for dW.
+// dx and dW in one launch, while both are small: both read G and neither waits for the other, and each is mostly latency (64 x 256 x 20000 float32:
+// 30 us apart, 25 together).  Larger ones run apart, with the registers each of them needs (12 x 3648 x 22455: 156 us apart, 180 together).  The first `dx_groups` workgroups
+// multiply for dx (tiles x ranges x row blocks), the others for dW.
 template <typename T, bool VC, int NF, int EPI>
-__global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const ThinDw w, int dx_blocks, int tiles, int ranges) {
-    int b = blockIdx.x;
-    if (b < dx_blocks) {
-        const int per = tiles * ranges, block = b / per;
-        b -= block * per;
-        thin_product<T, VC, NF, EPI>(a, b % tiles, b / tiles, ranges, block);
-    } else thin_dw<T>(w, (b - dx_blocks) % w.tiles, (b - dx_blocks) / w.tiles);
+__global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const ThinDw w, int dx_groups, int tiles, int ranges, int blocks) {
+    const int b = blockIdx.x;
+    if (b < dx_groups) {
+        int unit, block;
+        thin_place(b, tiles * ranges, blocks, unit, block);
+        if (unit >= tiles * ranges) return;
+        thin_product<T, VC, NF, EPI, 4>(a, unit % tiles, unit / tiles, ranges, block);
+    } else thin_dw<T, 1>(w, (b - dx_groups) % w.tiles, (b - dx_groups) / w.tiles);
 }
 
 }  // namespace rowops
