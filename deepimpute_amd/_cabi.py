@@ -39,8 +39,11 @@ class Config(C.Structure):
 
 
 class Layer(C.Structure):
-    """struct dimn_layer (include/dimn.h): one hidden Dense layer + the rate of the Dropout layer behind it."""
-    _fields_ = [("neurons", C.c_int32), ("activation", C.c_int32), ("dropout_rate", C.c_float)]
+    """struct dimn_layer (include/dimn.h): one hidden Dense layer (or a normalisation) + the rate of the Dropout layer behind it."""
+    _fields_ = [("neurons", C.c_int32), ("activation", C.c_int32), ("dropout_rate", C.c_float), ("epsilon", C.c_float)]
+
+
+LAYER_NORM = 64          # Layer.activation of a normalisation layer (DIMN_LAYER_NORM)
 
 
 class OutputLoss(C.Structure):
@@ -53,7 +56,8 @@ class OutputLoss(C.Structure):
 PRECISIONS = {"fp32": 0, "f32": 0, "float32": 0, "bf16": 1, "bfloat16": 1}
 LOSSES = {"wmse": 0, "wmse_binary": 1, "mean_squared_error": 2, "mse": 2, "mean_absolute_error": 3, "mae": 3,
           # round 5: the other element-wise keras.losses names (and their Keras aliases)
-          "mean_squared_logarithmic_error": 4, "msle": 4, "logcosh": 5, "log_cosh": 5, "huber": 6, "huber_loss": 6, "poisson": 7}
+          "mean_squared_logarithmic_error": 4, "msle": 4, "logcosh": 5, "log_cosh": 5, "huber": 6, "huber_loss": 6, "poisson": 7,
+          "categorical_crossentropy": 8}
 
 _H = C.c_void_p
 _P = C.c_void_p

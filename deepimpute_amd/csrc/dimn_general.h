@@ -582,6 +582,72 @@ __global__ __launch_bounds__(256) void k_gen_rowgemm(const GDesc* __restrict__ d
     }
 }
 
+// ---- normalisation layers (k_norm / k_norm_grad of dimn_norm.h on [sub-net][batch row][unit], parameters per sub-net) ----
+// The gate of a normalisation's output: the Dropout layer behind it (keep ? scale : 0, the same stream as behind a Dense layer).  grid (ceil(rows * width / 256), K)
+__global__ __launch_bounds__(256) void k_gen_dropout_gate(const SubnetDev* __restrict__ sn, float* __restrict__ G, int64_t g_stride, int rows, int width, float rate, float scale,
+                                                          uint64_t seed, uint32_t epoch, uint32_t step) {
+    const int e = blockIdx.x * 256 + threadIdx.x;
+    if (e >= rows * width) return;
+    G[(int64_t)blockIdx.y * g_stride + e] = dimn_dropout_keep(seed, (uint32_t)sn[blockIdx.y].kg, epoch, step, (uint32_t)e, rate) ? scale : 0.f;
+}
+__global__ __launch_bounds__(256) void k_gen_fill(float* __restrict__ p, int64_t n, float v) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e < n) p[e] = v;
+}
+// Keras-Adam on the n parameters from `off` of the flat arrays
+__global__ __launch_bounds__(256) void k_gen_norm_adam(float* __restrict__ P, float* __restrict__ Mo, float* __restrict__ Vo, int64_t off, int64_t n, const float* __restrict__ grad, AdamP ap) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= n) return;
+    float w = P[off + e], m = Mo[off + e], v = Vo[off + e];
+    adam1(w, m, v, grad[e], ap);
+    P[off + e] = w; Mo[off + e] = m; Vo[off + e] = v;
+}
+
+// Output layer under categorical_crossentropy: per cell, with f = softplus(z), p = f / sum(f) clipped to [eps, 1 - eps]: loss = -sum(y log p) and, in
+// training, dZ = dL/dz in place:  dL/df_j = (sum of the y's that were not clipped) / sum(f) - [j not clipped] y_j / f_j.  The loss normalises over a whole
+// row, so unlike the element-wise losses it cannot ride in the forward's epilogue.  grid (K, GEN_OUT_CH), 256 threads; workgroup (k, c) takes rows c,
+// c + GEN_OUT_CH, ... and owns slot c of loss_sum; a row's second and third read come from L2.  The slot holds O times the sum of the losses, since the
+// host divides every loss by cells * O.  Sums are float32 per thread, float64 across threads.
+__global__ __launch_bounds__(256) void k_gen_output_cce(float* __restrict__ Z, int ldz, int64_t z_stride, const float* __restrict__ Y, int64_t n_cells,
+                                                        const int32_t* __restrict__ rows, int b_cnt, Dims dm, int train, float inv_n, double* __restrict__ loss_sum) {
+    __shared__ double red[3][4];
+    const int k = blockIdx.x, tid = threadIdx.x;
+    const float eps = 1e-7f;
+    double total = 0.0;
+    auto sum = [&](float v, int slot) -> double {
+        double s = (double)v;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off);
+        if ((tid & 63) == 0) red[slot][tid >> 6] = s;
+        __syncthreads();
+        return (red[slot][0] + red[slot][1]) + (red[slot][2] + red[slot][3]);
+    };
+    for (int b = blockIdx.y; b < b_cnt; b += GEN_OUT_CH) {
+        float* z = Z + (int64_t)k * z_stride + (int64_t)b * ldz;
+        const float* y = Y + ((int64_t)k * n_cells + rows[b]) * dm.Op;
+        float part = 0.f;
+        for (int o = tid; o < dm.O; o += 256) part += softplus_f(z[o]);
+        const float S = (float)sum(part, 0);
+        float loss = 0.f, open = 0.f;
+        for (int o = tid; o < dm.O; o += 256) {
+            const float p = softplus_f(z[o]) / S, yo = y[o];
+            loss -= yo * logf(fminf(fmaxf(p, eps), 1.f - eps));
+            open += p >= eps && p <= 1.f - eps ? yo : 0.f;
+        }
+        total += sum(loss, 1);
+        const float all = (float)sum(open, 2) / S;
+        if (train)
+            for (int o = tid; o < dm.O; o += 256) {
+                float f, sg;
+                softplus_sigmoid_fast(z[o], f, sg);
+                const float p = f / S;
+                z[o] = (all - (p >= eps && p <= 1.f - eps ? y[o] / f : 0.f)) * sg * inv_n;
+            }
+        __syncthreads();                                         // (the next row's sums take the same slots)
+    }
+    if (tid == 0) loss_sum[(int64_t)k * GEN_OUT_CH + blockIdx.y] += total * dm.O;
+}
+
 // Xb[k][b][Dp_k] = X_k[rows[b]][:]  (the batch rows of every sub-net, dense, so that every GEMM operand is a plain matrix)
 template <typename XT>
 __global__ __launch_bounds__(256) void k_gen_gather_batch(const SubnetDev* __restrict__ sn, const XT* __restrict__ X, const int32_t* __restrict__ rows,

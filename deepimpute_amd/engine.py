@@ -194,22 +194,22 @@ class Engine:
 
 class GeneralEngine(Engine):
     """Engine for ANY architecture build() accepts (reference deepimpute/multinet.py:135-162): `layers` = the hidden Dense
-    layers as (neurons, activation name, dropout rate behind it); batch size and widths unrestricted; loss in
-    _cabi.LOSSES.  Same face as Engine; models with several hidden layers move weights per layer."""
+    layers as (neurons, activation name, dropout rate behind it), normalisations as (-1, ("layernormalization", epsilon), dropout
+    rate behind it); batch size and widths unrestricted; loss in _cabi.LOSSES.  Same face as Engine; models with several hidden layers move weights per layer."""
 
     def __init__(self, fns, D, layers, out_dim, batch_size=64, learning_rate=1e-4, beta1=0.9, beta2=0.999, eps=1e-7,
                  loss="wmse", seed=1234, device_id=0, subnet_offset=0, precision="fp32"):
         self._f = fns
         self.D = [int(d) for d in D]
         self.K = len(self.D)
-        self.layers = [(int(n), "linear" if a is None else str(a).lower(), float(p)) for n, a, p in layers]
+        self.layers = [(int(n), a if isinstance(a, tuple) else ("linear" if a is None else str(a).lower()), float(p)) for n, a, p in layers]
         # a leading (0, _, rate) entry: a Dropout layer BEFORE the first Dense layer (dropout on the inputs; include/dimn.h dimn_create_general)
         self.input_dropout = 0.0
         if self.layers and self.layers[0][0] == 0:
             self.input_dropout = self.layers[0][2]
             self.layers = self.layers[1:]
-        if not self.layers:
-            raise ValueError("architecture needs at least one dense layer")
+        if not self.layers or self.layers[0][0] < 0:
+            raise ValueError("architecture needs at least one dense layer" if not self.layers else "a normalisation needs a dense layer before it")
         self.L = len(self.layers)
         self.H = self.layers[0][0]
         self.O = int(out_dim)
@@ -218,8 +218,11 @@ class GeneralEngine(Engine):
         self.loss = str(loss).lower()
         if self.loss not in _cabi.LOSSES:
             raise NotImplementedError("loss %r: implemented are %s" % (loss, sorted(_cabi.LOSSES)))
-        for _, a, _p in self.layers:
-            if a not in _cabi.ACTIVATIONS:
+        for n, a, _p in self.layers:
+            if isinstance(a, tuple):
+                if n >= 0 or a[0] != "layernormalization":
+                    raise ValueError("layer %r" % ((n, a, _p),))
+            elif a not in _cabi.ACTIVATIONS:
                 raise NotImplementedError("hidden activation %r: implemented are %s" % (a, sorted(_cabi.ACTIVATIONS)))
         self.cfg = Config(n_subnets=self.K, subnet_offset=int(subnet_offset), hidden=self.H, out_dim=self.O, batch_size=self.B,
                           device_id=int(device_id), dropout_rate=0.0, learning_rate=float(learning_rate), beta1=float(beta1),
@@ -227,24 +230,30 @@ class GeneralEngine(Engine):
                           precision=_cabi.PRECISIONS[str(precision).lower()])
         self.precision = "bf16" if self.cfg.precision else "fp32"
         wire = ([(0, "linear", self.input_dropout)] if self.input_dropout > 0 else []) + self.layers
-        arr = (_cabi.Layer * len(wire))(*[_cabi.Layer(n, _cabi.ACTIVATIONS[a], p) for n, a, p in wire])
+        arr = (_cabi.Layer * len(wire))(*[_cabi.Layer(0, _cabi.LAYER_NORM, p, float(a[1])) if n < 0 else _cabi.Layer(n, _cabi.ACTIVATIONS[a], p, 0.0) for n, a, p in wire])
+        self.widths = []                                 # outputs of every entry, the output layer last
+        for n, _, _p in self.layers:
+            self.widths.append(n if n > 0 else self.widths[-1])
+        self.widths.append(self.O)
         self._h = C.c_void_p()
         self.n_cells = self.n_train = self.n_val = 0
         self._check(self._f["create_general"](C.byref(self.cfg), p_i32(i32(self.D)), arr, len(wire), _cabi.LOSSES[self.loss], C.byref(self._h)))
         self.activation = self.layers[0][1]
 
     def layer_shape(self, k, layer):
-        widths = [n for n, _, _ in self.layers] + [self.O]
-        return (self.D[k] if layer == 0 else widths[layer - 1]), widths[layer]
+        """Shape of the kernel of entry `layer` ([inputs, units]), or of gamma ([units]) for a normalisation."""
+        if layer < self.L and self.layers[layer][0] < 0:
+            return (self.widths[layer],)
+        return (self.D[k] if layer == 0 else self.widths[layer - 1]), self.widths[layer]
 
     def set_layer_weights(self, k, layer, W, b):
         W, b = f32(W), f32(b)
-        assert W.shape == self.layer_shape(k, layer) and b.shape == (W.shape[1],)
+        assert W.shape == self.layer_shape(k, layer) and b.shape == (W.shape[-1],)
         self._check(self._f["set_layer_weights"](self._h, k, layer, p_f32(W), p_f32(b)))
 
     def get_layer_weights(self, k, layer, which=0):
-        n_in, n_out = self.layer_shape(k, layer)
-        W, b = np.empty((n_in, n_out), np.float32), np.empty(n_out, np.float32)
+        shape = self.layer_shape(k, layer)
+        W, b = np.empty(shape, np.float32), np.empty(shape[-1], np.float32)
         self._check(self._f["get_layer_weights"](self._h, k, layer, int(which), p_f32(W), p_f32(b)))
         return W, b
 

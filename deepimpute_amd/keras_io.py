@@ -149,13 +149,16 @@ def _suffix(base, i):
 def layer_names(K, layers):
     """Keras' automatic names in build()'s creation order (multinet.py:132-146): inputs input_1..input_K; then for every
     architecture entry, one layer per branch; the K output Dense layers last.  -> (inputs, hidden[l][k], dropout[l][k] or None, outputs[k]);
-    hidden[0] is None for a leading (0, _, rate) entry = a Dropout layer before the first Dense layer."""
+    hidden[0] is None for a leading (0, _, rate) entry = a Dropout layer before the first Dense layer; a (-1, _, rate) entry is a normalisation."""
     inputs = ["input_%d" % (k + 1) for k in range(K)]
-    dense_i = drop_i = 0
+    dense_i = drop_i = norm_i = 0
     hidden, drops = [], []
     for units, _, rate in layers:
         if units == 0:                                   # a Dropout layer before the first Dense layer: no Dense of its own
             hidden.append(None)
+        elif units < 0:
+            hidden.append([_suffix("layer_normalization", norm_i + k) for k in range(K)])
+            norm_i += K
         else:
             hidden.append([_suffix("dense", dense_i + k) for k in range(K)])
             dense_i += K
@@ -179,6 +182,12 @@ def model_json(inputdims, layers, out_dim, seed, extra=None):
                            "kernel_initializer": {"class_name": "GlorotUniform", "config": {"seed": None}},
                            "bias_initializer": {"class_name": "Zeros", "config": {}}, "kernel_regularizer": None, "bias_regularizer": None,
                            "activity_regularizer": None, "kernel_constraint": None, "bias_constraint": None}}
+
+    def norm(name, epsilon, src):
+        return {"class_name": "LayerNormalization", "name": name, "inbound_nodes": [[[src, 0, 0, {}]]],
+                "config": {"name": name, "trainable": True, "dtype": "float32", "axis": [1], "epsilon": float(epsilon), "center": True, "scale": True,
+                           "beta_initializer": {"class_name": "Zeros", "config": {}}, "gamma_initializer": {"class_name": "Ones", "config": {}},
+                           "beta_regularizer": None, "gamma_regularizer": None, "beta_constraint": None, "gamma_constraint": None}}
     cfg_layers = [{"class_name": "InputLayer", "name": nm, "inbound_nodes": [],
                    "config": {"batch_input_shape": [None, int(d)], "dtype": "float32", "sparse": False, "ragged": False, "name": nm}}
                   for nm, d in zip(inputs, inputdims)]
@@ -186,7 +195,7 @@ def model_json(inputdims, layers, out_dim, seed, extra=None):
     for l, (units, act, rate) in enumerate(layers):
         if hidden[l] is not None:
             for k in range(K):
-                cfg_layers.append(dense(hidden[l][k], units, act, prev[k]))
+                cfg_layers.append(norm(hidden[l][k], act[1], prev[k]) if units < 0 else dense(hidden[l][k], units, act, prev[k]))
             prev = list(hidden[l])
         if drops[l] is not None:
             for k in range(K):
@@ -232,6 +241,13 @@ def parse_model_json(doc):
                 dn.append(layer["name"])
             elif layer["class_name"] == "Dropout":
                 a.append({"type": "dropout", "rate": float(layer["config"]["rate"])})
+            elif layer["class_name"] == "LayerNormalization":
+                cfg_n = layer["config"]
+                axis = cfg_n.get("axis", [1])
+                if not (cfg_n.get("center", True) and cfg_n.get("scale", True)) or list(axis if isinstance(axis, (list, tuple)) else [axis]) not in ([1], [-1]):
+                    raise NotImplementedError("a normalisation without gamma or beta, or not over the units, in model.json")
+                a.append({"type": "layernormalization", "epsilon": float(cfg_n["epsilon"])})
+                dn.append(layer["name"])
             else:
                 raise NotImplementedError("layer class %r in model.json" % layer["class_name"])
         out_dim = a.pop()["neurons"]                                 # the output Dense is not part of `architecture`
@@ -244,7 +260,8 @@ def parse_model_json(doc):
 
 # ----------------------------------------------------------------------------------------------- weights
 def write_weights_h5(path, layer_order, weights):
-    """Keras 2.x save_weights layout.  layer_order: every layer name of the model in order; weights: {dense name: (kernel [in][out], bias)}."""
+    """Keras 2.x save_weights layout.  layer_order: every layer name of the model in order; weights: {dense name: (kernel [in][out], bias),
+    normalisation name: (gamma, beta)}."""
     h5 = _libhdf5()
     if h5 is None:
         raise OSError("no HDF5 library on this machine")
@@ -256,11 +273,12 @@ def write_weights_h5(path, layer_order, weights):
         for name in layer_order:
             g = _check(h5.H5Gcreate2(f, name.encode(), 0, 0, 0), "H5Gcreate2 " + name)
             arrays = weights.get(name)
-            wn = ["%s/kernel:0" % name, "%s/bias:0" % name] if arrays is not None else []
+            two = ("kernel:0", "bias:0") if arrays is None or np.ndim(arrays[0]) == 2 else ("gamma:0", "beta:0")
+            wn = ["%s/%s" % (name, t) for t in two] if arrays is not None else []
             _write_str_attr(h5, g, "weight_names", wn)
             if arrays is not None:
                 inner = _check(h5.H5Gcreate2(g, name.encode(), 0, 0, 0), "H5Gcreate2 inner " + name)
-                for ds_name, arr in zip(("kernel:0", "bias:0"), arrays):
+                for ds_name, arr in zip(two, arrays):
                     arr = np.ascontiguousarray(arr, np.float32)
                     dims = (C.c_uint64 * arr.ndim)(*arr.shape)
                     space = _check(h5.H5Screate_simple(arr.ndim, dims, None), "H5Screate_simple")

@@ -148,7 +148,9 @@ def _parse_architecture(architecture):
     {"type": "dense", "neurons", "activation"} / {"type": "dropout", "rate"} entries; other types are skipped with the
     reference's message).  Consecutive Dropout layers compose (keep probabilities multiply would change the stream
     semantics, so they are rejected).  A Dropout before the first Dense layer (dropout on the inputs) becomes a leading
-    (0, "linear", rate) entry: the general path masks the batch's predictor rows (dimn_create_general)."""
+    (0, "linear", rate) entry: the general path masks the batch's predictor rows (dimn_create_general).  Extension:
+    {"type": "layernormalization", "epsilon"} (keras.layers.LayerNormalization over the units of the layer before it)
+    becomes (-1, ("layernormalization", epsilon), rate behind it)."""
     from ._cabi import ACTIVATIONS
     layers = []
     for spec in architecture:
@@ -166,6 +168,13 @@ def _parse_architecture(architecture):
             if layers[-1][2] > 0.0:
                 raise NotImplementedError("two Dropout layers in a row (got %r)" % (architecture,))
             layers[-1][2] = float(spec["rate"])
+        elif kind in ("layernormalization", "layer_normalization"):
+            if not layers or layers[0][0] == 0 and len(layers) == 1:
+                raise NotImplementedError("a normalisation of the inputs (got %r): a dense layer is needed before it" % (architecture,))
+            epsilon = float(spec.get("epsilon", 1e-3))
+            if not epsilon >= 0:
+                raise ValueError("layernormalization: epsilon %r is negative or not a number" % (epsilon,))
+            layers.append([-1, ("layernormalization", epsilon), 0.0])
         else:
             print("Unknown layer type.")       # the reference skips such entries (multinet.py:142-143)
     if not [l for l in layers if l[0] > 0]:
@@ -175,7 +184,8 @@ def _parse_architecture(architecture):
 
 def _loss_name(loss):
     """The loss of NN_parameters['loss'] (multinet.py:150-162: the module's wMSE by name or callable, or a keras.losses
-    name) as an id of the engines (_cabi.LOSSES: wmse / wmse_binary / mean_squared_error / mean_absolute_error / msle / logcosh / huber / poisson)."""
+    name) as an id of the engines (_cabi.LOSSES: wmse / wmse_binary / mean_squared_error / mean_absolute_error / msle / logcosh / huber / poisson /
+    categorical_crossentropy)."""
     from ._cabi import LOSSES
     if callable(loss):
         binary = bool(getattr(loss, "keywords", {}) and loss.keywords.get("binary"))       # functools.partial(wMSE, binary=True)
@@ -185,7 +195,7 @@ def _loss_name(loss):
     name = str(loss).lower()
     if name in LOSSES:
         return name
-    print('Unknown loss: {}. Aborting.'.format(loss))       # multinet.py:160-161 (_cabi.LOSSES: wMSE and the element-wise keras.losses)
+    print('Unknown loss: {}. Aborting.'.format(loss))       # multinet.py:160-161 (_cabi.LOSSES: wMSE, the element-wise keras.losses, categorical_crossentropy)
     exit(1)
 
 
@@ -474,7 +484,7 @@ class MultiNet:
                         continue
                     with np.load(path) as z:
                         blobs.update({f: z[f] for f in z.files})
-                n_dense = len([l for l in layers if l[0] > 0]) + 1
+                n_dense = len([l for l in layers if l[0] != 0]) + 1       # (entries with weights: Dense layers and normalisations)
                 missing = [key for k in range(len(dims)) for l in range(1, n_dense + 1) for key in ("W%d_%d" % (l, k), "b%d_%d" % (l, k)) if key not in blobs]
                 if missing and not problem:
                     problem = " the shards lack %d arrays (first: %s)" % (len(missing), missing[0])

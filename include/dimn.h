@@ -92,9 +92,14 @@ int dimn_create(const dimn_config* cfg, const int32_t* D, dimn_handle* out);
  * of the tuned kernels, so both paths train the default architecture on identical masks. */
 typedef struct dimn_layer {
     int32_t neurons;          /* units of the Dense layer                        */
-    int32_t activation;       /* DIMN_ACT_*                                      */
+    int32_t activation;       /* DIMN_ACT_*, or DIMN_LAYER_NORM                  */
     float dropout_rate;       /* rate of the Dropout layer that follows; 0: none */
+    float epsilon;            /* DIMN_LAYER_NORM: added to the variance (ABI 10) */
 } dimn_layer;
+/* ABI 10: an entry with this activation is a normalisation layer (keras.layers.LayerNormalization over the units) behind the entry before it --
+ * never the first Dense layer --, its neurons are ignored: y = gamma (x - mean) / sqrt(var + epsilon) + beta, gamma and beta per sub-net, initially 1
+ * and 0, trained like every other weight.  dimn_set/get_layer_weights move gamma as W and beta as b, [units] each; entries count as layers there. */
+#define DIMN_LAYER_NORM 64
 #define DIMN_LOSS_WMSE 0          /* multinet.py:36-41                                  */
 #define DIMN_LOSS_WMSE_BINARY 1   /* wMSE(binary=True)                                  */
 #define DIMN_LOSS_MSE 2           /* keras.losses.mean_squared_error                    */
@@ -104,7 +109,10 @@ typedef struct dimn_layer {
 #define DIMN_LOSS_LOGCOSH 5       /* logcosh: log(cosh(yhat - y)) = x + softplus(-2x) - log 2                           */
 #define DIMN_LOSS_HUBER 6         /* huber, delta = 1: e^2 / 2 for |e| <= 1, |e| - 1/2 beyond                           */
 #define DIMN_LOSS_POISSON 7       /* poisson: yhat - y log(yhat + eps)                                                  */
-#define DIMN_LOSS_LAST DIMN_LOSS_POISSON
+/* ABI 10: categorical_crossentropy: p = yhat / sum(yhat) over a sub-net's targets, clipped to [eps, 1 - eps]; -sum(y log p) per cell, mean over the
+ * cells (every other loss: mean over cells and targets) */
+#define DIMN_LOSS_CATEGORICAL_CROSSENTROPY 8
+#define DIMN_LOSS_LAST DIMN_LOSS_CATEGORICAL_CROSSENTROPY
 int dimn_create_general(const dimn_config* cfg, const int32_t* D, const dimn_layer* layers, int32_t n_layers,
                         int32_t loss, dimn_handle* out);
 /* Keras-layout kernel W[in][out] and bias[out] of dense layer `layer` (0 .. n_layers; the last one is the output layer);
