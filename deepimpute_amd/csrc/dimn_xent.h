@@ -202,8 +202,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN, li = lane & 15, lj = lane >> 4;
     auto turn = [](int row) { return PL == 1 ? row & 7 : (row >> 2) & 3; };
-    // Workgroup b runs on XCD b % 8: each XCD gets a consecutive range of the tiles, ordered in columns of eight m tiles, so that the 32
-    // workgroups of an XCD at a time share eight A and four B tiles in its L2.
+    // Workgroup b runs on XCD b % 8: each XCD gets a consecutive range of the tiles, ordered in columns of four m tiles, so that the 32
+    // workgroups of an XCD at a time share four A and eight B tiles in its L2 (columns of 8: 1 % more time, of 16: 4 %).
     int tile;
     {
         const int total = p.tiles_m * p.tiles_n, b = blockIdx.x, x = b & 7, q = total >> 3, rem = total & 7;
@@ -211,10 +211,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
     }
     int tm, tn;
     {
-        const int per = 8 * p.tiles_n, grp = tile / per, in = tile - grp * per;
-        const int h = p.tiles_m - grp * 8 < 8 ? p.tiles_m - grp * 8 : 8;
+        const int per = 4 * p.tiles_n, grp = tile / per, in = tile - grp * per;
+        const int h = p.tiles_m - grp * 4 < 4 ? p.tiles_m - grp * 4 : 4;
         tn = in / h;
-        tm = grp * 8 + in - tn * h;
+        tm = grp * 4 + in - tn * h;
     }
     const int m0 = tm * BM, n0 = tn * BN;
     // request c of this wave brings lines [LINE (wave LOADS + c), + LINE) of the stacked planes of [A; B]
