@@ -443,17 +443,32 @@ void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& 
 
 // workgroups of `units` x the row blocks (thin_place)
 int64_t thin_groups(const XentPlan& q, int64_t units) { return (units < 64 ? units : up(units, 8)) * q.blocks; }
+// k_xent_thin with four waves over `k` elements of the inner dimension.  Chunks in fours pay where a wave has several rounds of them: k-contiguous from
+// 64 chunks on (128 x 2922 x 25664 float32 dx: 356 us one by one, 295 in fours; 64 x 800 x 50000 bfloat16 logits: 27 and 33), class-contiguous
+// float32 from 512 (128 x 25664 logits, 1000 wide: 106 and 96 us; 500 wide: 53 and 55).  Class-contiguous bfloat16 and blocks of 64 rows gain
+// nothing (12 x 2000 x 40000: 37 and 41 us).  float32 blocks of up to 32 rows keep a second round in flight (295 against 313 us), the others do
+// better with the registers (64 x 1500 x 20000: 80 against 90).
+template <typename T, bool VC, int NF, int EPI>
+void thin_launch(const rowops::Thin& p, int64_t k, unsigned groups, int tiles, int ranges, int blocks, hipStream_t st) {
+    constexpr int FOURS = VC ? (sizeof(T) == 4 && NF <= 2 ? 1 : 0) : (sizeof(T) == 4 && NF <= 2 ? 2 : 1);
+    if constexpr (FOURS > 0)
+        if (k >= (VC ? 512 : (sizeof(T) == 2 ? 2048 : 1024))) {
+            hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF, EPI, 4, FOURS>), dim3(groups), dim3(256), 0, st, p, tiles, ranges, blocks);
+            return;
+        }
+    hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF, EPI, 4, 0>), dim3(groups), dim3(256), 0, st, p, tiles, ranges, blocks);
+}
 // the logits' product: epilogue XE_LSE or XE_GRAD
 template <typename T, int EPI>
 void xent_thin(const XentPlan& q, const rowops::Thin& p, hipStream_t st) {
-    const dim3 grid((unsigned)thin_groups(q, q.tiles_n));
+    const unsigned groups = (unsigned)thin_groups(q, q.tiles_n);
     const int tiles = (int)q.tiles_n, blocks = (int)q.blocks;
     // sixteen waves per workgroup while that leaves CUs to spare and every wave still has chunks of k
     const bool deep = q.nf <= 2 && q.tiles_n * q.blocks <= q.ncu && q.H >= 512;
 #define THIN(VC, NF)                                                                                                                              \
     do {                                                                                                                                          \
-        if (NF <= 2 && deep) hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF <= 2 ? NF : 1, EPI, 16>), grid, dim3(1024), 0, st, p, tiles, 1, blocks);  \
-        else hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF, EPI, 4>), grid, dim3(256), 0, st, p, tiles, 1, blocks);                              \
+        if (NF <= 2 && deep) hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF <= 2 ? NF : 1, EPI, 16, 0>), dim3(groups), dim3(1024), 0, st, p, tiles, 1, blocks);  \
+        else thin_launch<T, VC, NF, EPI>(p, q.H, groups, tiles, 1, blocks, st);                                                                  \
     } while (0)
     if (q.out_in) { if (q.nf == 1) THIN(false, 1); else if (q.nf == 2) THIN(false, 2); else THIN(false, 4); }
     else { if (q.nf == 1) THIN(true, 1); else if (q.nf == 2) THIN(true, 2); else THIN(true, 4); }
@@ -524,11 +539,10 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
         else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
 #undef BOTH
     } else {
-        const dim3 gx((unsigned)dx_groups);
 #define DX(NF, EPI)                                                                                                                                        \
     do {                                                                                                                                                   \
-        if (vc) hipLaunchKernelGGL((rowops::k_xent_thin<T, true, NF, EPI, 4>), gx, dim3(256), 0, st, a, tiles, ranges, blocks);                            \
-        else hipLaunchKernelGGL((rowops::k_xent_thin<T, false, NF, EPI, 4>), gx, dim3(256), 0, st, a, tiles, ranges, blocks);                              \
+        if (vc) thin_launch<T, true, NF, EPI>(a, q.V / ranges, (unsigned)dx_groups, tiles, ranges, blocks, st);                                           \
+        else thin_launch<T, false, NF, EPI>(a, q.V / ranges, (unsigned)dx_groups, tiles, ranges, blocks, st);                                             \
     } while (0)
         if (ranges == 1) { if (q.nf == 1) DX(1, rowops::XE_STORE); else if (q.nf == 2) DX(2, rowops::XE_STORE); else DX(4, rowops::XE_STORE); }
         else { if (q.nf == 1) DX(1, rowops::XE_ADD); else if (q.nf == 2) DX(2, rowops::XE_ADD); else DX(4, rowops::XE_ADD); }

@@ -3,7 +3,7 @@
 // With few rows the logits, dx and dW are bound by reading (or writing) the kernel once, and what dimn_xent.h does first -- laying the operands
 // out as k-contiguous bfloat16 planes -- costs more than the products: for float32 it moves 16 bytes per weight where 4 have to be read.  Here
 // the matrix instructions take their operands straight from global memory, in whichever order the caller holds the kernel:
-//   * k-contiguous (KC): a lane loads 16 bytes of one class row; float32: element r feeds instruction r (any assignment of k's to the slots of
+//   * k-contiguous (KC): a lane gets 16 bytes of one class row; float32: element r feeds instruction r (any assignment of k's to the slots of
 //     v_mfma_f32_16x16x4_f32 gives the same sum as long as the rows' operand follows it); bfloat16: the eight k's of one 16x16x32 instruction.
 //   * class-contiguous (VC): a lane loads four consecutive classes of one k; element j belongs to class set j, whose sixteen classes lie four
 //     apart -- a permutation of the classes inside the workgroup's 64 that the epilogue undoes.
@@ -36,56 +36,54 @@ template <typename T> struct Four;             // four consecutive elements of a
 template <> struct Four<float> { typedef f32x4u vec; };
 template <> struct Four<bf16_t> { typedef u16x4u vec; };
 
-// (class tile, k-range, row block) of one workgroup; `ranges` k-ranges in all
-template <typename T, bool VC, int NF, int EPI, int NW>
+// the 4 x 4 of v[t] over the lanes of a quad, transposed: lane q's v[t] becomes lane t's v[q] (li: the lane's number)
+template <typename V>
+__device__ __forceinline__ void quad_transpose(V (&v)[4], int li) {
+    constexpr int D = sizeof(V) / 4;
+    typedef uint32_t words __attribute__((ext_vector_type(D)));
+    words w[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w[t] = __builtin_bit_cast(words, v[t]);
+    const bool odd = li & 1, high = li & 2;
+    auto swap = [](uint32_t& x, uint32_t& y, bool upper, auto ctrl) {
+        const uint32_t fx = __builtin_amdgcn_mov_dpp((int)x, decltype(ctrl)::value, 15, 15, true), fy = __builtin_amdgcn_mov_dpp((int)y, decltype(ctrl)::value, 15, 15, true);
+        x = upper ? fy : x;
+        y = upper ? y : fx;
+    };
+    constexpr std::integral_constant<int, 0xB1> by_one{};       // quad_perm [1, 0, 3, 2]
+    constexpr std::integral_constant<int, 0x4E> by_two{};       // quad_perm [2, 3, 0, 1]
+#pragma unroll
+    for (int e = 0; e < D; ++e) {
+        uint32_t x[4] = {w[0][e], w[1][e], w[2][e], w[3][e]};
+        swap(x[0], x[1], odd, by_one);
+        swap(x[2], x[3], odd, by_one);
+        swap(x[0], x[2], high, by_two);
+        swap(x[1], x[3], high, by_two);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) w[t][e] = x[t];
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) v[t] = __builtin_bit_cast(V, w[t]);
+}
+
+// (class tile, k-range, row block) of one workgroup; `ranges` k-ranges in all.  FOURS: sets of four chunks per wave in registers (0: chunks one by one)
+template <typename T, bool VC, int NF, int EPI, int NW, int FOURS>
 __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range, int ranges, int block) {
     constexpr bool BF = sizeof(T) == 2, WIDE = BF && !VC;      // WIDE: the 16x16x32 instruction, eight k's per lane
     constexpr int EL = WIDE ? 8 : 4, KS = 4 * EL, NS = VC ? 4 : 2, CW = VC ? 64 : 32, ROWS = 16 * NF, LD = CW + 4;
-    // Chunks requested together.  KC: two sets of them in registers, one in flight while the other is multiplied (3 x 1901 x 81826 float32: 145 ->
-    // 122 us, 5.1 TB/s).  VC needs twice the registers for that, and the workgroups a CU loses by it cost more (846 x 64 x 18203: 62 -> 91 us).
-    constexpr int SETS = VC ? 1 : 2, U = VC ? (NF > 2 || NW > 4 ? 2 : 4) : (NF > 1 || NW > 4 ? 2 : 4);
     __shared__ __attribute__((aligned(16))) float red[NW / 2][ROWS][LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, lj = lane >> 4;
     const int64_t c0 = (int64_t)tile * CW, m0 = (int64_t)block * ROWS;
     const T* A = (const T*)p.A;
     const T* B = (const T*)p.B;
-    const T* arow[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        int64_t m = m0 + 16 * f + li;
-        m = m < p.M ? m : p.M - 1;                              // rows and classes past the end repeat the last one: never stored
-        arow[f] = A + m * p.lda;
-    }
-    const T* bptr[VC ? 1 : 2];
-    if constexpr (VC) {
-        const int64_t c = c0 + 4 * li;
-        bptr[0] = B + (c < p.N - 4 ? c : p.N - 4);              // (N >= 4: the caller's rule)
-    } else {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int64_t c = c0 + 16 * s + li;
-            bptr[s] = B + (c < p.N ? c : p.N - 1) * p.ldb;
-        }
-    }
     typedef typename std::conditional<BF, typename std::conditional<WIDE, u16x8u, u16x4u>::type, f32x4u>::type avec;
     typedef typename std::conditional<VC, typename Four<T>::vec, avec>::type bvec;
     constexpr int NB = VC ? 4 : 2;
-    avec a[SETS][U][NF];
-    bvec b[SETS][U][NB];
     f32x4 acc[NF][NS];
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int s = 0; s < NS; ++s) acc[f][s] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    auto request = [&](int64_t k, avec (&ra)[NF], bvec (&rb)[NB]) {
-#pragma unroll
-        for (int q = 0; q < NB; ++q) {
-            if constexpr (VC) rb[q] = *(const bvec*)(bptr[0] + (k + 4 * lj + q) * p.ldb);
-            else rb[q] = *(const bvec*)(bptr[q] + k + EL * lj);
-        }
-#pragma unroll
-        for (int f = 0; f < NF; ++f) ra[f] = *(const avec*)(arow[f] + k + EL * lj);
-    };
     auto multiply = [&](const avec (&ra)[NF], const bvec (&rb)[NB]) {
         if constexpr (WIDE) {
 #pragma unroll
@@ -112,49 +110,173 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
     // this workgroup's range of whole chunks; the chunk that crosses K belongs to the last range
     const int64_t whole = p.K / KS;
     const int64_t cbeg = whole * range / ranges, cend = whole * (range + 1) / ranges;
-    // whole rounds of U consecutive chunks per wave (256 bytes of a class row at a time), then single chunks
-    const int64_t rounds = (cend - cbeg) / (NW * U);
-    auto fetch = [&](int64_t i, int set) {
-        const int64_t c = cbeg + (NW * (i < rounds ? i : rounds - 1) + wave) * U;
+    // Four chunks at a time.  A lane that loaded its own 16 bytes of sixteen rows would have each lane looked up by itself (64 cache accesses per
+    // load measured, one per cycle and CU: 128 x 2922 x 25664 float32 dx was bound by them, 335 us).  So the lanes of a quad read 64 consecutive
+    // bytes of a row, in four loads those of four rows, and transpose the 4 x 4 among them: element [u] of a lane is then the 16 bytes at
+    // k + EL (4 lj + u) of its own row.  Offsets from the workgroup's first row take 32 bits (rows further apart go chunk by chunk below).
+    const int64_t nc = FOURS > 0 && p.lda < (1 << 24) && p.ldb < (1 << 24) ? cend - cbeg : 0;
+    const int64_t full = nc / (4 * NW), left = nc % (4 * NW);
+    const int quads = left > 2 * NW ? (int)left / 4 : 0;         // waves that take four more chunks: what is left over would cost as many single ones
+    const int64_t rounds = full + (wave < quads);
+    if constexpr (FOURS > 0) {
+        const int quad = li & ~3, part = 4 * lj + (li & 3);
+        const char* abase = (const char*)(A + m0 * p.lda);
+        const char* bbase = (const char*)(VC ? B : B + c0 * p.ldb);
+        uint32_t aoff[NF][4], boff[VC ? 1 : 2][4];
 #pragma unroll
-        for (int u = 0; u < U; ++u) request((c + u) * KS, a[set][u], b[set][u]);
-    };
-    auto consume = [&](int set) {
+        for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int u = 0; u < U; ++u) multiply(a[set][u], b[set][u]);
-    };
-    if constexpr (SETS == 1) {
-        for (int64_t i = 0; i < rounds; ++i) { fetch(i, 0); consume(0); }
-    } else if (rounds > 0) {
-        // (the barriers keep the compiler from moving every load down to its use)
-        fetch(0, 0);
-        for (int64_t i = 0; i + 1 < rounds; i += 2) {
-            fetch(i + 1, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(0);
-            __builtin_amdgcn_sched_barrier(0);
-            fetch(i + 2, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(1);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int t = 0; t < 4; ++t) {
+                const int64_t r = m0 + 16 * f + quad + t;           // rows and classes past the end repeat the last one: never stored
+                aoff[f][t] = (uint32_t)(((r < p.M ? r : p.M - 1) - m0) * p.lda + EL * part) * (uint32_t)sizeof(T);
+            }
+        if constexpr (VC) {
+            const int64_t c = c0 + 4 * li;
+            boff[0][0] = (uint32_t)(16 * lj * p.ldb) * (uint32_t)sizeof(T);
+            bbase += (c0 < p.N - 4 ? c0 : p.N - 4) * (int64_t)sizeof(T);
+            boff[0][0] += (uint32_t)((c < p.N - 4 ? c : p.N - 4) - (c0 < p.N - 4 ? c0 : p.N - 4)) * (uint32_t)sizeof(T);     // (N >= 4: the caller's rule)
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const int64_t r = c0 + 16 * s + quad + t;
+                    boff[s][t] = (uint32_t)(((r < p.N ? r : p.N - 1) - c0) * p.ldb + EL * part) * (uint32_t)sizeof(T);
+                }
         }
-        if (rounds & 1) consume(0);
+        const auto place = [&](int64_t i) -> int64_t {              // first k of the wave's round i (past its last: of the last)
+            i = i < rounds ? i : rounds - 1;
+            return (cbeg + (i < full ? 4 * (NW * i + wave) : 4 * NW * full + 4 * wave)) * KS;
+        };
+        const auto read_rows = [&](int64_t k, avec (&a)[NF][4]) {
+            const char* ak = abase + k * (int64_t)sizeof(T);
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) a[f][t] = *(const avec*)(ak + aoff[f][t]);
+        };
+        const auto chunk = [&](const avec (&a)[NF][4], int u, const bvec (&rb)[NB]) {
+            avec ra[NF];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) ra[f] = a[f][u];
+            multiply(ra, rb);
+        };
+        // (the barriers below keep the compiler from moving every load down to its use)
+        if constexpr (VC) {
+            // classes: a chunk ahead; rows: a round ahead
+            avec a[2][NF][4];
+            bvec b[2][NB];
+            const auto read_classes = [&](int64_t k, int u) {
+                const char* bk = bbase + (k + 4 * u) * p.ldb * (int64_t)sizeof(T);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) b[u & 1][q] = *(const bvec*)(bk + q * p.ldb * (int64_t)sizeof(T) + boff[0][0]);
+            };
+            const auto round = [&](int64_t i, int set) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    read_classes(place(i + (u == 3)), (u + 1) & 3);
+                    if (u == 0) read_rows(place(i + 1), a[set ^ 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (u == 0)
+#pragma unroll
+                        for (int f = 0; f < NF; ++f) quad_transpose(a[set][f], li);
+                    chunk(a[set], u, b[u & 1]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            if (rounds > 0) {
+                read_rows(place(0), a[0]);
+                read_classes(place(0), 0);
+                for (int64_t i = 0; i + 1 < rounds; i += 2) { round(i, 0); round(i + 1, 1); }
+                if (rounds & 1) round(rounds - 1, 0);
+            }
+        } else {
+            avec a[FOURS][NF][4];
+            bvec b[FOURS][NB][4];
+            const auto fetch = [&](int64_t i, int set) {
+                const int64_t k = place(i);
+                const char* bk = bbase + k * (int64_t)sizeof(T);
+#pragma unroll
+                for (int q = 0; q < NB; ++q)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) b[set][q][t] = *(const bvec*)(bk + boff[q][t]);
+                read_rows(k, a[set]);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            const auto consume = [&](int set) {
+#pragma unroll
+                for (int f = 0; f < NF; ++f) quad_transpose(a[set][f], li);
+#pragma unroll
+                for (int q = 0; q < NB; ++q) quad_transpose(b[set][q], li);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    bvec rb[NB];
+#pragma unroll
+                    for (int q = 0; q < NB; ++q) rb[q] = b[set][q][u];
+                    chunk(a[set], u, rb);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if constexpr (FOURS == 1) {
+                for (int64_t i = 0; i < rounds; ++i) { fetch(i, 0); consume(0); }
+            } else if (rounds > 0) {
+                fetch(0, 0);
+                for (int64_t i = 0; i + 1 < rounds; i += 2) {
+                    fetch(i + 1, FOURS - 1);
+                    consume(0);
+                    fetch(i + 2, 0);
+                    consume(FOURS - 1);
+                }
+                if (rounds & 1) consume(0);
+            }
+        }
     }
-    for (int64_t c = cbeg + rounds * NW * U + wave; c < cend; c += NW) { request(c * KS, a[0][0], b[0][0]); multiply(a[0][0], b[0][0]); }
-    if (whole * KS < p.K && range == ranges - 1 && wave == (int)(whole % NW)) {
+    // single chunks, from the first wave without four more; then the chunk that crosses K
+    const T* arow[NF];
+    const T* bptr[VC ? 1 : 2];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int64_t m = m0 + 16 * f + li;
+        arow[f] = A + (m < p.M ? m : p.M - 1) * p.lda;
+    }
+    if constexpr (VC) {
+        const int64_t c = c0 + 4 * li;
+        bptr[0] = B + (c < p.N - 4 ? c : p.N - 4);
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int64_t c = c0 + 16 * s + li;
+            bptr[s] = B + (c < p.N ? c : p.N - 1) * p.ldb;
+        }
+    }
+    avec ra[NF];
+    bvec rb[NB];
+    const int64_t single = cbeg + 4 * NW * full + 4 * quads;
+    const int turn = (wave + NW - quads % NW) % NW;
+    for (int64_t c = single + turn; c < cend; c += NW) {
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+            if constexpr (VC) rb[q] = *(const bvec*)(bptr[0] + (c * KS + 4 * lj + q) * p.ldb);
+            else rb[q] = *(const bvec*)(bptr[q] + c * KS + EL * lj);
+        }
+#pragma unroll
+        for (int f = 0; f < NF; ++f) ra[f] = *(const avec*)(arow[f] + c * KS + EL * lj);
+        multiply(ra, rb);
+    }
+    if (whole * KS < p.K && range == ranges - 1 && turn == (int)((cend - single) % NW)) {
         const int64_t k = whole * KS;
 #pragma unroll
         for (int q = 0; q < NB; ++q)
 #pragma unroll
             for (int i = 0; i < (VC ? 4 : EL); ++i) {
-                if constexpr (VC) b[0][0][q][i] = k + 4 * lj + q < p.K ? bptr[0][(k + 4 * lj + q) * p.ldb + i] : (T)0;
-                else b[0][0][q][i] = k + EL * lj + i < p.K ? bptr[q][k + EL * lj + i] : (T)0;
+                if constexpr (VC) rb[q][i] = k + 4 * lj + q < p.K ? bptr[0][(k + 4 * lj + q) * p.ldb + i] : (T)0;
+                else rb[q][i] = k + EL * lj + i < p.K ? bptr[q][k + EL * lj + i] : (T)0;
             }
 #pragma unroll
         for (int f = 0; f < NF; ++f)
 #pragma unroll
-            for (int i = 0; i < EL; ++i) a[0][0][f][i] = k + EL * lj + i < p.K ? arow[f][k + EL * lj + i] : (T)0;
-        multiply(a[0][0], b[0][0]);
+            for (int i = 0; i < EL; ++i) ra[f][i] = k + EL * lj + i < p.K ? arow[f][k + EL * lj + i] : (T)0;
+        multiply(ra, rb);
     }
     // element r of acc[f][s]: row 16 f + li, position 16 s + 4 lj + r (KC) / 4 (4 lj + r) + s (VC) of the workgroup's classes
     auto put = [&](int slot) {
@@ -449,21 +571,21 @@ __device__ __forceinline__ void thin_place(int b, int units, int blocks, int& un
     block = rest % blocks;
     unit = rest / blocks * 8 + (b & 7);
 }
-template <typename T, bool VC, int NF, int EPI, int NW>
+template <typename T, bool VC, int NF, int EPI, int NW, int FOURS>
 __global__ __launch_bounds__(64 * NW) void k_xent_thin(const Thin p, int tiles, int ranges, int blocks) {
     int unit, block;
     thin_place(blockIdx.x, tiles * ranges, blocks, unit, block);
     if (unit >= tiles * ranges) return;
-    thin_product<T, VC, NF, EPI, NW>(p, unit % tiles, unit / tiles, ranges, block);
+    thin_product<T, VC, NF, EPI, NW, FOURS>(p, unit % tiles, unit / tiles, ranges, block);
 }
 template <typename T, int SETS>
 __global__ __launch_bounds__(256) void k_xent_thin_dw(const ThinDw w) {
     thin_dw<T, SETS>(w, blockIdx.x % w.tiles, blockIdx.x / w.tiles);
 }
 
-// dx and dW in one launch, while both are small: both read G and neither waits for the other, and each is mostly latency (64 x 256 x 20000 float32:
-// 30 us apart, 25 together).  Larger ones run apart, with the registers each of them needs (12 x 3648 x 22455: 156 us apart, 180 together).  The first `dx_groups` workgroups
-// multiply for dx (tiles x ranges x row blocks), the others for dW.
+// dx and dW in one launch, while both are small: both read G and neither waits for the other, and each is mostly latency (float32, 10 x 800 x 8000:
+// 18.2 us apart, 16.2 together; 130 x 200 x 3000: 27 and 21).  Larger ones run apart, with the registers each of them needs (12 x 3648 x 22455: 127 us
+// apart, 154 together).  The first `dx_groups` workgroups multiply for dx (tiles x ranges x row blocks), the others for dW.
 template <typename T, bool VC, int NF, int EPI>
 __global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const ThinDw w, int dx_groups, int tiles, int ranges, int blocks) {
     const int b = blockIdx.x;
@@ -471,7 +593,7 @@ __global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const Thin
         int unit, block;
         thin_place(b, tiles * ranges, blocks, unit, block);
         if (unit >= tiles * ranges) return;
-        thin_product<T, VC, NF, EPI, 4>(a, unit % tiles, unit / tiles, ranges, block);
+        thin_product<T, VC, NF, EPI, 4, 0>(a, unit % tiles, unit / tiles, ranges, block);
     } else thin_dw<T, 1>(w, (b - dx_groups) % w.tiles, (b - dx_groups) / w.tiles);
 }
 
