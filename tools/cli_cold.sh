@@ -20,7 +20,6 @@ PY
     /tmp/counts_to_csv /tmp/$name.bin $n $g $csv && rm -f /tmp/$name.bin
   fi
   ls -la $csv | awk '{print "input:", $5/1e6, "MB"}'
-  sync; echo 3 > /proc/sys/vm/drop_caches 2>/dev/null      # a cold file system where the box lets us
   t0=$(date +%s.%N)
   DIMN_TRACE=1 python -m deepimpute_amd.deepImpute $csv -o /tmp/$name.out.csv --limit $g "$@" > $O/$name.out 2> $O/$name.err
   rc=$?
