@@ -180,7 +180,7 @@ int norm_backward(hipStream_t st, int32_t type, int64_t groups, NormP p, float* 
 static int norm_check(const char* who, int32_t type, int64_t groups, int64_t rows, int64_t width) {
     if (type != DIMN_TYPE_F32 && type != DIMN_TYPE_BF16) return dimn_fail(DIMN_ERR_UNSUP, "%s: element type %d (DIMN_TYPE_F32 or DIMN_TYPE_BF16)", who, type);
     if (groups < 0 || rows < 0 || groups > INT32_MAX || rows > INT32_MAX) return dimn_fail(DIMN_ERR_ARG, "%s: %lld groups of %lld rows", who, (long long)groups, (long long)rows);
-    if (width < 1 || width > (1 << 28)) return dimn_fail(DIMN_ERR_ARG, "%s: width %lld not in 1..2^28", who, (long long)width);
+    if (width < 1 || width > (1 << 26)) return dimn_fail(DIMN_ERR_ARG, "%s: width %lld not in 1..2^26", who, (long long)width);
     return DIMN_OK;
 }
 
@@ -320,7 +320,7 @@ struct XentPlan {
         const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0));
         const int64_t budget = (int64_t)512 << 20;
         P = per_class ? std::max<int64_t>(256, budget / per_class / 256 * 256) : up(V, 256);
-        P = std::min(std::min(P, far), up(V, 256));
+        P = std::min({P, far, up(V, 256), std::max<int64_t>(256, ((int64_t)1 << 22) / std::max<int64_t>(1, ceil_div64(N, 256)) * 256)});      // (the last: a launch has fewer than 2^32 threads)
         if (P < V && !w_direct) P = best_piece(P);
         else if (P < V && grad) P = best_piece(P);
         t_logits = pick_tile(f32, N, std::min(P, V), ncu);
@@ -485,10 +485,12 @@ rowops::Thin xent_thin_logits(const XentPlan& q) {
 }
 void xent_tsum(const XentPlan& q, float* tsum, hipStream_t st) {
     const dimn_output_loss* d = q.d;
-    if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(1024), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
+    const unsigned threads = q.N < 1 << 20 ? 1024 : 256;        // (a launch has fewer than 2^32 of them; so many rows fill the device anyhow)
+    if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(threads), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
 }
 rowops::SplitSum split_sum(const float* acc, int splits, int64_t rows, int64_t cols, void* out, int64_t ld) {
-    return {acc, rows * cols, splits, (int32_t)ceil_div64(rows * cols, 256), rows, cols, out, ld};
+    const int32_t per = rows * cols >= 1 << 20 ? 4 : 1;          // (4096 x 2048 bfloat16, two splits: 32 us one by one, 21 by four)
+    return {acc, rows * cols, splits, (int32_t)ceil_div64(rows * cols, 256 * per), per, rows, cols, out, ld};
 }
 void xent_finish(bool f32, const rowops::XentFinish& f, hipStream_t st) {
     const unsigned blocks = (unsigned)(f.m[0].blocks + f.m[1].blocks + (f.dbias && f.parts ? ceil_div64(f.classes, 256) : 0));

@@ -588,18 +588,19 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
 __global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t kind, int64_t target_row, int64_t classes, float* __restrict__ tsum) {
     const int64_t row = blockIdx.x;
     __shared__ float red[16];
+    const int64_t step = 4 * (int64_t)blockDim.x;
     float s = 0.f;
     if (kind == XT_F32) {
         const float* t = (const float*)target + row * target_row;
 #pragma unroll 4
-        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += 4096) {
+        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += step) {
             if (c + 4 <= classes) { const f32x4u v = *(const f32x4u*)(t + c); s += (v[0] + v[1]) + (v[2] + v[3]); }
             else for (int64_t k = c; k < classes; ++k) s += t[k];
         }
     } else {
         const uint16_t* t = (const uint16_t*)target + row * target_row;
 #pragma unroll 4
-        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += 4096) {
+        for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += step) {
             if (c + 4 <= classes) { const u16x4u v = *(const u16x4u*)(t + c); s += (from_bf16(v[0]) + from_bf16(v[1])) + (from_bf16(v[2]) + from_bf16(v[3])); }
             else for (int64_t k = c; k < classes; ++k) s += from_bf16(t[k]);
         }
@@ -610,16 +611,16 @@ __global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t 
     __syncthreads();
     if (threadIdx.x == 0) {
         s = 0.f;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) s += red[w];
+        for (int w = 0; w < (int)blockDim.x / 64; ++w) s += red[w];
         tsum[row] = s;
     }
 }
 
 // What is left of a backward pass, in one launch: out[m][n] = the sum of the splits' float32 sums for up to two matrices (dx, dW), dbias = the sum of
-// the partial column sums, each added in order and rounded once.  A thread takes one element: neighbours are neighbours in every split.
+// the partial column sums, each added in order and rounded once.  A thread takes one element of a small matrix, four consecutive ones of a large one.
 struct SplitSum {
     const float* acc; int64_t split; int32_t splits, blocks;     // [splits][rows][cols], `split` elements apart; blocks = 0: nothing to do
+    int32_t per;                                                 // 1 / 4 elements per thread
     int64_t rows, cols;
     void* out; int64_t ld;
 };
@@ -636,13 +637,30 @@ __global__ __launch_bounds__(256) void k_xent_finish(const XentFinish p) {
     for (int w = 0; w < 2; ++w) {
         if (block < p.m[w].blocks) {
             const SplitSum& q = p.m[w];
-            const int64_t e = (int64_t)block * 256 + threadIdx.x;
-            if (e >= q.rows * q.cols) return;
-            float s = 0.f;
+            const int64_t e = ((int64_t)block * 256 + threadIdx.x) * q.per, all = q.rows * q.cols;
+            if (e >= all) return;
+            int64_t m = e / q.cols, n = e - m * q.cols;
+            T* out = (T*)q.out + m * q.ld + n;
+            auto rounded = [](float v) -> T { if constexpr (sizeof(T) == 4) return v; else return to_bf16(v); };
+            if (q.per == 1) {
+                float s = 0.f;
 #pragma unroll 8
-            for (int k = 0; k < q.splits; ++k) s += q.acc[k * q.split + e];
-            const int64_t m = e / q.cols, n = e - m * q.cols;
-            if constexpr (sizeof(T) == 4) ((float*)q.out)[m * q.ld + n] = s; else ((uint16_t*)q.out)[m * q.ld + n] = to_bf16(s);
+                for (int k = 0; k < q.splits; ++k) s += q.acc[k * q.split + e];
+                *out = rounded(s);
+            } else if (n + 4 <= q.cols) {
+                typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+                f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                for (int k = 0; k < q.splits; ++k) s += *(const f32x4u*)(q.acc + k * q.split + e);
+                *(four*)out = (four){rounded(s[0]), rounded(s[1]), rounded(s[2]), rounded(s[3])};
+            } else {                                             // the end of a row, or of everything
+                for (int64_t i = e; i < e + 4 && i < all; ++i) {
+                    float s = 0.f;
+                    for (int k = 0; k < q.splits; ++k) s += q.acc[k * q.split + i];
+                    ((T*)q.out)[m * q.ld + n] = rounded(s);
+                    if (++n == q.cols) { n = 0; ++m; }
+                }
+            }
             return;
         }
         block -= p.m[w].blocks;

@@ -411,6 +411,7 @@ int dimn_col_stats_var(const double* a, int64_t n, int64_t g, int64_t ld, const 
 /* Layer normalisation of [groups][rows] rows of `width` elements (keras.layers.LayerNormalization, axis -1):
  *   y = (x - mean) * rstd * gamma + beta,  rstd = 1 / sqrt(mean((x - mean)^2) + eps).
  * x, y of element type `type`; gamma, beta float32 [groups][width] (NULL: 1 / 0); mean, rstd float32 [groups][rows] (NULL: not wanted).
+ * width: 1 to 2^26.
  * y may be x when their strides agree. */
 int dimn_layer_norm(int32_t device_id, void* stream, int32_t type, int64_t groups, int64_t rows, int64_t width,
                     const void* x, int64_t x_group, int64_t x_row, const float* gamma, const float* beta, float eps,
@@ -451,7 +452,7 @@ int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, int32_t grad,
 /* loss, lse: float32 [rows]. */
 int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream, float* loss, float* lse, void* workspace, int64_t workspace_bytes);
 /* The backward pass from the forward's lse and the gradient dloss [rows] of the losses: dx [rows][width], dkernel [width][classes] (strides
- * as the kernel's, one of them 1), both of element type `type`, and dbias float32 [classes] (NULL: not wanted). */
+ * as the kernel's, one of them 1), both of element type `type`, and dbias float32 [classes] (NULL: not wanted).  rows = 0 is refused here. */
 int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* stream, const float* dloss, const float* lse, void* dx, int64_t dx_row,
                                    void* dkernel, int64_t dkernel_in, int64_t dkernel_out, float* dbias, void* workspace, int64_t workspace_bytes);
 

@@ -143,6 +143,83 @@ def test_large(dtype, rows, width, classes, order, target):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,classes,order", [
+    ("f32", 12, 1480, 20011, "out_in"), ("f32", 30, 1537, 18004, "out_in"), ("f32", 60, 1100, 20011, "out_in"), ("f32", 12, 1480, 20011, "in_out"),
+    ("f32", 30, 1537, 18004, "in_out"), ("f32", 101, 700, 20011, "in_out"), ("bf16", 12, 2300, 20011, "out_in"), ("bf16", 30, 2061, 18004, "out_in"),
+    ("bf16", 60, 2432, 20011, "out_in"), ("bf16", 12, 2061, 20011, "in_out"), ("bf16", 60, 1300, 40001, "in_out"),
+])
+def test_few_rows_of_wide_layers(dtype, rows, width, classes, order):
+    """Few rows of long inner dimensions: whole rounds of chunks, leftovers of every kind behind them, blocks of 16 / 32 / 64 rows."""
+    _check(rows, width, classes, dtype, order, "labels")
+
+
+@pytest.mark.gpu
+def test_rows_far_apart():
+    """Strides of 2^24 elements and more, where an offset inside a tile passes 32 bits: x's rows, then the rows of a kernel in either order."""
+    from deepimpute_amd import ops
+    far = (1 << 24) + 4
+
+    def check(x, kernel, t, b, dloss):
+        loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+        ref = _reference(x, kernel, t, b, dloss)
+        _close("lse", lse, *ref["lse"])
+        _close("loss", loss, *ref["loss"])
+        for name, got in zip(("dx", "dkernel", "dbias"), ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)):
+            _close(name, got, *ref[name])
+
+    def spread(a):
+        wide = torch.empty((a.shape[0], far), dtype=a.dtype, device="cuda")
+        wide[:, :a.shape[1]] = a
+        return wide[:, :a.shape[1]]
+    for order in ("out_in", "in_out"):
+        x, kernel, t, b, dloss = _problem(20, 1500, 20011, torch.float32, order)
+        check(spread(x), kernel, t, b, dloss)
+        x, kernel, t, b, dloss = _problem(300, 200, 500, torch.bfloat16, order)
+        check(spread(x), kernel, t, b, dloss)
+    x, kernel, t, b, dloss = _problem(3, 8, 600001, torch.float32, "in_out")
+    check(x, spread(kernel), t, b, dloss)
+    x, kernel, t, b, dloss = _problem(3, 2100, 8, torch.bfloat16, "out_in")
+    check(x, spread(kernel.t()).t(), t, b, dloss)
+    x, kernel, t, b, dloss = _problem(200, 300, 40, torch.bfloat16, "out_in")
+    check(x, spread(kernel.t()).t(), t, b, dloss)
+
+
+@pytest.mark.gpu
+def test_broadcast_inputs():
+    """Axes of stride 0: the same row for every sample, one profile for all of them, a kernel of equal rows or columns."""
+    from deepimpute_amd import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        for rows in (9, 200):
+            x, kernel, t, b, dloss = _problem(rows, 70, 90, dtype, "in_out", "profile")
+            for X, K, T in ((x[1:2].expand(rows, 70), kernel, t[1:2].expand(rows, 90)), (x, kernel[:1].expand(70, 90), t), (x, kernel[:, :1].expand(70, 90), t),
+                            (x, kernel, t[:, :1].expand(rows, 90)), (x[:, :1].expand(rows, 70), kernel, t)):
+                got = ops.linear_cross_entropy(X, K, T, b)
+                ref = _reference(X, K, T, b, dloss)
+                _close("loss", got[0], *ref["loss"])
+                for name, g in zip(("dx", "dkernel", "dbias"), ops.linear_cross_entropy_grad(dloss, X, K, T, got[1], b)):
+                    _close(name, g, *ref[name])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,width,classes", [("f32", 4, 5), ("bf16", 64, 40)])
+def test_most_rows(dtype, width, classes):
+    """2^22 rows of a profile, the most a call takes: the losses and dx of the first and the last rows, and the sums over all of them."""
+    from deepimpute_amd import ops
+    rows = 1 << 22
+    x, kernel, t, b, dloss = _problem(rows, width, classes, DTYPES[dtype], "in_out", "profile")
+    loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+    dx, dk, db = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        ref = _reference(x[part], kernel, t[part], b, dloss[part])
+        _close("lse", lse[part], *ref["lse"])
+        _close("loss", loss[part], *ref["loss"])
+        _close("dx", dx[part], *ref["dx"])
+    ref = _reference(x, kernel, t, b, dloss)
+    _close("dkernel", dk, *ref["dkernel"])
+    _close("dbias", db, *ref["dbias"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [50, 150])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides(dtype, rows):

@@ -195,6 +195,52 @@ def test_no_rows_and_in_place():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_in_place_at_every_form(dtype):
+    """y over x, dx over dy and dx over x: short rows, rows of 16 / 64 / 256 / 1024 threads with and without a moved last piece, rows read thrice."""
+    from deepimpute_amd import ops
+    fns = _lib.load()
+    s = torch.cuda.current_stream().cuda_stream
+    kind = 0 if dtype == torch.float32 else 1
+    for width in (3, 37, 128, 301, 1027, 2401, 9001, 16385, 40003):
+        rows = 300 if width < 3000 else 9
+        x, dy = _make((rows, width), dtype, width), _make((rows, width), dtype, width + 1)
+        gamma = 1 + 0.1 * _make((width,), torch.float32, 3)
+        want, mean, rstd = ops.layer_norm(x, gamma)
+        y = x.clone()
+        assert fns["layer_norm"](0, s, kind, 1, rows, width, y.data_ptr(), 0, width, gamma.data_ptr(), None, 1e-3, y.data_ptr(), 0, width, None, None) == 0
+        assert torch.equal(y, want), width
+        dx, _, _ = ops.layer_norm_grad(dy, x, mean, rstd, gamma)
+        for over in ("dy", "x"):
+            a, b = dy.clone(), x.clone()
+            out = a if over == "dy" else b
+            assert fns["layer_norm_grad"](0, s, kind, 1, rows, width, a.data_ptr(), 0, width, b.data_ptr(), 0, width, mean.data_ptr(), rstd.data_ptr(),
+                                          gamma.data_ptr(), out.data_ptr(), 0, width, None, None, None, 0) == 0
+            assert torch.equal(out, dx), (width, over)
+
+
+@pytest.mark.gpu
+def test_longest_row():
+    """A row of 2^26 elements, the most there may be; a thread adds 2^16 of them one after the other: 2^16 + 64 half steps of the largest term."""
+    from deepimpute_amd import ops
+    width = 1 << 26
+    steps = (width / 1024 + 64) * F32
+    x, dy = _make((1, width), torch.float32, 1), _make((1, width), torch.float32, 2)
+    gamma = 1 + 0.1 * torch.rand(width, device="cuda")
+    y, mean, rstd = ops.layer_norm(x, gamma, None)
+    want, wmean, wrstd = _formula(x, gamma, None, 1e-3)
+    top = float(x.abs().max())
+    assert abs(float(mean) - float(wmean)) <= steps * top and abs(float(rstd) / float(wrstd) - 1) <= 2 * steps
+    _close(y, want, 2 * steps * (want.abs() + 1.2 * top))
+    dx, dgamma, dbeta = ops.layer_norm_grad(dy, x, mean, rstd, gamma)
+    want, wg, wb, xh = _formula_grad(dy, x, mean, rstd, gamma)
+    size = 1.2 * float(dy.abs().max()) * (1 + float(xh.abs().max()))
+    _close(dx, want, float(rstd) * (steps * size * (1 + xh.abs()) + 8 * F32 * size))
+    _close(dgamma, wg, 8 * F32 * wg.abs() + 1e-30)
+    assert torch.equal(dbeta, dy[0])
+
+
+@pytest.mark.gpu
 def test_values_at_the_edges():
     """Constant rows (spread 0), rows far from zero, huge and tiny values, an infinity or NaN stays in its row."""
     from deepimpute_amd import ops
@@ -282,6 +328,7 @@ def test_refusals_on_the_host():
     assert "element type" in message(norm(kind=7), -4)
     assert "width" in message(norm(width=0), -1)
     assert "width" in message(norm(width=1 << 40), -1)
+    assert "width" in message(norm(width=(1 << 26) + 1), -1)
     assert "rows" in message(norm(rows=-1), -1)
     assert "null" in message(norm(x=None), -1)
     assert "null" in message(norm(y=None), -1)
