@@ -318,11 +318,12 @@ struct XentPlan {
         w_direct = !f32 && out_in && H % 64 == 0 && aligned(d->kernel) && d->kernel_out % 8 == 0 && d->kernel_out <= far && d->kernel_out >= 0;
         wt_direct = !f32 && !out_in && V % 64 == 0 && aligned(d->kernel) && d->kernel_in % 8 == 0 && d->kernel_in <= far && d->kernel_in >= 0;
         const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0));
-        const int64_t budget = (int64_t)512 << 20;
+        // A piece's operands take up to 1 GiB: 4096 x 2048 x 64000 / x 100000 bfloat16 backward 3.02 / 4.66 ms (512 MiB: 3.09 / 4.88, 192 MiB: 3.17 / 5.02,
+        // 4 GiB: 2.93 / 4.78 -- but that keeps as much as the logits).
+        const int64_t budget = (int64_t)1 << 30;
         P = per_class ? std::max<int64_t>(256, budget / per_class / 256 * 256) : up(V, 256);
         P = std::min({P, far, up(V, 256), std::max<int64_t>(256, ((int64_t)1 << 22) / std::max<int64_t>(1, ceil_div64(N, 256)) * 256)});      // (the last: a launch has fewer than 2^32 threads)
-        if (P < V && !w_direct) P = best_piece(P);
-        else if (P < V && grad) P = best_piece(P);
+        if (P < V && (grad || !w_direct)) P = best_piece(P);
         t_logits = pick_tile(f32, N, std::min(P, V), ncu);
         tiles_m = ceil_div64(N, kTiles[f32][t_logits].bm);
         tiles_n = ceil_div64(V, kTiles[f32][t_logits].bn);

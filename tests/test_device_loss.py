@@ -154,6 +154,18 @@ def test_few_rows_of_wide_layers(dtype, rows, width, classes, order):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,classes,order,target", [
+    ("f32", 3001, 64, 40007, "out_in", "labels"),
+    ("f32", 300, 4000, 47001, "in_out", "labels64"),
+    ("bf16", 8200, 70, 40011, "in_out", "profile16"),
+    ("bf16", 8200, 64, 70003, "out_in", "labels"),
+])
+def test_several_pieces(dtype, rows, width, classes, order, target):
+    """More classes than one piece of the workspace holds: the last piece is an odd one, dx adds up over all of them."""
+    _check(rows, width, classes, dtype, order, target)
+
+
+@pytest.mark.gpu
 def test_rows_far_apart():
     """Strides of 2^24 elements and more, where an offset inside a tile passes 32 bits: x's rows, then the rows of a kernel in either order."""
     from deepimpute_amd import ops
