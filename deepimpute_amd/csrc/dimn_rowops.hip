@@ -286,8 +286,9 @@ struct XentPlan {
         }
         return best;
     }
-    // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 256 .. 4096 and 300 .. 32000
-    // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles)
+    // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 64 .. 4096 and 300 .. 50000
+    // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles).  Backward: a least-squares fit to 98
+    // shapes of 40 .. 800 rows; the form it takes costs 0.4 % more than the better one on average, 26 % at worst.
     bool prefers_thin() const {
         const double hv = (double)H * (double)V, work = hv * (double)N, steps = (f32 ? 2.0 : 0.5) * (double)(Hp / 64);
         double t, g;
@@ -296,9 +297,9 @@ struct XentPlan {
             g = (x_direct ? 0 : 5) + (w_direct ? 0 : 5 + hv * (f32 ? 3.9e-6 : 0.9e-6));
             g += std::max(work * (f32 ? 8e-6 : 2.1e-6) * 1e-3, steps) - 4;
         } else {
-            const double nv = (double)N * (double)V * 1e-6 / 4;  // (G is written and read: 12 / 6 bytes an entry, laid out for the large products 24 / 8)
-            t = work * (f32 ? 62e-6 : 22e-6) * 1e-3 + 0.01 * (double)N + nv * (f32 ? 12 : 6);
-            g = 25 + hv * (f32 ? 10e-6 : 2e-6) + std::max(work * (f32 ? 30e-6 : 7e-6) * 1e-3, steps) + nv * (f32 ? 24 : 8);
+            const double weights = hv * 1e-6, gs = (double)N * (double)V * 1e-6, padded = (double)Hp * (double)V * (double)up(N, 128);
+            t = (f32 ? 24 : 22) + hv * (double)up(N, f32 ? 32 : 64) * (f32 ? 70e-9 : 20e-9) + (f32 ? 0 : 0.5) * weights + (f32 ? 3.9 : 3.3) * gs;
+            g = (f32 ? 41 : 33) + padded * (f32 ? 28e-9 : 6e-9) + (f32 ? 4.6 : 2.0) * weights + (f32 ? 5.7 : 1.8) * gs + (f32 ? 0.027 : 0.001) * (double)Hp;
         }
         return t < g;
     }
@@ -331,9 +332,10 @@ struct XentPlan {
         // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.
         thin = V >= 4 && H >= 4 && prefers_thin();
         if (thin) {
-            // 64 rows per block read the kernel least often, 32 give twice the workgroups (and, class-contiguous float32, half the registers)
+            // 64 rows per block read the kernel least often, 32 give twice the workgroups.  float32, bound by the matrix instructions: up to 32, half the
+            // registers (64 / 80 x 1344 x 28165 logits 82 / 120 us, with 64 rows 94 / 143), 16 where a third of two blocks of 32 would be no rows (48: 75, 81 us)
             tiles_n = ceil_div64(V, out_in ? 32 : 64);
-            nf = N <= 16 ? 1 : (N <= 32 || (f32 && !out_in) || tiles_n * ceil_div64(N, 64) < 2 * ncu ? 2 : 4);
+            nf = N <= 16 || (f32 && N > 32 && N <= 48) ? 1 : (N <= 32 || f32 || tiles_n * ceil_div64(N, 64) < 2 * ncu ? 2 : 4);
             blocks = ceil_div64(N, 16 * nf);
             if (!grad) {
                 part = take(8 * tiles_n * N);
@@ -444,14 +446,15 @@ void xent_logits(const XentPlan& q, char* ws, int64_t c0, int64_t pv, XentGemm& 
 
 // workgroups of `units` x the row blocks (thin_place)
 int64_t thin_groups(const XentPlan& q, int64_t units) { return (units < 64 ? units : up(units, 8)) * q.blocks; }
+template <typename T> constexpr int kRows = sizeof(T) == 2 ? 4 : 2;      // the largest XentPlan::nf
 // k_xent_thin with four waves over `k` elements of the inner dimension.  Chunks in fours pay where a wave has several rounds of them: k-contiguous from
 // 64 chunks on (128 x 2922 x 25664 float32 dx: 356 us one by one, 295 in fours; 64 x 800 x 50000 bfloat16 logits: 27 and 33), class-contiguous
-// float32 from 512 (128 x 25664 logits, 1000 wide: 106 and 96 us; 500 wide: 53 and 55).  Class-contiguous bfloat16 and blocks of 64 rows gain
-// nothing (12 x 2000 x 40000: 37 and 41 us).  float32 blocks of up to 32 rows keep a second round in flight (295 against 313 us), the others do
-// better with the registers (64 x 1500 x 20000: 80 against 90).
+// float32 from 512 (128 x 25664 logits, 1000 wide: 106 and 96 us; 500 wide: 53 and 55).  Class-contiguous bfloat16 gains
+// nothing (12 x 2000 x 40000: 37 and 41 us).  float32 keeps a second round in flight (295 against 313 us), bfloat16 does
+// better with the registers (64 x 1500 x 20000: 21 against 23).
 template <typename T, bool VC, int NF, int EPI>
 void thin_launch(const rowops::Thin& p, int64_t k, unsigned groups, int tiles, int ranges, int blocks, hipStream_t st) {
-    constexpr int FOURS = VC ? (sizeof(T) == 4 && NF <= 2 ? 1 : 0) : (sizeof(T) == 4 && NF <= 2 ? 2 : 1);
+    constexpr int FOURS = VC ? (sizeof(T) == 4 ? 1 : 0) : (sizeof(T) == 4 ? 2 : 1);
     if constexpr (FOURS > 0)
         if (k >= (VC ? 512 : (sizeof(T) == 2 ? 2048 : 1024))) {
             hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF, EPI, 4, FOURS>), dim3(groups), dim3(256), 0, st, p, tiles, ranges, blocks);
@@ -471,8 +474,8 @@ void xent_thin(const XentPlan& q, const rowops::Thin& p, hipStream_t st) {
         if (NF <= 2 && deep) hipLaunchKernelGGL((rowops::k_xent_thin<T, VC, NF <= 2 ? NF : 1, EPI, 16, 0>), dim3(groups), dim3(1024), 0, st, p, tiles, 1, blocks);  \
         else thin_launch<T, VC, NF, EPI>(p, q.H, groups, tiles, 1, blocks, st);                                                                  \
     } while (0)
-    if (q.out_in) { if (q.nf == 1) THIN(false, 1); else if (q.nf == 2) THIN(false, 2); else THIN(false, 4); }
-    else { if (q.nf == 1) THIN(true, 1); else if (q.nf == 2) THIN(true, 2); else THIN(true, 4); }
+    if (q.out_in) { if (q.nf == 1) THIN(false, 1); else if (q.nf == 2) THIN(false, 2); else THIN(false, kRows<T>); }
+    else { if (q.nf == 1) THIN(true, 1); else if (q.nf == 2) THIN(true, 2); else THIN(true, kRows<T>); }
 #undef THIN
 }
 rowops::Thin xent_thin_logits(const XentPlan& q) {
@@ -538,8 +541,8 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
         if (vc) hipLaunchKernelGGL((rowops::k_xent_thin_both<T, true, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_groups, tiles, ranges, blocks);          \
         else hipLaunchKernelGGL((rowops::k_xent_thin_both<T, false, NF, EPI>), grid, dim3(256), 0, st, a, w, dx_groups, tiles, ranges, blocks);            \
     } while (0)
-        if (ranges == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(4, rowops::XE_STORE); }
-        else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(4, rowops::XE_ADD); }
+        if (ranges == 1) { if (q.nf == 1) BOTH(1, rowops::XE_STORE); else if (q.nf == 2) BOTH(2, rowops::XE_STORE); else BOTH(kRows<T>, rowops::XE_STORE); }
+        else { if (q.nf == 1) BOTH(1, rowops::XE_ADD); else if (q.nf == 2) BOTH(2, rowops::XE_ADD); else BOTH(kRows<T>, rowops::XE_ADD); }
 #undef BOTH
     } else {
 #define DX(NF, EPI)                                                                                                                                        \
@@ -547,12 +550,11 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
         if (vc) thin_launch<T, true, NF, EPI>(a, q.V / ranges, (unsigned)dx_groups, tiles, ranges, blocks, st);                                           \
         else thin_launch<T, false, NF, EPI>(a, q.V / ranges, (unsigned)dx_groups, tiles, ranges, blocks, st);                                             \
     } while (0)
-        if (ranges == 1) { if (q.nf == 1) DX(1, rowops::XE_STORE); else if (q.nf == 2) DX(2, rowops::XE_STORE); else DX(4, rowops::XE_STORE); }
-        else { if (q.nf == 1) DX(1, rowops::XE_ADD); else if (q.nf == 2) DX(2, rowops::XE_ADD); else DX(4, rowops::XE_ADD); }
+        if (ranges == 1) { if (q.nf == 1) DX(1, rowops::XE_STORE); else if (q.nf == 2) DX(2, rowops::XE_STORE); else DX(kRows<T>, rowops::XE_STORE); }
+        else { if (q.nf == 1) DX(1, rowops::XE_ADD); else if (q.nf == 2) DX(2, rowops::XE_ADD); else DX(kRows<T>, rowops::XE_ADD); }
 #undef DX
         const dim3 gw((unsigned)(w.tiles * w.ranges));
-        if (q.N > 64) hipLaunchKernelGGL((rowops::k_xent_thin_dw<T, 2>), gw, dim3(256), 0, st, w);
-        else hipLaunchKernelGGL((rowops::k_xent_thin_dw<T, 1>), gw, dim3(256), 0, st, w);
+        hipLaunchKernelGGL((rowops::k_xent_thin_dw<T>), gw, dim3(256), 0, st, w);
     }
     rowops::XentFinish f{};
     if (q.splits > 1) f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);

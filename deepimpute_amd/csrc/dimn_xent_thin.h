@@ -10,7 +10,7 @@
 // float32 runs on the exact float32 matrix instructions: at 64 rows their rate (154 TFLOP/s measured) and the HBM's meet.
 // Measured: one row x 1024 x 32000 bfloat16 14.4 us = 4.6 TB/s; 12 x 2000 x 40000 bfloat16 dx 27 us = 5.8 TB/s (part of the kernel still lies in the
 // memory-side cache); 12 x 3648 x 22455 float32 dx 67, dW 59 us = 4.9, 5.5 TB/s, class-contiguous logits 115 us = 2.9 TB/s; 128 x 2922 x 25664 float32
-// 241 / 296 / 236 us (logits / dx / dW), 80 / 65 / 82 TFLOP/s.
+// 241 / 296 / 234 us (logits / dx / dW), 80 / 65 / 82 TFLOP/s.
 // A workgroup owns 32 (KC) / 64 (VC) classes x up to 64 rows; its waves (four, or sixteen where there are few workgroups and a long inner
 // dimension: 3840 x 222 float32 ran 45 us with four) share the chunks of k and are added through LDS, upper half onto lower half, in a fixed order.
 #pragma once
@@ -471,9 +471,9 @@ struct ThinDw {
     int32_t tiles_b, tiles;                    // workgroups along b (256 columns each), in all
     int32_t ranges; float* acc;                // ranges > 1: range r of the rows leaves its float32 sums in acc[r][na][nb]
 };
-// SETS = 2: sixteen rows in flight while sixteen are multiplied; for more than 64 rows (106 x 2922 x 25672 float32: 280 -> 233 us; with 12 rows the
-// registers it takes cost 56 -> 95 us)
-template <typename T, int SETS>
+// Sixteen rows at a time, no more of them in flight: the registers of a second sixteen cost more workgroups than they hide latency (80 x 1344 x 28165
+// float32: 91 against 106 us; 12 rows 33 us = 4.6 TB/s), and a copy of the loads without the test for the last row changes nothing.
+template <typename T>
 __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const T *P = (const T*)p.P, *Q = (const T*)p.Q;
     T* C = (T*)p.C;
@@ -492,23 +492,23 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const vec zero = {0, 0, 0, 0};
-    vec a[SETS][4], b[SETS][4];
-    auto fetch = [&](int64_t k, int set) {
+    vec a[4], b[4];
+    auto fetch = [&](int64_t k) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t row = BF ? k + 4 * lj + r : k + 4 * r + lj;       // bfloat16: four consecutive rows make one lane's operand
-            a[set][r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
-            b[set][r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
+            a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
+            b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
         }
     };
-    auto consume = [&](int set) {
+    auto consume = [&] {
         if constexpr (BF) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const s16x4 u = {(short)a[set][0][i], (short)a[set][1][i], (short)a[set][2][i], (short)a[set][3][i]};
+                const s16x4 u = {(short)a[0][i], (short)a[1][i], (short)a[2][i], (short)a[3][i]};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const s16x4 v = {(short)b[set][0][j], (short)b[set][1][j], (short)b[set][2][j], (short)b[set][3][j]};
+                    const s16x4 v = {(short)b[0][j], (short)b[1][j], (short)b[2][j], (short)b[3][j]};
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(u, v, acc[i][j], 0, 0, 0);
                 }
             }
@@ -518,24 +518,10 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[set][r][i], b[set][r][j], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][i], b[r][j], acc[i][j], 0, 0, 0);
         }
     };
-    if constexpr (SETS == 1) {
-        for (int64_t k = beg; k < n; k += 16) { fetch(k, 0); consume(0); }
-    } else {
-        fetch(beg, 0);
-        for (int64_t k = beg; k < n; k += 32) {
-            fetch(k + 16, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(0);
-            __builtin_amdgcn_sched_barrier(0);
-            fetch(k + 32, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            consume(1);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+    for (int64_t k = beg; k < n; k += 16) { fetch(k); consume(); }
     // acc[i][j][r]: a = set i of lane 4 lj + r, b = set j of lane li
     const bool whole = cb == b0 + 4 * li;
 #pragma unroll
@@ -581,9 +567,9 @@ __global__ __launch_bounds__(64 * NW) void k_xent_thin(const Thin p, int tiles, 
     if (unit >= tiles * ranges) return;
     thin_product<T, VC, NF, EPI, NW, FOURS>(p, unit % tiles, unit / tiles, ranges, block);
 }
-template <typename T, int SETS>
+template <typename T>
 __global__ __launch_bounds__(256) void k_xent_thin_dw(const ThinDw w) {
-    thin_dw<T, SETS>(w, blockIdx.x % w.tiles, blockIdx.x / w.tiles);
+    thin_dw<T>(w, blockIdx.x % w.tiles, blockIdx.x / w.tiles);
 }
 
 // dx and dW in one launch, while both are small: both read G and neither waits for the other, and each is mostly latency (float32, 10 x 800 x 8000:
@@ -597,7 +583,7 @@ __global__ __launch_bounds__(256) void k_xent_thin_both(const Thin a, const Thin
         thin_place(b, tiles * ranges, blocks, unit, block);
         if (unit >= tiles * ranges) return;
         thin_product<T, VC, NF, EPI, 4, 0>(a, unit % tiles, unit / tiles, ranges, block);
-    } else thin_dw<T, 1>(w, (b - dx_groups) % w.tiles, (b - dx_groups) / w.tiles);
+    } else thin_dw<T>(w, (b - dx_groups) % w.tiles, (b - dx_groups) / w.tiles);
 }
 
 }  // namespace rowops
