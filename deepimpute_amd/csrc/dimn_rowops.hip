@@ -589,6 +589,7 @@ extern "C" int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, in
     const char* who = "dimn_linear_cross_entropy_workspace";
     CHK(xent_check(who, d));
     if (!bytes) return dimn_fail(DIMN_ERR_ARG, "%s: null", who);
+    if (d->rows == 0) { *bytes = 0; return DIMN_OK; }            // (nothing to plan: a plan divides by the number of row blocks)
     OnDevice on;
     CHK(on.enter(who, d->device_id));
     XentPlan q;
@@ -645,14 +646,14 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
                                               void* dkernel, int64_t dkernel_in, int64_t dkernel_out, float* dbias, void* workspace, int64_t workspace_bytes) {
     const char* who = "dimn_linear_cross_entropy_grad";
     CHK(xent_check(who, d));
-    if (!dkernel || (d->rows > 0 && (!dloss || !lse || !dx))) return dimn_fail(DIMN_ERR_ARG, "%s: null array", who);
+    if (d->rows == 0) return dimn_fail(DIMN_ERR_ARG, "%s: no rows", who);
+    if (!dkernel || !dloss || !lse || !dx) return dimn_fail(DIMN_ERR_ARG, "%s: null array", who);
     if (dkernel_in != 1 && dkernel_out != 1) return dimn_fail(DIMN_ERR_ARG, "%s: one of the strides of dkernel (%lld, %lld) has to be 1", who, (long long)dkernel_in, (long long)dkernel_out);
     OnDevice on;
     CHK(on.enter(who, d->device_id));
     hipStream_t st = (hipStream_t)stream;
     XentPlan q;
     q.make(d, true, compute_units(d->device_id));
-    if (d->rows == 0) return dimn_fail(DIMN_ERR_ARG, "%s: no rows", who);
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
     if (q.thin) {

@@ -447,7 +447,7 @@ typedef struct dimn_output_loss {
     int64_t target_row;
     int32_t target_kind;          /* DIMN_TARGET_*                                              */
 } dimn_output_loss;
-/* Bytes of workspace (256-byte aligned) of the forward (grad = 0) / backward (grad != 0) call. */
+/* Bytes of workspace (256-byte aligned) of the forward (grad = 0) / backward (grad != 0) call; 0 without rows. */
 int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, int32_t grad, int64_t* bytes);
 /* loss, lse: float32 [rows]. */
 int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream, float* loss, float* lse, void* workspace, int64_t workspace_bytes);

@@ -447,6 +447,21 @@ def test_refusals_on_the_host():
     assert fns["linear_cross_entropy"](_describe(rows=0), None, 4096, 4096, None, 0) == 0
 
 
+@pytest.mark.parametrize("target_kind", [0, 3])
+@pytest.mark.parametrize("kind", [0, 1])
+def test_no_rows_at_the_c_entries(kind, target_kind):
+    """rows = 0: no workspace for either direction, nothing to do forward, refused backward -- before a plan is made (no GPU needed)."""
+    fns = _lib.load()
+    for width, classes in ((8, 16), (2048, 32000), (3, 2)):
+        d = _describe(type=kind, rows=0, width=width, classes=classes, kernel_in=classes, target_kind=target_kind, x=None, kernel=None, target=None)
+        for grad in (0, 1):
+            n = C.c_int64(-1)
+            assert fns["linear_cross_entropy_workspace"](d, grad, n) == 0 and n.value == 0
+        assert fns["linear_cross_entropy"](d, None, None, None, None, 0) == 0
+        assert fns["linear_cross_entropy_grad"](d, None, None, None, None, width, 4096, classes, 1, None, None, 0) == -1
+        assert b"no rows" in fns["last_error"]()
+
+
 def test_refusals_of_tensors():
     from deepimpute_amd import ops
     x, k, t = torch.zeros((4, 8)), torch.zeros((8, 16)), torch.zeros(4, dtype=torch.int32)
