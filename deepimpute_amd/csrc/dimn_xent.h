@@ -11,7 +11,7 @@
 //     for 256 logits), k_xent_lse joins them.
 //   * Backward, per piece of the classes: the logits again, G of the piece in the epilogue -- kept in both memory orders, because each of the
 //     two products that read it wants its own inner dimension contiguous --, then dx += G W^T and dW = x^T G of the piece.
-//   * float32 operands are split into three bfloat16 terms each (8 + 8 + 8 bits of the 24-bit significand, exact), and the six products whose
+//   * float32 operands are split into three bfloat16 terms each (8 + 8 + 8 bits of the 24-bit significand; exact from 2^-110 up), and the six products whose
 //     weight is 2^-16 or more are summed: what is left out is below 2^-23 of a product, the rounding of a float32 product itself.  Six passes
 //     of the bf16 matrix cores still have 2.7 times the rate of the float32 ones.
 //   * Operands that are k-contiguous, aligned and a multiple of 64 long are read in place; everything else is laid out by k_xent_lay.
@@ -34,15 +34,24 @@ typedef uint16_t u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 __device__ __forceinline__ float from_bf16(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 
-// x = hi + mid + lo, each a bfloat16.  The remainders are exact (Sterbenz); an infinity or NaN stays in the first term alone.
+// The next term of a float32 number in bfloat16 terms, the first of three unless it is the `last`; what is left of the number stays in `rest`: three
+// terms hold every finite one of 2^-110 or more exactly.  Values within half a step of the largest float32 would round to an infinity and take the largest bfloat16
+// instead; the remainders are exact either way (Sterbenz; above, 16 bits are left).
+// An infinity is the LAST term, its sign the others: so it is multiplied by the other operand's first term alone, which has the operand's own sign
+// and is 0 where the operand is.  As the first term it would also meet the second and third ones, which are 0 or have the other sign, and make a
+// NaN of inf x 0.5.  What its other terms add is finite and has the sign of the result.  A NaN is every term.
+__device__ __forceinline__ uint16_t split_term(float& rest, bool last) {
+    if (last) return to_bf16(rest);
+    constexpr float top = 3.38953139e38f;                        // (2 - 2^-7) 2^127
+    const float size = fabsf(rest);
+    const bool inf = size == INFINITY;
+    const uint16_t b = to_bf16(inf || size > top ? copysignf(inf ? 1.f : top, rest) : rest);
+    rest = inf ? rest : rest - from_bf16(b);
+    return b;
+}
 __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
-    b[0] = to_bf16(x);
-    const float hi = from_bf16(b[0]);
-    const bool finite = fabsf(hi) <= 3.38953139e38f;
-    const float r1 = finite ? x - hi : 0.f;
-    b[1] = to_bf16(r1);
-    const float r2 = r1 - from_bf16(b[1]);
-    b[2] = to_bf16(r2);
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) b[pl] = split_term(x, pl == 2);
 }
 
 // ---- operand layout -----------------------------------------------------------------------------------------------------------
@@ -506,8 +515,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                     for (int j = 0; j < FN; ++j)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            o[i][4 * j + r] = to_bf16(acc[i][j][r]);
-                            if (pl + 1 < PL) acc[i][j][r] -= from_bf16(o[i][4 * j + r]);
+                            float rest = acc[i][j][r];
+                            o[i][4 * j + r] = split_term(rest, pl + 1 == PL);
+                            acc[i][j][r] = rest;
                         }
                 uint16_t* G = p.G + pl * p.g_plane;
                 uint16_t* GT = p.GT + pl * p.gt_plane;

@@ -325,6 +325,80 @@ def test_masks_and_odd_labels(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,classes", [(9, 128, 300), (4000, 128, 2001)])
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_masks_in_the_operands(dtype, order, rows, width, classes):
+    """The lowest value and infinities in the kernel and in x, few rows and many: a class they mask is not there, a product with 0 is 0 (lowest value),
+    and nothing spreads to other classes or rows."""
+    from deepimpute_amd import ops
+    dt = DTYPES[dtype]
+    low, inf = torch.finfo(dt).min, float("inf")
+    x, kernel, t, b, dloss = _problem(rows, width, classes, dt, order)
+    x[:, 5] = 0
+    x[:, 7] = x[:, 7].abs() + 0.25
+    x[2, 9], x[3, 9] = low, -low
+    kernel[9] = 0                                                    # (x's lowest and largest value meet zeros only)
+    kernel[5], kernel[7] = 0, 0
+    masked = torch.zeros(classes, dtype=torch.bool, device="cuda")
+    masked[1::3] = True
+    t = torch.where((t >= 0) & masked[t.clamp(min=0).long()], t - 1, t)              # labels that are there
+    keep = torch.nonzero(~masked).squeeze(1)
+    place = torch.cumsum(~masked, 0) - 1
+    sub_t = torch.where(t >= 0, place[t.clamp(min=0).long()].to(t.dtype), t)
+    ref = _reference(x, kernel[:, keep], sub_t, b[keep], dloss)
+    for at_zero, mask in ((0.0, low), (low, low), (-low, low), (0.0, -inf), (low, -inf)):
+        k = kernel.clone()
+        k[5, ::2] = at_zero                                          # meets x = 0
+        k[7, masked] = mask                                          # meets x >= 0.25
+        loss, lse = ops.linear_cross_entropy(x, k, t, b)
+        _close("lse", lse, *ref["lse"])
+        _close("loss", loss, *ref["loss"])
+        dx, dk, db = ops.linear_cross_entropy_grad(dloss, x, k, t, lse, b)
+        assert not bool(dk[:, masked].any()) and not bool(db[masked].any())
+        rest = [i for i in range(width) if i not in (5, 7)]          # (there dx multiplies the masks themselves)
+        _close("dx", dx[:, rest], *(v[:, rest] for v in ref["dx"]))
+        _close("dkernel", dk[:, keep], *ref["dkernel"])
+        _close("dbias", db[keep], *(v for v in ref["dbias"]))
+        if mask == low and at_zero == 0.0:
+            assert bool(torch.isfinite(dx).all())
+    # an infinite input: a logit of -infinity, or a row without a softmax, never another row
+    y = x.clone()
+    y[4, 9] = -inf
+    k = kernel.clone()
+    k[9] = 0.5
+    k[9, ~masked] = -0.5
+    y[2, 9], y[3, 9] = 0, inf
+    loss, lse = ops.linear_cross_entropy(y, k, t, b)
+    assert bool(lse[4].isnan()) and not bool(lse[[0, 1, 2] + list(range(5, rows))].isnan().any())
+    k[9] = 0.5
+    k[9, keep[1]] = 1e-3 if dtype == "bf16" else 1.000001e-3         # one of them with terms of either sign
+    y[4, 9], y[3, 9] = -inf, 0
+    _, lse = ops.linear_cross_entropy(y, k, t, b)
+    assert float(lse[4]) == -inf                                     # every logit is -infinity: no class left
+    for a, c in ((inf, -inf), (-inf, inf), (inf, low), (low, inf)):
+        y[4, 9], k[9] = a, c
+        y[[r for r in range(rows) if r != 4], 9] = 1
+        _, lse = ops.linear_cross_entropy(y, k, t, b)
+        assert float(lse[4]) == -inf
+    # values within half a bfloat16 step of the largest float32, times small ones
+    if dtype == "f32":
+        k = kernel.clone()
+        k[11] = 3.4e38
+        y = x.clone()
+        y[:, 11] = torch.linspace(-1e-30, 1e-30, rows, device="cuda")
+        loss, lse = ops.linear_cross_entropy(y, k, t, b)
+        ref = _reference(y, k, t, b)
+        _close("lse", lse, *ref["lse"])
+        y[:, 11] = 0
+        loss, lse = ops.linear_cross_entropy(y, k, t, b)
+        k[11] = 0
+        ref = _reference(y, k, t, b)
+        _close("lse", lse, *ref["lse"])
+        _close("loss", loss, *ref["loss"])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("target", ["labels", "profile"])
 def test_gradient_against_differences(target):
     """Central differences of sum(dloss * loss) of the float64 formula at the float32 point."""
