@@ -258,7 +258,7 @@ struct XentPlan {
     int64_t tiles_m, tiles_n;                 // logits
     int t_dx, splits, t_dw, dw_splits;
     bool thin; int nf; int64_t blocks;        // few rows: dimn_xent_thin.h; 16 nf rows per block
-    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, dbias, acc, acc_w, bytes;
+    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, weight, dbias, acc, acc_w, bytes;
 
     // The largest piece allowed, or a smaller one whose 256 x 256 tiles fill the device in whole rounds: a piece of 84 class tiles at 16 row tiles
     // takes 6 rounds of 256 workgroups where 96 class tiles take the same six (64000 classes: 16 rounds instead of 18, 8 instead of 9 for dW).
@@ -347,6 +347,7 @@ struct XentPlan {
             }
             g = take((f32 ? 4 : 2) * N * V);
             tsum = take(4 * N);
+            weight = labels ? 0 : take(4 * N);
             dbias = take(4 * blocks * V);
             const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
             splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, ceil_div64(4 * ncu, wgs), chunks / 2}));
@@ -369,6 +370,7 @@ struct XentPlan {
         g = take(2 * planes * N * P);
         gt = take(2 * planes * P * Np);
         tsum = take(4 * N);
+        weight = labels ? 0 : take(4 * N);
         dbias = take(4 * tiles_m * kTiles[f32][t_logits].wm * V);
         // dx has few tiles and a long inner dimension, so has dW of a narrow layer: ranges of it, each with float32 sums of its own
         const int64_t pv = std::min(P, V);
@@ -407,9 +409,9 @@ void xent_gemm(bool f32, int tile, int splits, XentGemm& p, hipStream_t st) {
 // Operands to lay out, gathered and launched together
 struct Lay {
     rowops::LayJobs jobs{};
-    void add(bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane) {
+    void add(bool transposed, const void* from, int64_t ld, int64_t rows, int64_t cols, uint16_t* to, int64_t ldk, int64_t plane, bool live = false) {
         rowops::LayJob& j = jobs.job[jobs.n++];
-        j = {from, ld, rows, cols, to, ldk, plane, transposed, (int32_t)(transposed ? ceil_div64(rows, 64) * (ldk / 64) : ceil_div64(rows * ldk, 2048))};
+        j = {from, ld, rows, cols, to, ldk, plane, transposed, (int32_t)(transposed ? ceil_div64(rows, 64) * (ldk / 64) : ceil_div64(rows * ldk, 2048)), live};
     }
     void launch(bool f32, hipStream_t st) {
         int64_t blocks = 0;
@@ -489,10 +491,13 @@ rowops::Thin xent_thin_logits(const XentPlan& q) {
     p.bias = d->bias; p.target = d->target; p.target_row = d->target_row; p.target_kind = d->target_kind;
     return p;
 }
-void xent_tsum(const XentPlan& q, float* tsum, hipStream_t st) {
+// the rows with a gradient; of a profile their sums are made here (ws + tsum), and their dloss stands at ws + weight
+rowops::LiveRows xent_live(const XentPlan& q, char* ws, const float* dloss, hipStream_t st) {
     const dimn_output_loss* d = q.d;
     const unsigned threads = q.N < 1 << 20 ? 1024 : 256;        // (a launch has fewer than 2^32 of them; so many rows fill the device anyhow)
-    if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(threads), 0, st, d->target, d->target_kind, d->target_row, q.V, tsum);
+    float* weight = (float*)(ws + q.weight);
+    if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(threads), 0, st, d->target, d->target_kind, d->target_row, q.V, dloss, (float*)(ws + q.tsum), weight);
+    return {q.labels ? dloss : weight, d->target, d->target_kind, q.V};
 }
 rowops::SplitSum split_sum(const float* acc, int splits, int64_t rows, int64_t cols, void* out, int64_t ld) {
     const int32_t per = rows * cols >= 1 << 20 ? 4 : 1;          // (4096 x 2048 bfloat16, two splits: 32 us one by one, 21 by four)
@@ -511,11 +516,10 @@ void finish_bias(rowops::XentFinish& f, const XentPlan& q, char* ws, int parts, 
 template <typename T>
 void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
     const dimn_output_loss* d = q.d;
-    float* tsum = (float*)(ws + q.tsum);
     T* G = (T*)(ws + q.g);
-    xent_tsum(q, tsum, st);
+    const rowops::LiveRows live = xent_live(q, ws, dloss, st);
     rowops::Thin p = xent_thin_logits(q);
-    p.lse = lse; p.dloss = dloss; p.tsum = tsum;
+    p.lse = lse; p.dloss = live.dloss; p.tsum = (float*)(ws + q.tsum);
     p.G = G; p.ldg = q.V;
     p.dbias_part = dbias ? (q.blocks == 1 ? dbias : (float*)(ws + q.dbias)) : nullptr;
     xent_thin<T, rowops::XE_GRAD>(q, p, st);
@@ -533,6 +537,7 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     w.tiles = w.tiles_b * (int)ceil_div64(w.na, 64);
     w.ranges = q.dw_splits;
     w.acc = (float*)(ws + q.acc_w);
+    w.live = live;
     const bool vc = q.out_in;
     const int tiles = (int)ceil_div64(q.H, vc ? 64 : 32), dx_groups = (int)thin_groups(q, (int64_t)tiles * q.splits);
     const dim3 grid((unsigned)(dx_groups + w.tiles * w.ranges));
@@ -662,12 +667,12 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         HIPCHK(hipGetLastError());
         return DIMN_OK;
     }
-    float* tsum = (float*)(ws + q.tsum);
-    xent_tsum(q, tsum, st);
+    const rowops::LiveRows live = xent_live(q, ws, dloss, st);
     Lay lay;
+    lay.jobs.rows = live;
     uint16_t* xt = (uint16_t*)(ws + q.xt);
     const int64_t xt_plane = q.H * q.Np;
-    lay.add(true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane);
+    lay.add(true, d->x, d->x_row, q.H, q.N, xt, q.Np, xt_plane, true);
     const bool dk_out_in = dkernel_in == 1;
     for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
         const int64_t pv = std::min(q.P, q.V - c0), ldg = up(pv, 64);
@@ -680,7 +685,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
             else lay.add(false, at(d, d->kernel, c0), d->kernel_in, q.H, pv, wt, ldg, wt_plane);
         }
         lay.launch(q.f32, st);
-        p.lse = lse; p.dloss = dloss; p.tsum = tsum;
+        p.lse = lse; p.dloss = live.dloss; p.tsum = (float*)(ws + q.tsum);
         p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
         p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
         p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = q.V;

@@ -54,6 +54,19 @@ __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
     for (int pl = 0; pl < 3; ++pl) b[pl] = split_term(x, pl == 2);
 }
 
+// The rows of a batch that have a gradient: those whose label is a class (profiles: dloss is 0 where all weights are) and whose dloss is not 0.  The
+// G of the others is 0, but x may hold anything there, NaN too (padding), and 0 x NaN would reach dW: x^T G takes their x as zeros.
+enum { XT_I32 = 0, XT_I64 = 1, XT_F32 = 2, XT_BF16 = 3 };        // DIMN_TARGET_*
+struct LiveRows {
+    const float* dloss; const void* target; int32_t kind; int64_t classes;
+    __device__ __forceinline__ bool operator()(int64_t row) const {
+        int64_t y = 0;
+        if (kind == XT_I64) y = ((const int64_t*)target)[row];
+        else if (kind == XT_I32) y = ((const int32_t*)target)[row];
+        return dloss[row] != 0.f && y >= 0 && y < classes;
+    }
+};
+
 // ---- operand layout -----------------------------------------------------------------------------------------------------------
 // to[plane][r][k] = bfloat16 term `plane` of from[r][k], zero for cols <= k < ldk (ldk: a multiple of 64).  T = float: three planes, T = bf16_t: one.
 // Copying bounds both; everything moves in 16-byte pieces (64000 x 2048 bfloat16 transposed: 524 MB in 113 us, 4.7 TB/s).
@@ -78,12 +91,13 @@ __device__ __forceinline__ void lay_store(const T (&v)[8], uint16_t* to, int64_t
 }
 // One operand to lay out.  Not transposed: from is [r][k] with k contiguous, a thread takes eight k's.  Transposed: from is [k][r] with r contiguous
 // (row stride `ld` along k), 64 x 64 tiles through LDS, whose line of 65 (float) / 66 (bfloat16) elements spreads a column over the banks.
+// `live`: the k's are rows of the batch, and one without a gradient is laid out as zeros.
 struct LayJob {
     const void* from; int64_t ld, rows, cols;
     uint16_t* to; int64_t ldk, plane;
-    int32_t transposed, blocks;
+    int32_t transposed, blocks, live;
 };
-struct LayJobs { LayJob job[4]; int32_t n; };                    // (one launch for everything a piece needs: each is a few microseconds of copying)
+struct LayJobs { LayJob job[4]; int32_t n; LiveRows rows; };                    // (one launch for everything a piece needs: each is a few microseconds of copying)
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
     constexpr int LD = sizeof(T) == 4 ? 65 : 66;
@@ -117,6 +131,7 @@ __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
         const int64_t k = k0 + s + 32 * i, r = r0 + 8 * q;
         const T* f = from + k * p.ld + r;
         T v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        const bool live = k < p.cols && (!p.live || all.rows(k));
         if (k < p.cols) {
             if (r + 8 <= p.rows) {
                 const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)f;
@@ -127,7 +142,7 @@ __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
                 for (int j = 0; j < 8; ++j) if (r + j < p.rows) v[j] = f[j];
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) tile[s + 32 * i][8 * q + j] = v[j];
+        for (int j = 0; j < 8; ++j) tile[s + 32 * i][8 * q + j] = live ? v[j] : (T)0;
     }
     __syncthreads();
 #pragma unroll
@@ -168,7 +183,6 @@ struct XentGemm {
     float* acc; int64_t acc_split; int32_t acc_first;   // epilogue 3: acc[split][M][N] (+)= C
 };
 enum { XE_LSE = 0, XE_GRAD = 1, XE_STORE = 2, XE_ADD = 3 };
-enum { XT_I32 = 0, XT_I64 = 1, XT_F32 = 2, XT_BF16 = 3 };        // DIMN_TARGET_*
 
 __device__ __forceinline__ int64_t xent_label(const XentGemm& p, int64_t row) {
     return p.target_kind == XT_I64 ? ((const int64_t*)p.target)[row] : (int64_t)((const int32_t*)p.target)[row];
@@ -599,35 +613,41 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
     p.loss[row] = loss;
 }
 
-// tsum = the sum of every row of a profile; one workgroup per row (64 x 20000 float32: 4.7 us, latency)
-__global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t kind, int64_t target_row, int64_t classes, float* __restrict__ tsum) {
+// tsum = the sum of every row of a profile, weight = dloss, or 0 where all of the row is; one workgroup per row (64 x 20000 float32: 4.7 us, latency)
+__global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t kind, int64_t target_row, int64_t classes, const float* __restrict__ dloss,
+                                                    float* __restrict__ tsum, float* __restrict__ weight) {
     const int64_t row = blockIdx.x;
     __shared__ float red[16];
+    __shared__ int some[16];
     const int64_t step = 4 * (int64_t)blockDim.x;
     float s = 0.f;
+    bool any = false;
     if (kind == XT_F32) {
         const float* t = (const float*)target + row * target_row;
 #pragma unroll 4
         for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += step) {
-            if (c + 4 <= classes) { const f32x4u v = *(const f32x4u*)(t + c); s += (v[0] + v[1]) + (v[2] + v[3]); }
-            else for (int64_t k = c; k < classes; ++k) s += t[k];
+            if (c + 4 <= classes) { const f32x4u v = *(const f32x4u*)(t + c); s += (v[0] + v[1]) + (v[2] + v[3]); any |= v[0] != 0.f || v[1] != 0.f || v[2] != 0.f || v[3] != 0.f; }
+            else for (int64_t k = c; k < classes; ++k) { s += t[k]; any |= t[k] != 0.f; }
         }
     } else {
         const uint16_t* t = (const uint16_t*)target + row * target_row;
 #pragma unroll 4
         for (int64_t c = (int64_t)threadIdx.x * 4; c < classes; c += step) {
-            if (c + 4 <= classes) { const u16x4u v = *(const u16x4u*)(t + c); s += (from_bf16(v[0]) + from_bf16(v[1])) + (from_bf16(v[2]) + from_bf16(v[3])); }
-            else for (int64_t k = c; k < classes; ++k) s += from_bf16(t[k]);
+            if (c + 4 <= classes) { const u16x4u v = *(const u16x4u*)(t + c); s += (from_bf16(v[0]) + from_bf16(v[1])) + (from_bf16(v[2]) + from_bf16(v[3])); any |= ((v[0] | v[1] | v[2] | v[3]) & 0x7fff) != 0; }
+            else for (int64_t k = c; k < classes; ++k) { s += from_bf16(t[k]); any |= (t[k] & 0x7fff) != 0; }
         }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    const bool wave_any = __builtin_amdgcn_ballot_w64(any) != 0;
+    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6] = s; some[threadIdx.x >> 6] = wave_any; }
     __syncthreads();
     if (threadIdx.x == 0) {
         s = 0.f;
-        for (int w = 0; w < (int)blockDim.x / 64; ++w) s += red[w];
+        int live = 0;
+        for (int w = 0; w < (int)blockDim.x / 64; ++w) { s += red[w]; live |= some[w]; }
         tsum[row] = s;
+        weight[row] = live ? dloss[row] : 0.f;
     }
 }
 

@@ -470,6 +470,7 @@ struct ThinDw {
     void* C; int64_t ldc;
     int32_t tiles_b, tiles;                    // workgroups along b (256 columns each), in all
     int32_t ranges; float* acc;                // ranges > 1: range r of the rows leaves its float32 sums in acc[r][na][nb]
+    LiveRows live;
 };
 // Sixteen rows at a time, no more of them in flight: the registers of a second sixteen cost more workgroups than they hide latency (80 x 1344 x 28165
 // float32: 91 against 106 us; 12 rows 33 us = 4.6 TB/s), and a copy of the loads without the test for the last row changes nothing.
@@ -494,12 +495,18 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const vec zero = {0, 0, 0, 0};
     vec a[4], b[4];
     auto fetch = [&](int64_t k) {
+        const bool off = k + li < n && !p.live(k + li);             // sixteen rows, in each quarter of the wave
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t row = BF ? k + 4 * lj + r : k + 4 * r + lj;       // bfloat16: four consecutive rows make one lane's operand
             a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
             b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
         }
+        const uint32_t dead = (uint32_t)__builtin_amdgcn_ballot_w64(off) & 0xffff;
+        if (dead)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (dead >> (BF ? 4 * lj + r : 4 * r + lj) & 1) { a[r] = zero; b[r] = zero; }
     };
     auto consume = [&] {
         if constexpr (BF) {

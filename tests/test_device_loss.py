@@ -399,6 +399,44 @@ def test_masks_in_the_operands(dtype, order, rows, width, classes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,classes", [(9, 70, 90), (70, 64, 2001), (300, 70, 40), (4000, 128, 2001)])
+@pytest.mark.parametrize("target", ["labels", "labels64", "profile", "profile16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rows_without_a_gradient_hold_anything(dtype, target, rows, width, classes):
+    """Padding rows (no label, a label that is no class, a profile of zeros, dloss = 0) full of NaN and infinities: the gradients of the same call with
+    zeros there, bit by bit."""
+    from deepimpute_amd import ops
+    x, kernel, t, b, dloss = _problem(rows, width, classes, DTYPES[dtype], "in_out" if rows % 2 else "out_in", target)
+    dead = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    dead[1::3] = True
+    dead[-1] = True
+    if t.dim() == 1:
+        t[dead] = -1
+        t[4] = classes
+        dead = dead | (t < 0) | (t >= classes)
+    else:
+        t[dead] = 0
+        dead = dead | ~(t != 0).any(1)
+        t[6], t[6, 2], t[6, 5] = 0, 1, -1                            # a sum of 0 that is a target all the same
+        dead[6] = False
+    dloss[7] = 0
+    dead[7] = True
+    clean = torch.where(dead[:, None], torch.zeros_like(x), x)
+    dirty = clean.clone()
+    at = torch.nonzero(dead).squeeze(1)
+    dirty[at] = float("nan")
+    dirty[at[::2], ::2] = float("inf")
+    _, lse = ops.linear_cross_entropy(clean, kernel, t, b)
+    want = ops.linear_cross_entropy_grad(dloss, clean, kernel, t, lse, b)
+    loss, bad = ops.linear_cross_entropy(dirty, kernel, t, b)
+    assert torch.equal(bad[~dead], lse[~dead]) and not bool(loss[dead & (t < 0 if t.dim() == 1 else ~(t != 0).any(1))].any())
+    got = ops.linear_cross_entropy_grad(dloss, dirty, kernel, t, bad, b)
+    assert not bool(got[0][dead].any()) and all(bool(torch.isfinite(g).all()) for g in want)
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("target", ["labels", "profile"])
 def test_gradient_against_differences(target):
     """Central differences of sum(dloss * loss) of the float64 formula at the float32 point."""
