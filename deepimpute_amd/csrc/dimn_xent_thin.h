@@ -495,18 +495,17 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const vec zero = {0, 0, 0, 0};
     vec a[4], b[4];
     auto fetch = [&](int64_t k) {
-        const bool off = k + li < n && !p.live(k + li);             // sixteen rows, in each quarter of the wave
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t row = BF ? k + 4 * lj + r : k + 4 * r + lj;       // bfloat16: four consecutive rows make one lane's operand
             a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
             b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
         }
-        const uint32_t dead = (uint32_t)__builtin_amdgcn_ballot_w64(off) & 0xffff;
-        if (dead)
+    };
+    auto without = [&](uint32_t dead) {                             // bit i: the fetch's row i has no gradient
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (dead >> (BF ? 4 * lj + r : 4 * r + lj) & 1) { a[r] = zero; b[r] = zero; }
+        for (int r = 0; r < 4; ++r)
+            if (dead >> (BF ? 4 * lj + r : 4 * r + lj) & 1) { a[r] = zero; b[r] = zero; }
     };
     auto consume = [&] {
         if constexpr (BF) {
@@ -528,7 +527,19 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
                     for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][i], b[r][j], acc[i][j], 0, 0, 0);
         }
     };
-    for (int64_t k = beg; k < n; k += 16) { fetch(k); consume(); }
+    for (int64_t k0 = beg; k0 < n; k0 += 64) {
+        const bool off = k0 + lane < n && !p.live(k0 + lane);       // 64 rows at once, requested in front of the first sixteen
+        fetch(k0);
+        uint64_t dead = __builtin_amdgcn_ballot_w64(off);
+        for (int64_t k = k0;;) {
+            if ((uint32_t)dead & 0xffff) without((uint32_t)dead);
+            consume();
+            dead >>= 16;
+            k += 16;
+            if (k >= n || k == k0 + 64) break;
+            fetch(k);
+        }
+    }
     // acc[i][j][r]: a = set i of lane 4 lj + r, b = set j of lane li
     const bool whole = cb == b0 + 4 * li;
 #pragma unroll
