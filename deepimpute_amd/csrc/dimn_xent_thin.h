@@ -116,8 +116,9 @@ __device__ __forceinline__ void thin_product(const Thin& p, int tile, int range,
     // Four chunks at a time.  A lane that loaded its own 16 bytes of sixteen rows would have each lane looked up by itself (64 cache accesses per
     // load measured, one per cycle and CU: 128 x 2922 x 25664 float32 dx was bound by them, 335 us).  So the lanes of a quad read 64 consecutive
     // bytes of a row, in four loads those of four rows, and transpose the 4 x 4 among them: element [u] of a lane is then the 16 bytes at
-    // k + EL (4 lj + u) of its own row.  Offsets from the workgroup's first row take 32 bits (rows further apart go chunk by chunk below).
-    const int64_t nc = FOURS > 0 && p.lda < (1 << 24) && p.ldb < (1 << 24) ? cend - cbeg : 0;
+    // k + EL (4 lj + u) of its own row.  Offsets from the workgroup's first row take 32 bits (rows further apart, and rows
+    // in descending order, whose offsets are negative, go chunk by chunk below).
+    const int64_t nc = FOURS > 0 && p.lda >= 0 && p.ldb >= 0 && p.lda < (1 << 24) && p.ldb < (1 << 24) ? cend - cbeg : 0;
     const int64_t full = nc / (4 * NW), left = nc % (4 * NW);
     const int quads = left > 2 * NW ? (int)left / 4 : 0;         // waves that take four more chunks: what is left over would cost as many single ones
     const int64_t rounds = full + (wave < quads);

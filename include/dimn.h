@@ -404,7 +404,7 @@ int dimn_col_stats_var(const double* a, int64_t n, int64_t g, int64_t ld, const 
  * Every array is device memory of `device_id`; `stream` is a hipStream_t of that device (NULL: its default stream).  A call queues its
  * kernels on the stream and returns; nothing is allocated, copied to the host or waited for, so it can be captured into a graph, and two
  * calls on different streams run side by side as long as their workspaces and outputs differ.  The calling thread's current device is
- * left as it was.  Strides count elements; the last axis of every plane is contiguous and nothing else is assumed about alignment
+ * left as it was.  Strides count elements and may be 0 or negative; the last axis of every plane is contiguous and nothing else is assumed about alignment
  * (workspaces: 16 bytes).  Rows past `rows` are neither read nor written.  The same arguments give the same bits. */
 #define DIMN_TYPE_F32 0
 #define DIMN_TYPE_BF16 1

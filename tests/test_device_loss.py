@@ -197,6 +197,41 @@ def test_rows_far_apart():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,width,classes", [("f32", 20, 1500, 3001), ("f32", 300, 200, 500), ("f32", 20, 700, 20011), ("bf16", 20, 2304, 3001), ("bf16", 300, 256, 512)])
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+def test_rows_in_descending_order(dtype, rows, width, classes, order):
+    """Negative strides, which tensors cannot have, through the C entries: x, the kernel and its gradient walked from their last row, few rows and many:
+    the bits of the same rows in ascending order up to the order of a sum (which test_sizes bounds)."""
+    from deepimpute_amd import ops
+    fns = _lib.load()
+    x, kernel, t, b, dloss = _problem(rows, width, classes, DTYPES[dtype], order)
+    k = kernel if order == "in_out" else kernel.t()                  # rows in memory
+    size = x.element_size()
+    ref = _reference(x, kernel, t, b, dloss)
+    xd, kd = x.flip(0).contiguous(), k.flip(0).contiguous()
+    ld = kd.shape[1]
+    strides = (-ld, 1) if order == "in_out" else (1, -ld)
+    last = lambda a: a.data_ptr() + (a.shape[0] - 1) * a.shape[1] * size  # noqa: E731
+    stream = torch.cuda.current_stream().cuda_stream
+    d = _cabi.OutputLoss(0, 0 if dtype == "f32" else 1, rows, width, classes, last(xd), -width, last(kd), strides[0], strides[1], b.data_ptr(), t.data_ptr(), 0, 0)
+    out = torch.empty((2, rows), device="cuda")
+
+    def space(grad):
+        n = C.c_int64()
+        assert fns["linear_cross_entropy_workspace"](d, grad, n) == 0
+        return torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    work = space(0)
+    assert fns["linear_cross_entropy"](d, stream, out[0].data_ptr(), out[1].data_ptr(), work.data_ptr(), work.numel()) == 0, fns["last_error"]()
+    _close("loss", out[0], *ref["loss"])
+    _close("lse", out[1], *ref["lse"])
+    work, dx, dk, db = space(1), torch.empty_like(xd), torch.empty_like(kd), torch.empty(classes, device="cuda")
+    assert fns["linear_cross_entropy_grad"](d, stream, dloss.data_ptr(), out[1].data_ptr(), last(dx), -width, last(dk), strides[0], strides[1], db.data_ptr(), work.data_ptr(), work.numel()) == 0, fns["last_error"]()
+    dk = dk.flip(0)
+    for name, got in (("dx", dx.flip(0)), ("dkernel", dk if order == "in_out" else dk.t()), ("dbias", db)):
+        _close(name, got, *ref[name])
+
+
+@pytest.mark.gpu
 def test_broadcast_inputs():
     """Axes of stride 0: the same row for every sample, one profile for all of them, a kernel of equal rows or columns."""
     from deepimpute_amd import ops
