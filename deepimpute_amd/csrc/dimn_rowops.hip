@@ -247,6 +247,10 @@ int pick_tile(bool f32, int64_t M, int64_t N, int ncu) {
     return cost(t[2]) < cost(t[best]) ? 2 : best;
 }
 
+// A piece's operands (and the G of the form for few rows) take up to 1 GiB: 4096 x 2048 x 64000 / x 100000 bfloat16 backward 3.02 / 4.66 ms (512 MiB:
+// 3.09 / 4.88, 192 MiB: 3.17 / 5.02, 4 GiB: 2.93 / 4.78 -- but that keeps as much as the logits).
+constexpr int64_t kBudget = (int64_t)1 << 30;
+
 // what a call needs: operand forms, pieces of the classes, and where everything lies in the workspace
 struct XentPlan {
     const dimn_output_loss* d;
@@ -258,7 +262,7 @@ struct XentPlan {
     int64_t tiles_m, tiles_n;                 // logits
     int t_dx, splits, t_dw, dw_splits;
     bool thin; int nf; int64_t blocks;        // few rows: dimn_xent_thin.h; 16 nf rows per block
-    size_t x, xt, w, wt, g, gt, part, part_t, picked, tsum, weight, dbias, acc, acc_w, bytes;
+    size_t x, xt, w, wt, g, gt, part, part_t, picked, carry, tsum, weight, dbias, acc, acc_w, bytes;
 
     // The largest piece allowed, or a smaller one whose 256 x 256 tiles fill the device in whole rounds: a piece of 84 class tiles at 16 row tiles
     // takes 6 rounds of 256 workgroups where 96 class tiles take the same six (64000 classes: 16 rounds instead of 18, 8 instead of 9 for dW).
@@ -320,19 +324,19 @@ struct XentPlan {
         x_direct = !f32 && H % 64 == 0 && aligned(d->x) && d->x_row % 8 == 0 && d->x_row <= far && d->x_row >= 0;
         w_direct = !f32 && out_in && H % 64 == 0 && aligned(d->kernel) && d->kernel_out % 8 == 0 && d->kernel_out <= far && d->kernel_out >= 0;
         wt_direct = !f32 && !out_in && V % 64 == 0 && aligned(d->kernel) && d->kernel_in % 8 == 0 && d->kernel_in <= far && d->kernel_in >= 0;
-        const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0));
-        // A piece's operands take up to 1 GiB: 4096 x 2048 x 64000 / x 100000 bfloat16 backward 3.02 / 4.66 ms (512 MiB: 3.09 / 4.88, 192 MiB: 3.17 / 5.02,
-        // 4 GiB: 2.93 / 4.78 -- but that keeps as much as the logits).
-        const int64_t budget = (int64_t)1 << 30;
-        P = per_class ? std::max<int64_t>(256, budget / per_class / 256 * 256) : up(V, 256);
+        // bytes of the workspace that a class of a piece takes: its operands, and what its tiles leave per row (forward: 8 or 16 bytes for 128 classes or
+        // more) or per 64 rows (backward: a sum for dbias)
+        const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0)) + (grad ? Np / 16 : Np / (labels ? 16 : 8));
+        P = std::max<int64_t>(256, kBudget / std::max<int64_t>(1, per_class) / 256 * 256);
         P = std::min({P, far, up(V, 256), std::max<int64_t>(256, ((int64_t)1 << 22) / std::max<int64_t>(1, ceil_div64(N, 256)) * 256)});      // (the last: a launch has fewer than 2^32 threads)
         if (P < V && (grad || !w_direct)) P = best_piece(P);
         t_logits = pick_tile(f32, N, std::min(P, V), ncu);
         tiles_m = ceil_div64(N, kTiles[f32][t_logits].bm);
-        tiles_n = ceil_div64(V, kTiles[f32][t_logits].bn);
+        tiles_n = ceil_div64(std::min(P, V), kTiles[f32][t_logits].bn);
         bytes = 0;
-        // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.
-        thin = V >= 4 && H >= 4 && prefers_thin();
+        // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.  Its backward pass keeps G of
+        // all classes: no more of it than a piece takes (a narrow float32 layer would use this form with any number of rows, 65536 x 32 x 100000: 24 GiB).
+        thin = V >= 4 && H >= 4 && (!grad || (f32 ? 4 : 2) * N * V <= std::max(kBudget, P * per_class)) && prefers_thin();
         if (thin) {
             // 64 rows per block read the kernel least often, 32 give twice the workgroups.  float32, bound by the matrix instructions: up to 32, half the
             // registers (64 / 80 x 1344 x 28165 logits 82 / 120 us, with 64 rows 94 / 143), 16 where a third of two blocks of 32 would be no rows (48: 75, 81 us)
@@ -351,7 +355,7 @@ struct XentPlan {
             dbias = take(4 * blocks * V);
             const int64_t wgs = ceil_div64(H, out_in ? 64 : 32) * blocks, chunks = V / 64;
             splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)64, ceil_div64(4 * ncu, wgs), chunks / 2}));
-            acc = take(4 * (int64_t)splits * N * H);
+            acc = splits > 1 ? take(4 * (int64_t)splits * N * H) : 0;
             const int64_t wt_wgs = ceil_div64(H, 64) * ceil_div64(V, 256);        // (dW: 64 x 256 of the product per workgroup, either way round)
             dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)32, 2 * ncu / wt_wgs, N / 128}));
             acc_w = dw_splits > 1 ? take(4 * (int64_t)dw_splits * H * V) : 0;
@@ -363,6 +367,7 @@ struct XentPlan {
             part = take(8 * tiles_n * N);
             part_t = labels ? 0 : take(8 * tiles_n * N);
             picked = take(4 * N);
+            carry = P < V ? take(16 * N) : 0;
             return;
         }
         xt = take(2 * planes * H * Np);
@@ -371,7 +376,7 @@ struct XentPlan {
         gt = take(2 * planes * P * Np);
         tsum = take(4 * N);
         weight = labels ? 0 : take(4 * N);
-        dbias = take(4 * tiles_m * kTiles[f32][t_logits].wm * V);
+        dbias = take(4 * tiles_m * kTiles[f32][t_logits].wm * std::min(P, V));
         // dx has few tiles and a long inner dimension, so has dW of a narrow layer: ranges of it, each with float32 sums of its own
         const int64_t pv = std::min(P, V);
         auto tile_for = [&](int64_t M, int64_t N_, int64_t steps) {        // (the large tile if a few ranges of k fill the device with it)
@@ -509,9 +514,9 @@ void xent_finish(bool f32, const rowops::XentFinish& f, hipStream_t st) {
     if (f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, f);
     else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, f);
 }
-// the bias gradient from `parts` partial sums in the workspace
-void finish_bias(rowops::XentFinish& f, const XentPlan& q, char* ws, int parts, float* dbias) {
-    f.part = (const float*)(ws + q.dbias); f.part_ld = q.V; f.parts = parts; f.classes = q.V; f.dbias = dbias;
+// the bias gradient of `classes` classes from `parts` rows of partial sums in the workspace
+void finish_bias(rowops::XentFinish& f, const XentPlan& q, char* ws, int64_t classes, int parts, float* dbias) {
+    f.part = (const float*)(ws + q.dbias); f.part_ld = classes; f.parts = parts; f.classes = classes; f.dbias = dbias;
 }
 template <typename T>
 void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const float* lse, void* dx, int64_t dx_row, void* dkernel, int64_t dk_in, int64_t dk_out, float* dbias, hipStream_t st) {
@@ -566,7 +571,7 @@ void xent_thin_backward(const XentPlan& q, char* ws, const float* dloss, const f
     rowops::XentFinish f{};
     if (q.splits > 1) f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
     if (w.ranges > 1) f.m[1] = split_sum(w.acc, w.ranges, w.na, w.nb, w.C, w.ldc);
-    if (q.blocks > 1) finish_bias(f, q, ws, (int)q.blocks, dbias);
+    if (q.blocks > 1) finish_bias(f, q, ws, q.V, (int)q.blocks, dbias);
     xent_finish(q.f32, f, st);
 }
 
@@ -615,7 +620,20 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
     q.make(d, false, compute_units(d->device_id));
     CHK(xent_space(who, q, workspace, workspace_bytes));
     char* ws = (char*)workspace;
-    const Tile& t = kTiles[q.f32][q.t_logits];
+    rowops::XentRows r{};
+    r.part = (const float2*)(ws + q.part);
+    r.part_t = q.labels ? nullptr : (const float2*)(ws + q.part_t);
+    r.picked = (const float*)(ws + q.picked);
+    r.rows = q.N; r.classes = q.V;
+    r.target = d->target; r.target_kind = d->target_kind;
+    r.carry = (float4*)(ws + q.carry);
+    r.loss = loss; r.lse = lse;
+    auto join = [&](int64_t tiles, bool first, bool last) {
+        r.tiles = tiles; r.first = first; r.last = last;
+        r.per = 1;                                               // rows per workgroup: fewer, with more strands over the tiles each, while a strand has more than two
+        while (r.per < 64 && 2 * r.per <= q.N && (r.per < 4 || 1024 / (2 * r.per) * 2 >= tiles)) r.per *= 2;
+        hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, r.per)), dim3(1024), 0, st, r);
+    };
     if (q.thin) {
         rowops::Thin p = xent_thin_logits(q);
         p.part = (float2*)(ws + q.part);
@@ -623,26 +641,19 @@ extern "C" int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream
         p.picked = (float*)(ws + q.picked);
         if (q.f32) xent_thin<float, rowops::XE_LSE>(q, p, st);
         else xent_thin<bf16_t, rowops::XE_LSE>(q, p, st);
+        join(q.tiles_n, true, true);
     } else for (int64_t c0 = 0; c0 < q.V; c0 += q.P) {
+        const int64_t pv = std::min(q.P, q.V - c0);
         XentGemm p;
         Lay lay;
-        xent_logits(q, ws, c0, std::min(q.P, q.V - c0), p, lay);
+        xent_logits(q, ws, c0, pv, p, lay);
         lay.launch(q.f32, st);
-        p.part = (float2*)(ws + q.part) + c0 / t.bn * q.N;
-        if (!q.labels) p.part_t = (float2*)(ws + q.part_t) + c0 / t.bn * q.N;
+        p.part = (float2*)(ws + q.part);
+        if (!q.labels) p.part_t = (float2*)(ws + q.part_t);
         p.picked = (float*)(ws + q.picked);
         xent_gemm<rowops::XE_LSE>(q.f32, q.t_logits, 1, p, st);
+        join(ceil_div64(pv, kTiles[q.f32][q.t_logits].bn), c0 == 0, c0 + pv == q.V);
     }
-    rowops::XentRows r{};
-    r.part = (const float2*)(ws + q.part);
-    r.part_t = q.labels ? nullptr : (const float2*)(ws + q.part_t);
-    r.picked = (const float*)(ws + q.picked);
-    r.tiles = q.tiles_n; r.rows = q.N; r.classes = q.V;
-    r.target = d->target; r.target_kind = d->target_kind;
-    r.loss = loss; r.lse = lse;
-    r.per = 1;                                                   // rows per workgroup: fewer, with more strands over the tiles each, while a strand has more than two
-    while (r.per < 64 && 2 * r.per <= q.N && (r.per < 4 || 1024 / (2 * r.per) * 2 >= q.tiles_n)) r.per *= 2;
-    hipLaunchKernelGGL(rowops::k_xent_lse, dim3((unsigned)ceil_div64(q.N, r.per)), dim3(1024), 0, st, r);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
 }
@@ -688,7 +699,7 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
         p.lse = lse; p.dloss = live.dloss; p.tsum = (float*)(ws + q.tsum);
         p.G = (uint16_t*)(ws + q.g); p.ldg = ldg; p.g_plane = q.N * ldg;
         p.GT = (uint16_t*)(ws + q.gt); p.ldgt = q.Np; p.gt_plane = pv * q.Np;
-        p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = q.V;
+        p.dbias_part = (float*)(ws + q.dbias); p.dbias_ld = pv;
         xent_gemm<rowops::XE_GRAD>(q.f32, q.t_logits, 1, p, st);
         // dx += G W^T
         XentGemm a{};
@@ -712,18 +723,16 @@ extern "C" int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* s
             w.B = gt; w.ldb = q.Np; w.b_plane = p.gt_plane; w.N = (int)pv;
             w.C = const_cast<void*>(at(d, dkernel, c0)); w.ldc = dkernel_in;
         }
+        rowops::XentFinish f{};
         if (q.dw_splits > 1) {
             w.acc = (float*)(ws + q.acc_w); w.acc_split = (int64_t)w.M * w.N; w.acc_first = 1;
             xent_gemm<rowops::XE_ADD>(q.f32, q.t_dw, q.dw_splits, w, st);
-            rowops::XentFinish f{};
             f.m[0] = split_sum(w.acc, q.dw_splits, w.M, w.N, w.C, w.ldc);
-            xent_finish(q.f32, f, st);
         } else xent_gemm<rowops::XE_STORE>(q.f32, q.t_dw, 1, w, st);
+        if (c0 + pv == q.V) f.m[1] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
+        if (dbias) finish_bias(f, q, ws, pv, (int)(q.tiles_m * kTiles[q.f32][q.t_logits].wm), dbias + c0);
+        xent_finish(q.f32, f, st);
     }
-    rowops::XentFinish f{};
-    f.m[0] = split_sum((const float*)(ws + q.acc), q.splits, q.N, q.H, dx, dx_row);
-    finish_bias(f, q, ws, (int)(q.tiles_m * kTiles[q.f32][q.t_logits].wm), dbias);
-    xent_finish(q.f32, f, st);
     HIPCHK(hipGetLastError());
     return DIMN_OK;
 }

@@ -177,7 +177,7 @@ struct XentGemm {
     const float* tsum;                         // profile: [M]
     uint16_t* G; int64_t ldg, g_plane;         // [plane][M][ldg], columns N .. ldg zero
     uint16_t* GT; int64_t ldgt, gt_plane;      // [plane][N][ldgt], columns M .. ldgt zero
-    float* dbias_part; int64_t dbias_ld;       // [2 tiles_m][dbias_ld]: column sums of G over the rows of one wave row
+    float* dbias_part; int64_t dbias_ld;       // [WM tiles_m][dbias_ld]: column sums of G over the rows of one wave row (WM of them per tile)
     // result
     void* C; int64_t ldc;                      // epilogue 2: C[m][n], float32 (three planes) or bfloat16 (one)
     float* acc; int64_t acc_split; int32_t acc_first;   // epilogue 3: acc[split][M][N] (+)= C
@@ -516,7 +516,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                     for (int i = 0; i < FM; ++i) s += acc[i][j][r];
 #pragma unroll
                     for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-                    if (li == 0 && nb + 4 * j + r < p.N) p.dbias_part[(int64_t)(tm * WM + wm) * p.dbias_ld + p.class0 + nb + 4 * j + r] = s;
+                    if (li == 0 && nb + 4 * j + r < p.N) p.dbias_part[(int64_t)(tm * WM + wm) * p.dbias_ld + nb + 4 * j + r] = s;
                 }
             typedef uint16_t rowvec __attribute__((ext_vector_type(4 * FN)));
             typedef uint16_t colvec __attribute__((ext_vector_type(FM)));
@@ -568,7 +568,9 @@ __device__ __forceinline__ float2 join_lse(float2 a, float2 b) {
 }
 
 // loss and lse of every row from the partial sums of the class tiles (4096 rows of 391 tiles: 15 us; one row of 1000: 4.4 us): 1024 threads, `per` rows (a power of two up to 64) x 1024 / per strands of tiles
+// One call per piece of the classes: what the pieces so far come to waits in `carry`, the last one gives the results.
 struct XentRows {
+    float4* carry; int32_t first, last;        // [rows] (maximum, sum, sum of t, sum of t z)
     const float2* part; const float2* part_t; const float* picked;
     int64_t tiles, rows, classes;
     int32_t per;
@@ -577,10 +579,11 @@ struct XentRows {
 };
 __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
     __shared__ float2 red[1024], red_t[1024];
-    const int c = threadIdx.x & (p.per - 1), strands = 1024 / p.per, strand = threadIdx.x / p.per;
-    const int64_t row = (int64_t)blockIdx.x * p.per + c;
+    const int in = threadIdx.x & (p.per - 1), strands = 1024 / p.per, strand = threadIdx.x / p.per;
+    const int64_t row = (int64_t)blockIdx.x * p.per + in;
     float2 v = make_float2(-INFINITY, 0.f), t = make_float2(0.f, 0.f);
     if (row < p.rows) {
+        if (!p.first && strand == 0) { const float4 c = p.carry[row]; v = make_float2(c.x, c.y); t = make_float2(c.z, c.w); }
 #pragma unroll 4
         for (int64_t k = strand; k < p.tiles; k += strands) v = join_lse(v, p.part[k * p.rows + row]);
         if (p.part_t) {
@@ -601,6 +604,7 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
         }
     }
     if (strand != 0 || row >= p.rows) return;
+    if (!p.last) { p.carry[row] = make_float4(v.x, v.y, t.x, t.y); return; }
     const float lse = v.x == -INFINITY ? (v.y == 0.f ? -INFINITY : v.y) : v.x + __logf(v.y);
     p.lse[row] = lse;
     float loss;
@@ -651,7 +655,7 @@ __global__ __launch_bounds__(1024) void k_xent_tsum(const void* target, int32_t 
     }
 }
 
-// What is left of a backward pass, in one launch: out[m][n] = the sum of the splits' float32 sums for up to two matrices (dx, dW), dbias = the sum of
+// What is left of a backward pass (of a piece of its classes), in one launch: out[m][n] = the sum of the splits' float32 sums for up to two matrices (dx, dW), dbias = the sum of
 // the partial column sums, each added in order and rounded once.  A thread takes one element of a small matrix, four consecutive ones of a large one.
 struct SplitSum {
     const float* acc; int64_t split; int32_t splits, blocks;     // [splits][rows][cols], `split` elements apart; blocks = 0: nothing to do

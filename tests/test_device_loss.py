@@ -267,6 +267,30 @@ def test_most_rows(dtype, width, classes):
 
 
 @pytest.mark.gpu
+def test_workspaces_are_far_smaller_than_the_logits():
+    """Many rows and classes, narrow layers among them: one piece of the classes at a time, whatever form a call takes (the query only)."""
+    fns = _lib.load()
+
+    def space(grad, kind, rows, width, classes, order, target_kind):
+        n = C.c_int64()
+        k_in, k_out = (1, width) if order == "out_in" else (classes, 1)
+        d = _describe(type=kind, rows=rows, width=width, classes=classes, x_row=width, kernel_in=k_in, kernel_out=k_out, target_kind=target_kind, target_row=classes)
+        assert fns["linear_cross_entropy_workspace"](d, grad, n) == 0, fns["last_error"]()
+        return n.value
+    for kind in (0, 1):
+        for order in ("out_in", "in_out"):
+            for target_kind in (0, 2):
+                for rows, width, classes in ((65536, 32, 100000), (65536, 72, 100000), (1 << 20, 32, 1 << 15), (1 << 20, 64, 262144), (1 << 22, 64, 65536), (1 << 22, 16, 30000)):
+                    for grad in (0, 1):
+                        operands = 12 * rows * ((width + 63) // 64 * 64) * 2 + 4 * rows * width
+                        # a piece of 256 classes at least: G in two orders and three terms, 12 bytes for each of its elements
+                        piece = max(1 << 30, 256 * 12 * rows if grad else 0)
+                        got = space(grad, kind, rows, width, classes, order, target_kind)
+                        assert got <= 1.1 * (piece + operands) + (64 << 20), (kind, order, target_kind, rows, width, classes, grad, got)
+                        assert got < rows * classes * (4 if kind == 0 else 2)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [50, 150])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides(dtype, rows):
