@@ -328,7 +328,7 @@ struct XentPlan {
         // more) or per 64 rows (backward: a sum for dbias)
         const int64_t per_class = 2 * planes * ((w_direct ? 0 : Hp) + (grad ? (wt_direct ? 0 : H) + N + Np : 0)) + (grad ? Np / 16 : Np / (labels ? 16 : 8));
         P = std::max<int64_t>(256, kBudget / std::max<int64_t>(1, per_class) / 256 * 256);
-        P = std::min({P, far, up(V, 256), std::max<int64_t>(256, ((int64_t)1 << 22) / std::max<int64_t>(1, ceil_div64(N, 256)) * 256)});      // (the last: a launch has fewer than 2^32 threads)
+        P = std::min({P, far, up(V, 256), std::max<int64_t>(256, ((int64_t)1 << 20) / std::max<int64_t>(1, ceil_div64(N, 256)) * 256)});      // (the last: a launch has fewer than 2^32 threads, whatever its tiles)
         if (P < V && (grad || !w_direct)) P = best_piece(P);
         t_logits = pick_tile(f32, N, std::min(P, V), ncu);
         tiles_m = ceil_div64(N, kTiles[f32][t_logits].bm);
@@ -411,6 +411,13 @@ void xent_gemm(bool f32, int tile, int splits, XentGemm& p, hipStream_t st) {
     }
 }
 
+// `blocks` workgroups of 256 threads, in as many launches as keep each below 2^32 threads
+template <typename F>
+void in_launches(int64_t blocks, F&& launch) {
+    constexpr int64_t most = 1 << 23;
+    for (int64_t b = 0; b < blocks; b += most) launch(b, (unsigned)std::min(most, blocks - b));
+}
+
 // Operands to lay out, gathered and launched together
 struct Lay {
     rowops::LayJobs jobs{};
@@ -421,9 +428,11 @@ struct Lay {
     void launch(bool f32, hipStream_t st) {
         int64_t blocks = 0;
         for (int i = 0; i < jobs.n; ++i) blocks += jobs.job[i].blocks;
-        if (blocks == 0) return;
-        if (f32) hipLaunchKernelGGL(rowops::k_xent_lay<float>, dim3((unsigned)blocks), dim3(256), 0, st, jobs);
-        else hipLaunchKernelGGL(rowops::k_xent_lay<bf16_t>, dim3((unsigned)blocks), dim3(256), 0, st, jobs);
+        in_launches(blocks, [&](int64_t first, unsigned count) {
+            jobs.first = (int32_t)first;
+            if (f32) hipLaunchKernelGGL(rowops::k_xent_lay<float>, dim3(count), dim3(256), 0, st, jobs);
+            else hipLaunchKernelGGL(rowops::k_xent_lay<bf16_t>, dim3(count), dim3(256), 0, st, jobs);
+        });
         jobs.n = 0;
     }
 };
@@ -508,11 +517,12 @@ rowops::SplitSum split_sum(const float* acc, int splits, int64_t rows, int64_t c
     const int32_t per = rows * cols >= 1 << 20 ? 4 : 1;          // (4096 x 2048 bfloat16, two splits: 32 us one by one, 21 by four)
     return {acc, rows * cols, splits, (int32_t)ceil_div64(rows * cols, 256 * per), per, rows, cols, out, ld};
 }
-void xent_finish(bool f32, const rowops::XentFinish& f, hipStream_t st) {
-    const unsigned blocks = (unsigned)(f.m[0].blocks + f.m[1].blocks + (f.dbias && f.parts ? ceil_div64(f.classes, 256) : 0));
-    if (blocks == 0) return;
-    if (f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(blocks), dim3(256), 0, st, f);
-    else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(blocks), dim3(256), 0, st, f);
+void xent_finish(bool f32, rowops::XentFinish& f, hipStream_t st) {
+    in_launches((int64_t)f.m[0].blocks + f.m[1].blocks + (f.dbias && f.parts ? ceil_div64(f.classes, 256) : 0), [&](int64_t first, unsigned count) {
+        f.first = (int32_t)first;
+        if (f32) hipLaunchKernelGGL(rowops::k_xent_finish<float>, dim3(count), dim3(256), 0, st, f);
+        else hipLaunchKernelGGL(rowops::k_xent_finish<bf16_t>, dim3(count), dim3(256), 0, st, f);
+    });
 }
 // the bias gradient of `classes` classes from `parts` rows of partial sums in the workspace
 void finish_bias(rowops::XentFinish& f, const XentPlan& q, char* ws, int64_t classes, int parts, float* dbias) {

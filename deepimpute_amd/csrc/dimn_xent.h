@@ -97,12 +97,12 @@ struct LayJob {
     uint16_t* to; int64_t ldk, plane;
     int32_t transposed, blocks, live;
 };
-struct LayJobs { LayJob job[4]; int32_t n; LiveRows rows; };                    // (one launch for everything a piece needs: each is a few microseconds of copying)
+struct LayJobs { LayJob job[4]; int32_t n, first; LiveRows rows; };                    // (one launch for everything a piece needs: each is a few microseconds of copying)
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
     constexpr int LD = sizeof(T) == 4 ? 65 : 66;
     __shared__ T tile[64][LD];
-    int block = blockIdx.x, w = 0;
+    int block = blockIdx.x + all.first, w = 0;
     while (w + 1 < all.n && block >= all.job[w].blocks) { block -= all.job[w].blocks; ++w; }
     const LayJob& p = all.job[w];
     const T* from = (const T*)p.from;
@@ -665,13 +665,14 @@ struct SplitSum {
 };
 struct XentFinish {
     SplitSum m[2];
+    int32_t first;                                               // number of the launch's first workgroup
     const float* part; int64_t part_ld; int32_t parts;
     int64_t classes;
     float* dbias;
 };
 template <typename T>
 __global__ __launch_bounds__(256) void k_xent_finish(const XentFinish p) {
-    int block = blockIdx.x;
+    int block = blockIdx.x + p.first;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         if (block < p.m[w].blocks) {

@@ -291,6 +291,44 @@ def test_workspaces_are_far_smaller_than_the_logits():
 
 
 @pytest.mark.gpu
+def test_most_threads():
+    """Calls whose products, layouts and last sums have 2^32 threads or more in all, which one launch cannot hold: 2^22 rows x 65536 classes forward
+    (float32), 2^22 rows of 4096 inputs backward (all rows of x the same row: what is expected is a product of vectors)."""
+    from deepimpute_amd import ops
+    rows = 1 << 22
+    x, kernel, t, b, dloss = _problem(rows, 64, 65536, torch.float32, "in_out")
+    loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        ref = _reference(x[part], kernel, t[part], b)
+        _close("lse", lse[part], *ref["lse"])
+        _close("loss", loss[part], *ref["loss"])
+    del x, kernel, t, b, dloss, loss, lse
+    torch.cuda.empty_cache()
+    width, classes = 4096, 200
+    one, kernel, _, b, _ = _problem(1, width, classes, torch.bfloat16, "in_out")
+    t = torch.arange(rows, device="cuda", dtype=torch.int32) % classes
+    dloss = (0.5 + (torch.arange(rows, device="cuda") % 7) / 8).float() / rows
+    x = one.expand(rows, width)
+    _, lse1 = ops.linear_cross_entropy(one, kernel, t[:1], b)
+    dx, dk, db = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse1.expand(rows).contiguous(), b)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        ref = _reference(x[part], kernel, t[part], b, dloss[part])
+        _close("dx", dx[part], *ref["dx"])
+    del dx
+    ref = _reference(one, kernel, t[:1], b, torch.ones(1, device="cuda"))
+    p = torch.exp((one.double() @ kernel.double() + b.double() - lse1.double()[:, None]))[0]
+    at = torch.zeros(classes, dtype=torch.float64, device="cuda").index_add_(0, t.long(), dloss.double())
+    G = dloss.double().sum() * p - at                                # per class, over all rows
+    size = dloss.double().sum() * p + at                             # of its terms
+    room = (_products(width) * 64 * 10 + _half(torch.bfloat16)) * size + 2 * U * (rows / 2 + 32) * size
+    _close("dbias", db, G, room)
+    X = one.double()[0]
+    _close("dkernel", dk, X[:, None] * G[None], X.abs()[:, None] * (room + _products(rows) * size)[None] + _half(torch.bfloat16) * (X[:, None] * G[None]).abs())
+    del x, dk, db
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [50, 150])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_strides(dtype, rows):
