@@ -613,7 +613,8 @@ __global__ __launch_bounds__(1024) void k_xent_lse(const XentRows p) {
         if (y < 0) loss = 0.f;
         else if (y >= p.classes) loss = NAN;
         else { const float z = p.picked[row]; loss = z == -INFINITY ? INFINITY : lse - z; }
-    } else loss = t.x == 0.f && t.y == 0.f ? 0.f : t.x * lse - t.y;
+    } else if (t.x == 0.f && t.y == 0.f) loss = 0.f;
+    else loss = fabsf(t.y) == INFINITY && !isnan(lse) ? -t.y : t.x * lse - t.y;      // (weight on a class that is not there, also where none is: lse = -inf)
     p.loss[row] = loss;
 }
 

@@ -431,7 +431,7 @@ int dimn_layer_norm_grad(int32_t device_id, void* stream, int32_t type, int64_t 
  *   labels:   loss = lse - z[label].  A negative label is a row without a target: loss 0, no gradient.  A label >= classes: loss NaN, no
  *             gradient.  A label whose logit is -infinity (masked by the bias): loss +infinity.
  *   profiles: loss = sum(t) lse - sum(t z) for a row t of weights over the classes (counts, probabilities); t = 0 takes no part, a row of zeros
- *             is a row without a target.
+ *             is a row without a target.  Weight on a class whose logit is -infinity: loss +infinity, as for labels.
  * Rows without a gradient (those, and rows whose dloss is 0) may hold anything in x, NaN too: none of it reaches dkernel or dbias, their dx is 0.
  * A class with z = -infinity has probability 0, also in a row that has no other class left; masks may stand in the bias or, as an infinity or
  * the lowest value of the type, in the kernel or in x.  (Backward, the products are the plain ones: 0 x infinity in dx is NaN, so a kernel that

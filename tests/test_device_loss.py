@@ -422,6 +422,26 @@ def test_masks_and_odd_labels(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,width,classes", [(9, 64, 40), (4000, 128, 2001)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_profiles_of_masked_classes(dtype, rows, width, classes):
+    """Weight on classes that a bias of -infinity masks: the loss of a label there, +infinity, also where no class is left at all; finite gradients."""
+    from deepimpute_amd import ops
+    inf = float("inf")
+    x, kernel, t, _, dloss = _problem(rows, width, classes, DTYPES[dtype], target="profile")
+    t[:: 4] = 0
+    weighted = (t != 0).any(1)
+    some = torch.zeros(classes, device="cuda")
+    some[1::2] = -inf
+    for b in (some, torch.full_like(some, -inf)):
+        hit = ((t != 0) & torch.isinf(b)).any(1)
+        loss, lse = ops.linear_cross_entropy(x, kernel, t, b)
+        assert bool((loss[hit] == inf).all()) and bool(torch.isfinite(loss[~hit]).all()) and not bool(loss[~weighted].any())
+        assert bool((lse == -inf).all() if b is not some else torch.isfinite(lse).all())
+        assert all(bool(torch.isfinite(g).all()) for g in ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,width,classes", [(9, 128, 300), (4000, 128, 2001)])
 @pytest.mark.parametrize("order", ["out_in", "in_out"])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
