@@ -8,7 +8,8 @@ hold their activations in tensors.  Nothing else of the package imports torch.
   on the same stream, so the calls order like torch's own and can be captured into a graph.
 * Activations and output kernels are float32 or bfloat16, everything else (parameters of a normalisation, biases, statistics, losses) is
   float32.  Sums are float32; a bfloat16 result is rounded once.
-* The operators stand outside autograd: they return plain tensors, and the *_grad functions are the backward pass.
+* The operators stand outside autograd: they return plain tensors, and the *_grad functions are the backward pass (inside a
+  torch.autograd.Function, say).  While gradients are recorded, tensors that require one are refused.
 * A tensor whose last axis is not contiguous is copied first; every other stride, and any alignment, is taken as it is.
 """
 import ctypes as C
@@ -36,13 +37,19 @@ def _check(rc):
 
 
 def _device(what, x, *others):
-    """Index of the one GPU all the tensors live on."""
+    """Index of the one GPU all the tensors live on.  What autograd would record is refused: the results could not carry it on."""
+    dev, lost = x.device, x.requires_grad
+    for t in others:
+        if t is not None:
+            if t.device != dev:
+                raise ValueError("%s: tensors on %s and %s" % (what, dev, t.device))
+            if t.requires_grad:
+                lost = True
+    if lost and torch.is_grad_enabled():
+        raise ValueError("%s: a tensor requires a gradient, which autograd would lose here: call it under torch.no_grad() or on detached tensors, with the "
+                         "*_grad function as the backward pass" % what)
     if not x.is_cuda:
         raise ValueError("%s: tensors must live on a GPU (got %s)" % (what, x.device))
-    dev = x.device
-    for t in others:
-        if t is not None and t.device != dev:
-            raise ValueError("%s: tensors on %s and %s" % (what, dev, t.device))
     return dev.index
 
 
@@ -157,7 +164,7 @@ def layer_norm_grad(dy, x, mean, rstd, gamma=None):
 _TARGETS = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.bfloat16: 3}
 
 
-def _output_loss(what, x, kernel, target, bias):
+def _output_loss(what, x, kernel, target, bias, *others):
     """The checked description of a linear output layer and its targets (struct dimn_output_loss) and the tensors it points into."""
     kind = _type(what, x)
     if kernel.dtype != x.dtype:
@@ -171,7 +178,7 @@ def _output_loss(what, x, kernel, target, bias):
     if target_kind is None or target.shape != ((rows,) if target_kind < 2 else (rows, classes)):
         raise ValueError("%s: target must be int32 / int64 labels [%d] or a float32 / bfloat16 profile [%d, %d], got %s %s"
                          % (what, rows, rows, classes, target.dtype, tuple(target.shape)))
-    dev = _device(what, x, kernel, target, bias)
+    dev = _device(what, x, kernel, target, bias, *others)
     if x.stride(1) != 1 and width > 1:
         x = x.contiguous()
     if target.stride(-1) != 1:
@@ -214,9 +221,8 @@ def linear_cross_entropy_grad(dloss, x, kernel, target, lse, bias=None):
     """The backward pass of linear_cross_entropy: (dx, dkernel, dbias) from the gradient dloss [rows] of the losses and the forward's lse.
     dx and dkernel have the types of x and kernel, dkernel lies in memory as the kernel does; dbias is float32 [classes]."""
     what = "linear_cross_entropy_grad"
-    d, (x, kernel, _target, _bias) = _output_loss(what, x, kernel, target, bias)
+    d, (x, kernel, _target, _bias) = _output_loss(what, x, kernel, target, bias, dloss, lse)
     dloss, lse = _f32(what, "dloss", dloss, (d.rows,)), _f32(what, "lse", lse, (d.rows,))
-    _device(what, x, dloss, lse)
     if d.kernel_in == 1 and d.kernel_out != 1:
         dkernel = torch.empty((d.classes, d.width), dtype=x.dtype, device=x.device).t()
     else:

@@ -709,6 +709,24 @@ def test_refusals_of_tensors():
             ops.linear_cross_entropy(x, k, bad)
 
 
+def test_tensors_that_require_a_gradient_are_refused():
+    """While gradients are recorded (a result would silently be a constant of the graph); not under no_grad (no GPU needed)."""
+    from deepimpute_amd import ops
+    x, k, t, v, b = torch.zeros((4, 8)), torch.zeros((8, 16)), torch.zeros(4, dtype=torch.int32), torch.zeros(4), torch.zeros(16)
+    g = torch.ones(8)
+    calls = [(ops.layer_norm, (x, g, g), (0, 1, 2)), (ops.layer_norm_grad, (x, x, v, v, g), (0, 1, 2, 3, 4)),
+             (ops.linear_cross_entropy, (x, k, t, b), (0, 1, 3)), (ops.linear_cross_entropy_grad, (v, x, k, t, v, b), (0, 1, 2, 4, 5))]
+    for call, args, which in calls:
+        with pytest.raises(ValueError, match="GPU"):
+            call(*args)
+        for i in which:
+            leaf = args[:i] + (args[i].clone().requires_grad_(),) + args[i + 1:]
+            with pytest.raises(ValueError, match="requires a gradient"):
+                call(*leaf)
+            with torch.no_grad(), pytest.raises(ValueError, match="GPU"):
+                call(*leaf)
+
+
 @pytest.mark.gpu
 def test_refusals_on_the_device():
     from deepimpute_amd import ops
