@@ -147,7 +147,7 @@ __device__ __forceinline__ bool res_unwritten(f32x4 x) {
 // The bulk loads that follow validate every piece again (res_fix): the canary only keeps the polling traffic small.
 __device__ __forceinline__ bool res_poll(__amdgpu_buffer_rsrc_t r, uint32_t base, int n, uint32_t stride, unsigned* abort_w) {
 #ifdef DIMN_RES_NOCANARY   // test build (tests/test_gpu_configs.py): no canary, so the bulk requests leave early and res_fix's retry path runs all the time
-    return true;
+    return __hip_atomic_load(abort_w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u;      // (an abandoned launch leaves, as with the canary)
 #endif
     const int lane = threadIdx.x & 63;
     unsigned spins = 0;
@@ -590,6 +590,13 @@ __global__ __launch_bounds__(DIMN_RES_THREADS, 2) void k_epoch_resident(ResParam
             for (int h2 = 0; h2 < 2; ++h2)
 #pragma unroll
                 for (int m = 0; m < 4; ++m) a4[h2][m] = res_ld(rT, tb + (uint32_t)(h2 * 4096 + 16 * (64 * m + 4 * li + lj)));
+#ifdef DIMN_RES_NOCANARY   // without the canary the pieces alone say that both tiles are out, and the slot re-armed below still holds dD(t-1) until then: a manager that had
+                           // not gathered it waited for it until its bound (R:2 of the parity tests timed out)
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) if (okd) res_fix(a4[h2][m], rT, tb + (uint32_t)(h2 * 4096 + 16 * (64 * m + 4 * li + lj)), abort_w);
+#endif
             // Dd(t) of managers 2 wave, 2 wave + 1 is out, so both -- and their siblings, whose P(t) they summed first -- have finished
             // gathering the dD partials of the step before: tiles (ot, 2 wave), (ot, 2 wave + 1) of that dD slot are free -- marked "not
             // written" for the step after this one; acknowledged by the drain at the end of this step's tile loop (role1), a step before
