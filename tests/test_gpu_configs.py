@@ -465,6 +465,25 @@ def test_resident_hand_off_retry_path():
     assert " passed" in res.stdout and "failed" not in res.stdout
 
 
+def test_resident_launch_that_is_refused_says_why(monkeypatch, capfd):
+    """A launch that the runtime refuses (DIMN_RES_TEST="refuse=1" pretends it) falls back like one that times out, and the message has what was asked
+    for and what the runtime answered."""
+    from helpers import make_problem, load_problem
+    monkeypatch.setenv("DIMN_RESIDENT", "1")
+    monkeypatch.setenv("DIMN_RES_TEST", "refuse=1")
+    prob = make_problem(n=500, g=900, Ds=[300, 280], H=256, O=512, seed=5, val_frac=0.1)
+    kw = dict(batch_size=64, dropout_rate=0.2, learning_rate=1e-3, seed=99)
+    a, b = load_problem(_hip(), prob, **kw), load_problem(_oracle(), prob, **kw)
+    a.init_weights(); b.init_weights()
+    a.set_profiling(True)
+    for epoch in range(2):
+        np.testing.assert_allclose(a.train_epoch(epoch), b.train_epoch(epoch), rtol=1e-4)
+    assert a.get_timers()[7] == 0
+    err = capfd.readouterr().err
+    assert err.count("cannot have all its workgroups resident") == 1 and "CUs, 1 per CU; " in err and "ooperative" in err, err
+    a.close(); b.close()
+
+
 @pytest.mark.parametrize("K,precision,want", [
     (5, "fp32", dict(path="resident", resident_groups=1, resident_splits=3)),        # one rank of the 8-GPU job
     (10, "fp32", dict(path="resident", resident_groups=2)),                          # 4-GPU share: two groups of 5
