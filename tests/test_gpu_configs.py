@@ -484,6 +484,28 @@ def test_resident_launch_that_is_refused_says_why(monkeypatch, capfd):
     a.close(); b.close()
 
 
+def test_resident_launch_without_a_cooperative_queue(monkeypatch, capfd):
+    """Where the runtime has no queue for cooperative launches (DIMN_RES_TEST="refuse=2" pretends its answer), the resident kernel is launched the
+    ordinary way: same numbers, no fall back."""
+    from helpers import make_problem, load_problem
+    monkeypatch.setenv("DIMN_RESIDENT", "1")
+    prob = make_problem(n=500, g=900, Ds=[300, 280], H=256, O=512, seed=5, val_frac=0.1)
+    kw = dict(batch_size=64, dropout_rate=0.2, learning_rate=1e-3, seed=99)
+    got = []
+    for knob in ("", "refuse=2"):
+        monkeypatch.setenv("DIMN_RES_TEST", knob)
+        a = load_problem(_hip(), prob, **kw)
+        a.init_weights()
+        a.set_profiling(True)
+        losses = [a.train_epoch(epoch) for epoch in range(2)]
+        assert a.get_timers()[7] == a.step_count() > 0
+        got.append(losses + [v for k in range(a.K) for v in a.get_weights(k)])
+        a.close()
+    for u, v in zip(*got):
+        assert np.array_equal(u, v)
+    assert "libdimn:" not in capfd.readouterr().err
+
+
 @pytest.mark.parametrize("K,precision,want", [
     (5, "fp32", dict(path="resident", resident_groups=1, resident_splits=3)),        # one rank of the 8-GPU job
     (10, "fp32", dict(path="resident", resident_groups=2)),                          # 4-GPU share: two groups of 5
