@@ -79,6 +79,19 @@ def test_kernel_resource_invariants():
     assert any(n.startswith("void k_predict_bf16<true, false>") for n in names) and any("k_w1_update_fwd_ring<16, 1, 3, 1, float>" in n for n in names)
 
 
+def test_kernel_resources_of_every_translation_unit():
+    """tools/kernel_resources.py reads all code objects of the library, so its invariants cover the row operators' kernels too."""
+    import sys
+    sys.path.insert(0, os.path.join(ROOT, "tools"))
+    import kernel_resources
+    table, problems = kernel_resources.check(_lib.LIB_PATH)
+    assert not problems, problems
+    names = [r["demangled"] for r in table.values()]
+    for part in ("k_predict_bf16<", "k_epoch_resident<", "rowops::k_norm<", "rowops::k_norm_grad<", "rowops::k_xent_gemm<", "rowops::k_xent_thin<", "rowops::k_xent_lay<"):
+        assert any(part in n for n in names), part
+    assert len({r["co"] for r in table.values()}) == 2
+
+
 def test_constructing_a_multinet_has_no_side_effects():
     """The reference's constructor only stores its arguments (multinet.py:67-103); ours must not start threads or touch the GPU
     (a warm-up thread started in __init__ ran for load-only use and before a fork)."""

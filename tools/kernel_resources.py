@@ -1,13 +1,14 @@
 """Register / scratch / LDS use of every gfx950 kernel in a built libdimn.so, from the code object's own metadata, plus -- for the kernels whose
-inner loops rely on hand-counted `s_waitcnt vmcnt(N)` (k_predict_bf16) -- the invariants that make those counts right:
-no scratch, and the number of vector-memory requests between two waits of the loop.
+inner loops rely on hand-counted `s_waitcnt vmcnt(N)` (k_predict_bf16) -- the invariants that make those counts right: no scratch, and the number
+of vector-memory requests between two waits of the loop -- and no scratch in any kernel of the row operators.
 
     python tools/kernel_resources.py [path/to/libdimn.so] [name-substring ...]
 
-Runs on the build host (no GPU): objcopy + clang-offload-bundler + llvm-readelf / llvm-objdump from /opt/rocm/lib/llvm/bin.
+Runs on the build host (no GPU): objcopy, and llvm-readelf / llvm-objdump from /opt/rocm/lib/llvm/bin.
 tests/test_abi.py::test_kernel_resource_invariants calls check() on the shipped library."""
 import os
 import re
+import struct
 import subprocess
 import sys
 import tempfile
@@ -16,13 +17,27 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LLVM = "/opt/rocm/lib/llvm/bin"
 
 
-def code_object(lib, workdir):
+def code_objects(lib, workdir):
+    """The gfx950 code objects of a library, one per translation unit, as files."""
     fat = os.path.join(workdir, "fat.bin")
-    co = os.path.join(workdir, "gfx950.co")
     subprocess.check_call(["objcopy", "-O", "binary", "--only-section=.hip_fatbin", lib, fat])
-    subprocess.check_call([os.path.join(LLVM, "clang-offload-bundler"), "--unbundle", "--type=o", "--targets=hipv4-amdgcn-amd-amdhsa--gfx950",
-                           "--input=" + fat, "--output=" + co])
-    return co
+    with open(fat, "rb") as f:
+        data = f.read()
+    # clang's offload bundles, one behind the other: magic, number of entries, then (offset, size, length of the name, name) each
+    magic, files, at = b"__CLANG_OFFLOAD_BUNDLE__", [], 0
+    while (at := data.find(magic, at)) >= 0:
+        count, = struct.unpack_from("<Q", data, at + len(magic))
+        pos = at + len(magic) + 8
+        for _ in range(count):
+            offset, size, n = struct.unpack_from("<QQQ", data, pos)
+            name = data[pos + 24:pos + 24 + n].decode()
+            pos += 24 + n
+            if name.startswith("hip") and name.endswith("gfx950") and size:
+                files.append(os.path.join(workdir, "gfx950_%d.co" % len(files)))
+                with open(files[-1], "wb") as f:
+                    f.write(data[at + offset:at + offset + size])
+        at = pos
+    return files
 
 
 def kernel_table(co):
@@ -53,8 +68,10 @@ def check(lib=None):
     lib = lib or os.path.join(ROOT, "deepimpute_amd", "csrc", "libdimn.so")
     problems = []
     with tempfile.TemporaryDirectory() as wd:
-        co = code_object(lib, wd)
-        tab = kernel_table(co)
+        tab = {}
+        for co in code_objects(lib, wd):
+            for sym, rec in kernel_table(co).items():
+                tab[sym] = dict(rec, co=co)
         nice = demangle(list(tab))
         for sym, rec in tab.items():
             rec["demangled"] = nice.get(sym, sym)
@@ -72,7 +89,7 @@ def check(lib=None):
             # (3) k_predict_bf16: between two hand-counted waits of the first layer's loop (`s_waitcnt vmcnt(8)` / `vmcnt(16)`) the wave must have
             #     issued exactly the requests the count assumes, and no scratch access may sit among them (it would share the counter)
             if name.startswith("void k_predict_bf16<"):
-                ins = disassemble(co, sym)
+                ins = disassemble(rec["co"], sym)
                 waits = [i for i, l in enumerate(ins) if re.match(r"s_waitcnt vmcnt\((8|16)\)", l)]
                 for a, b in zip(waits, waits[1:]):
                     seg = ins[a:b]
@@ -83,6 +100,9 @@ def check(lib=None):
                 rec["counted_waits"] = len(waits)
                 if not waits:
                     problems.append("%s: no hand-counted vmcnt(8) / vmcnt(16) wait found -- was the loop rewritten? update tools/kernel_resources.py" % name)
+            # (4) the row operators keep rows, tiles and accumulators in registers: a spill would send them to the memory that bounds these kernels
+            if "rowops::" in name and (rec.get("private_segment_fixed_size", 0) or rec.get("vgpr_spill_count", 0)):
+                problems.append("%s: %d B of scratch, %d spilled VGPRs" % (name, rec.get("private_segment_fixed_size", 0), rec.get("vgpr_spill_count", 0)))
     return tab, problems
 
 
