@@ -106,8 +106,11 @@ void norm_launch(const NormForm& f, dim3 grid, hipStream_t st, const NormP& p) {
 #define FORM(TPR, E) case TPR * 16 + E: norm_launch_one<T, GRAD, TPR, E, V>(grid, st, p); return
         FORM(16, 1); FORM(16, 2);
         FORM(64, 1); FORM(64, 2); FORM(64, 3);
-        FORM(256, 1); FORM(256, 2); FORM(256, 3);
-        FORM(1024, 1); FORM(1024, 2);
+        FORM(256, 2); FORM(256, 3);
+        FORM(1024, 2);
+    }
+    if constexpr (bf && GRAD) {                                  // (the other forms hold more pieces on a quarter of the threads)
+        switch (f.tpr * 16 + f.e) { FORM(256, 1); FORM(1024, 1); }
     }
     if constexpr (!bf || !GRAD) {
         switch (f.tpr * 16 + f.e) { FORM(64, 4); FORM(64, 5); FORM(256, 4); FORM(256, 5); }

@@ -315,6 +315,31 @@ def test_streams_graphs_and_repeats():
             assert torch.equal(a, b)
 
 
+def test_every_form_is_some_width(monkeypatch):
+    """The library has the forms (threads per row, pieces per thread) that some width takes, and no others (no GPU needed)."""
+    import os
+    import re
+    monkeypatch.syspath_prepend(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools"))
+    import kernel_resources
+    table, _ = kernel_resources.check(_lib.LIB_PATH)
+    built = {(g, t, int(a), int(e), int(v)) for r in table.values()
+             for g, t, a, e, v in re.findall(r"void rowops::k_norm(_grad)?<(float|unsigned short), (\d+), (\d+), (\d+)>", r["demangled"])}
+
+    def form(bf, grad, width):
+        v = 8 if bf else 4
+        if width < v:
+            return 16, 1, 1
+        pieces = -(-width // v)
+        most, most1k = (3 if grad else 5, 2) if bf else (6, 4)
+        for threads, limit in ((16, 32), (64, 64 * most), (256, 256 * most), (1024, 1024 * most1k)):
+            if pieces <= limit:
+                return threads, -(-pieces // threads), v
+        return None                                                  # longer rows: the kernels that read a row more than once
+    wanted = {("_grad" if grad else "", "unsigned short" if bf else "float") + form(bf, grad, width)
+              for bf in (0, 1) for grad in (0, 1) for width in range(1, 20000) if form(bf, grad, width)}
+    assert built == wanted, (built - wanted, wanted - built)
+
+
 def test_refusals_on_the_host():
     """What a call must not do is refused before anything reaches a GPU (no GPU needed): wrong sizes, types, null arrays."""
     fns = _lib.load()
