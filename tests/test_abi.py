@@ -92,6 +92,22 @@ def test_kernel_resources_of_every_translation_unit():
     assert len({r["co"] for r in table.values()}) == 2
 
 
+@pytest.mark.parametrize("tool", ["res_timeline.py", "res_trace.py", "predict_timeline.py"])
+def test_instrumented_builds_have_every_translation_unit(tool):
+    """The tools that build the library with marks in it do so by the Makefile's rule, which compiles as the library is compiled and links what it
+    consists of (compiling dimn.hip alone leaves the row operators' symbols undefined)."""
+    import subprocess
+    csrc = os.path.join(ROOT, "deepimpute_amd", "csrc")
+    with open(os.path.join(ROOT, "tools", tool)) as f:
+        text = f.read()
+    assert "hipcc\"" not in text and '"variant"' in text
+    plan = subprocess.run(["make", "-n", "-C", csrc, "variant", "OUT=libdimn_x.so", "DEFS=-DDIMN_MARK"], capture_output=True, text=True)
+    assert plan.returncode == 0, plan.stderr
+    compiles = [l for l in plan.stdout.splitlines() if "-DDIMN_MARK" in l]
+    links = [l for l in plan.stdout.splitlines() if "-o libdimn_x.so" in l]
+    assert len(compiles) == 1 and "-packed-fp32-ops" in compiles[0] and len(links) == 1 and "libdimn_x.o" in links[0] and "dimn_rowops.o" in links[0]
+
+
 def test_constructing_a_multinet_has_no_side_effects():
     """The reference's constructor only stores its arguments (multinet.py:67-103); ours must not start threads or touch the GPU
     (a warm-up thread started in __init__ ran for load-only use and before a fork)."""

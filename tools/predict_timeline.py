@@ -12,8 +12,7 @@ import numpy as np
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 lib = os.path.join(ROOT, "deepimpute_amd", "csrc", "libdimn_ptl.so")
-subprocess.check_call(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "-shared", "--offload-arch=gfx950", "-DDIMN_PRED_TL"] + sys.argv[1:] +
-                      ["-o", lib, os.path.join(ROOT, "deepimpute_amd", "csrc", "dimn.hip"), "-ldl", "-lpthread"])
+subprocess.check_call(["make", "-C", os.path.dirname(lib), "variant", "OUT=" + os.path.basename(lib), "DEFS=" + " ".join(["-DDIMN_PRED_TL"] + sys.argv[1:])])
 os.environ["DIMN_LIB_PATH"] = lib
 import time
 

@@ -14,8 +14,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 sys.path.insert(0, ROOT)
 K = int(sys.argv[1]) if len(sys.argv) > 1 else 5
 lib = os.path.join(ROOT, "deepimpute_amd", "csrc", "libdimn_tl.so")
-subprocess.check_call(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "-shared", "--offload-arch=gfx950", "-DDIMN_RES_TL"] + sys.argv[2:] +
-                      ["-o", lib, os.path.join(ROOT, "deepimpute_amd", "csrc", "dimn.hip"), "-ldl"])
+subprocess.check_call(["make", "-C", os.path.dirname(lib), "variant", "OUT=" + os.path.basename(lib), "DEFS=" + " ".join(["-DDIMN_RES_TL"] + sys.argv[2:])])
 os.environ["DIMN_LIB_PATH"] = lib
 import bench
 from deepimpute_amd import _lib

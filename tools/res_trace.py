@@ -16,8 +16,7 @@ sys.path.insert(0, ROOT)
 K = int(sys.argv[1]) if len(sys.argv) > 1 else 5
 lib = os.path.join(ROOT, "deepimpute_amd", "csrc", "libdimn_tl2.so")
 if not os.environ.get("RES_TRACE_NO_BUILD"):
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "-shared", "--offload-arch=gfx950", "-march=x86-64-v3", "-DDIMN_RES_TL2"] + sys.argv[2:] +
-                          ["-o", lib, os.path.join(ROOT, "deepimpute_amd", "csrc", "dimn.hip"), "-ldl", "-lpthread"])
+    subprocess.check_call(["make", "-C", os.path.dirname(lib), "variant", "OUT=" + os.path.basename(lib), "DEFS=" + " ".join(["-DDIMN_RES_TL2"] + sys.argv[2:])])
 os.environ["DIMN_LIB_PATH"] = lib
 import bench
 from deepimpute_amd import _lib
