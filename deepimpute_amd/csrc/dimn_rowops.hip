@@ -299,6 +299,9 @@ struct XentPlan {
     // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles).  Backward: a least-squares fit to 98
     // shapes of 40 .. 800 rows; the form it takes costs 0.4 % more than the better one on average, 26 % at worst.
     bool prefers_thin() const {
+#ifdef DIMN_XENT_FORM      // (tools/xent_forms.py times either form at every shape)
+        return DIMN_XENT_FORM;
+#endif
         const double hv = (double)H * (double)V, work = hv * (double)N, steps = (f32 ? 2.0 : 0.5) * (double)(Hp / 64);
         double t, g;
         if (!grad) {
@@ -514,7 +517,9 @@ rowops::LiveRows xent_live(const XentPlan& q, char* ws, const float* dloss, hipS
     const unsigned threads = q.N < 1 << 20 ? 1024 : 256;        // (a launch has fewer than 2^32 of them; so many rows fill the device anyhow)
     float* weight = (float*)(ws + q.weight);
     if (!q.labels) hipLaunchKernelGGL(rowops::k_xent_tsum, dim3((unsigned)q.N), dim3(threads), 0, st, d->target, d->target_kind, d->target_row, q.V, dloss, (float*)(ws + q.tsum), weight);
-    return {q.labels ? dloss : weight, d->target, d->target_kind, q.V};
+    if (!q.labels) return {weight, (const char*)weight, 4, 0, 0, UINT32_MAX};
+    if (d->target_kind == DIMN_TARGET_I64) return {dloss, (const char*)d->target, 8, 4, UINT32_MAX, (uint32_t)(q.V - 1)};
+    return {dloss, (const char*)d->target, 4, 0, 0, (uint32_t)(q.V - 1)};
 }
 rowops::SplitSum split_sum(const float* acc, int splits, int64_t rows, int64_t cols, void* out, int64_t ld) {
     const int32_t per = rows * cols >= 1 << 20 ? 4 : 1;          // (4096 x 2048 bfloat16, two splits: 32 us one by one, 21 by four)

@@ -21,6 +21,8 @@
 // 4096 x 2048 x 64000 backward 3.0 ms: logits again 1.17, dx 0.99, dW 0.98 (1.1 PFLOP/s), layouts 0.11.  float32 1024 x 1024 x 20000: 264 us forward,
 // 159 TFLOP/s (the float32 matrix instructions reach 154 in a product without a softmax behind it).
 #pragma once
+#include <type_traits>
+
 #include "dimn_rowops.h"
 
 namespace rowops {
@@ -57,14 +59,16 @@ __device__ __forceinline__ void split3(float x, uint16_t (&b)[3]) {
 // The rows of a batch that have a gradient: those whose label is a class (profiles: dloss is 0 where all weights are) and whose dloss is not 0.  The
 // G of the others is 0, but x may hold anything there, NaN too (padding), and 0 x NaN would reach dW: x^T G takes their x as zeros.
 enum { XT_I32 = 0, XT_I64 = 1, XT_F32 = 2, XT_BF16 = 3 };        // DIMN_TARGET_*
+// look() only loads, without a branch or a use of what it loads, so that other loads can follow before has() waits.
 struct LiveRows {
-    const float* dloss; const void* target; int32_t kind; int64_t classes;
-    __device__ __forceinline__ bool operator()(int64_t row) const {
-        int64_t y = 0;
-        if (kind == XT_I64) y = ((const int64_t*)target)[row];
-        else if (kind == XT_I32) y = ((const int32_t*)target)[row];
-        return dloss[row] != 0.f && y >= 0 && y < classes;
+    const float* dloss;
+    const char* label; uint32_t step, high_at, high;      // the labels' words: bytes between them, to the upper one, and its mask; profiles: dloss again
+    uint32_t last;                                         // the last class; profiles: every word passes
+    struct Row { uint32_t low, high; float dloss; };
+    __device__ __forceinline__ Row look(uint32_t row) const {                 // (rows: up to 2^22, so the offsets take 32 bits)
+        return {*(const uint32_t*)(label + row * step), *(const uint32_t*)(label + high_at + row * step), *(const float*)((const char*)dloss + row * 4)};
     }
+    __device__ __forceinline__ bool has(const Row& r) const { return (r.dloss != 0.f) & (r.low <= last) & ((r.high & high) == 0); }
 };
 
 // ---- operand layout -----------------------------------------------------------------------------------------------------------
@@ -131,7 +135,8 @@ __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
         const int64_t k = k0 + s + 32 * i, r = r0 + 8 * q;
         const T* f = from + k * p.ld + r;
         T v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        const bool live = k < p.cols && (!p.live || all.rows(k));
+        LiveRows::Row row = {0, 0, 1.f};
+        if (p.live) row = all.rows.look((uint32_t)(k < p.cols ? k : p.cols - 1));
         if (k < p.cols) {
             if (r + 8 <= p.rows) {
                 const typename Eight<T>::vec x = *(const typename Eight<T>::vec*)f;
@@ -141,6 +146,7 @@ __global__ __launch_bounds__(256) void k_xent_lay(const LayJobs all) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) if (r + j < p.rows) v[j] = f[j];
         }
+        const bool live = !p.live || all.rows.has(row);
 #pragma unroll
         for (int j = 0; j < 8; ++j) tile[s + 32 * i][8 * q + j] = live ? v[j] : (T)0;
     }
@@ -520,6 +526,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                 }
             typedef uint16_t rowvec __attribute__((ext_vector_type(4 * FN)));
             typedef uint16_t colvec __attribute__((ext_vector_type(FM)));
+            auto store = [&](auto edges) {
 #pragma unroll
             for (int pl = 0; pl < PL; ++pl) {
                 uint16_t o[FM][4 * FN];
@@ -530,7 +537,11 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             float rest = acc[i][j][r];
-                            o[i][4 * j + r] = split_term(rest, pl + 1 == PL);
+                            if constexpr (decltype(edges)::value) o[i][4 * j + r] = split_term(rest, pl + 1 == PL);
+                            else {
+                                o[i][4 * j + r] = to_bf16(rest);
+                                rest -= from_bf16(o[i][4 * j + r]);
+                            }
                             acc[i][j][r] = rest;
                         }
                 uint16_t* G = p.G + pl * p.g_plane;
@@ -556,6 +567,18 @@ __global__ __launch_bounds__(64 * WM * WN) void k_xent_gemm(const XentGemm p) {
                     }
                 }
             }
+            };
+            // (split_term's care for values at float32's end and infinities costs 5 % of a product with 800 rows: only where a wave has one)
+            float most = 0.f;
+            if constexpr (PL == 3)
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) most = fmaxf(most, fabsf(acc[i][j][r]));
+            if (PL == 3 && __builtin_amdgcn_ballot_w64(most > 3.38953139e38f) != 0) store(std::true_type{});
+            else store(std::false_type{});
         }
     }
 }

@@ -474,13 +474,15 @@ struct ThinDw {
     LiveRows live;
 };
 // Sixteen rows at a time, no more of them in flight: the registers of a second sixteen cost more workgroups than they hide latency (80 x 1344 x 28165
-// float32: 91 against 106 us; 12 rows 33 us = 4.6 TB/s), and a copy of the loads without the test for the last row changes nothing.
+// float32: 91 against 106 us; 12 rows 33 us = 4.6 TB/s).  Four waves per SIMD: 118 / 122 registers, since whole sixteens are read without a test for the
+// last row and the sums stay out of the accumulation registers (150 x 2048 x 8000 float32: 65.6 us; 69.8 with three waves).
 template <typename T>
 __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
     const T *P = (const T*)p.P, *Q = (const T*)p.Q;
     T* C = (T*)p.C;
     const int64_t ldp = p.ldp, ldq = p.ldq, na = p.na, nb = p.nb, ldc = p.ldc;
-    const int64_t chunks = (p.n + 15) >> 4, beg = chunks * range / p.ranges * 16, end = chunks * (range + 1) / p.ranges * 16, n = end < p.n ? end : p.n;
+    const int64_t chunks = (p.n + 15) >> 4, end = chunks * (range + 1) / p.ranges * 16;
+    const int beg = (int)(chunks * range / p.ranges * 16), n = (int)(end < p.n ? end : p.n);      // (rows: up to 2^22)
     constexpr bool BF = sizeof(T) == 2;
     typedef typename Four<T>::vec vec;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lj = lane >> 4;
@@ -495,18 +497,23 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
         for (int j = 0; j < 4; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
     const vec zero = {0, 0, 0, 0};
     vec a[4], b[4];
-    auto fetch = [&](int64_t k) {
+    // this lane's rows of the sixteen from k: 4 lj + r (bfloat16: four consecutive rows make one lane's operand), 4 r + lj (float32)
+    const int first = BF ? 4 * lj : lj, apart = BF ? 1 : 4;
+    const T *pa = P + (beg + first) * ldp + ca, *pb = Q + (beg + first) * ldq + cb;
+    auto fetch = [&](int k, auto whole) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int64_t row = BF ? k + 4 * lj + r : k + 4 * r + lj;       // bfloat16: four consecutive rows make one lane's operand
-            a[r] = row < n ? *(const vec*)(P + row * ldp + ca) : zero;
-            b[r] = row < n ? *(const vec*)(Q + row * ldq + cb) : zero;
+            const bool have = decltype(whole)::value || k + first + r * apart < n;
+            a[r] = have ? *(const vec*)(pa + r * apart * ldp) : zero;
+            b[r] = have ? *(const vec*)(pb + r * apart * ldq) : zero;
         }
+        pa += 16 * ldp;
+        pb += 16 * ldq;
     };
     auto without = [&](uint32_t dead) {                             // bit i: the fetch's row i has no gradient
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (dead >> (BF ? 4 * lj + r : 4 * r + lj) & 1) { a[r] = zero; b[r] = zero; }
+            if (dead >> (first + r * apart) & 1) { a[r] = zero; b[r] = zero; }
     };
     auto consume = [&] {
         if constexpr (BF) {
@@ -528,19 +535,17 @@ __device__ __forceinline__ void thin_dw(const ThinDw& p, int tile, int range) {
                     for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r][i], b[r][j], acc[i][j], 0, 0, 0);
         }
     };
-    for (int64_t k0 = beg; k0 < n; k0 += 64) {
-        const bool off = k0 + lane < n && !p.live(k0 + lane);       // 64 rows at once, requested in front of the first sixteen
-        fetch(k0);
-        uint64_t dead = __builtin_amdgcn_ballot_w64(off);
-        for (int64_t k = k0;;) {
-            if ((uint32_t)dead & 0xffff) without((uint32_t)dead);
-            consume();
-            dead >>= 16;
-            k += 16;
-            if (k >= n || k == k0 + 64) break;
-            fetch(k);
-        }
-    }
+    // (the sixteen rows are looked up in every quarter of the wave, requested in front of their operands and awaited behind)
+    auto rows = [&](int k, auto whole) {
+        const LiveRows::Row row = p.live.look((uint32_t)(whole || k + li < n ? k + li : n - 1));
+        fetch(k, whole);
+        const uint32_t dead = ~(uint32_t)__builtin_amdgcn_ballot_w64(p.live.has(row)) & 0xffff;
+        if (dead) without(dead);
+        consume();
+    };
+    int k = beg;
+    for (; k + 16 <= n; k += 16) rows(k, std::true_type{});
+    if (k < n) rows(k, std::false_type{});
     // acc[i][j][r]: a = set i of lane 4 lj + r, b = set j of lane li
     const bool whole = cb == b0 + 4 * li;
 #pragma unroll
@@ -587,7 +592,7 @@ __global__ __launch_bounds__(64 * NW) void k_xent_thin(const Thin p, int tiles, 
     thin_product<T, VC, NF, EPI, NW, FOURS>(p, unit % tiles, unit / tiles, ranges, block);
 }
 template <typename T>
-__global__ __launch_bounds__(256) void k_xent_thin_dw(const ThinDw w) {
+__global__ __launch_bounds__(256, 4) void k_xent_thin_dw(const ThinDw w) {
     thin_dw<T>(w, blockIdx.x % w.tiles, blockIdx.x / w.tiles);
 }
 
