@@ -203,9 +203,8 @@ __device__ __forceinline__ float softplus_out(float x) {
     return x > thr ? x : r;
 }
 
-// The same function on two elements at a time: every multiply / add / fma becomes ONE packed instruction (v_pk_mul_f32, v_pk_add_f32,
-// v_pk_fma_f32: IEEE results, element for element those of softplus_out), only the three transcendentals and the selects stay per element --
-// 18 instead of 27 instructions per element in k_predict_bf16's output epilogue.
+// The same function on two elements, step by step side by side: results element for element those of softplus_out, two independent chains for the
+// scheduler.  (The library is compiled without packed fp32 instructions -- see the Makefile --, so a step is two instructions.)
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ f32x2 softplus_out2(f32x2 x) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -296,8 +296,9 @@ struct XentPlan {
         return best;
     }
     // Which form is faster: estimates in microseconds from both forms' measured times over 16 .. 2048 rows, widths of 64 .. 4096 and 300 .. 50000
-    // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles).  Backward: a least-squares fit to 98
-    // shapes of 40 .. 800 rows; the form it takes costs 0.4 % more than the better one on average, 26 % at worst.
+    // classes (launches, laying out operands, a product's rate, the latency of a step where there are few tiles); backward, a least-squares fit.  Over 98
+    // shapes of 40 .. 800 rows each (profiles/xent_forms.txt) the form taken costs 1.1 / 0.7 % more than the better one forward (float32 / bfloat16; 31 %
+    // at worst) and 1.7 / 2.1 % backward (46 %), on average; a fit to those shapes alone comes to 0.5 / 1.5 and 1.1 / 0.9 % (tools/xent_forms.py).
     bool prefers_thin() const {
 #ifdef DIMN_XENT_FORM      // (tools/xent_forms.py times either form at every shape)
         return DIMN_XENT_FORM;
