@@ -14,8 +14,8 @@
 //   * Backward: a thread owns its columns for all rows it handles, so dgamma / dbeta are sums in its registers; a workgroup writes one
 //     partial row, k_norm_param_grad adds the partial rows in a fixed order.  No atomics: the same call gives the same bits.
 // All arithmetic is float32; a bfloat16 result is rounded once, to nearest even.
-// Measured: 50k x 2400 bfloat16 forward 93 us = 5.1 TB/s, float32 backward 270 + 6 us = 5.3 TB/s (a large copy: 5.3); 40 groups of 64 x 256 float32
-// 3.8 us forward, 5.8 + 2.6 backward, where the launch is most of it.
+// Measured: 50k x 2400 bfloat16 forward 94 us = 5.1 TB/s, float32 backward 271 + 6 us = 5.2 TB/s (a large copy: 5.3); 40 groups of 64 x 256 float32
+// 3.8 us forward, 5.5 + 2.5 backward, where the launch is most of it.
 #pragma once
 #include "dimn_rowops.h"
 

@@ -17,9 +17,9 @@
 //   * Operands that are k-contiguous, aligned and a multiple of 64 long are read in place; everything else is laid out by k_xent_lay.
 //   * Of bfloat16 operands G is rounded to bfloat16 too (half a step, 2^-8 of it): it is the operand of two more products, and three planes of it would
 //     cost three passes each where x and the kernel hold eight bits themselves.  float32 G keeps its three planes.
-// Measured, bfloat16: 4096 x 2048 x 100000 forward 1.39-1.55 ms (1.08-1.2 PFLOP/s; the library's product of the same sizes alone: 1.2);
-// 4096 x 2048 x 64000 backward 3.0 ms: logits again 1.17, dx 0.99, dW 0.98 (1.1 PFLOP/s), layouts 0.11.  float32 1024 x 1024 x 20000: 264 us forward,
-// 159 TFLOP/s (the float32 matrix instructions reach 154 in a product without a softmax behind it).
+// Measured, bfloat16: 4096 x 2048 x 100000 forward 1.38-1.45 ms (1.16-1.2 PFLOP/s; the library's product of the same sizes alone: 1.2);
+// 4096 x 2048 x 64000 backward 3.0 ms: logits again 1.10, dx 0.90, dW 0.88 (1.0-1.2 PFLOP/s), layouts 0.11.  float32 1024 x 1024 x 20000: 264 us forward
+// (layouts 35, product 224), 159 TFLOP/s (the float32 matrix instructions reach 154 in a product without a softmax behind it); backward 925 us.
 #pragma once
 #include <type_traits>
 
@@ -73,7 +73,7 @@ struct LiveRows {
 
 // ---- operand layout -----------------------------------------------------------------------------------------------------------
 // to[plane][r][k] = bfloat16 term `plane` of from[r][k], zero for cols <= k < ldk (ldk: a multiple of 64).  T = float: three planes, T = bf16_t: one.
-// Copying bounds both; everything moves in 16-byte pieces (64000 x 2048 bfloat16 transposed: 524 MB in 113 us, 4.7 TB/s).
+// Copying bounds both; everything moves in 16-byte pieces (64000 x 2048 and 4096 x 2048 bfloat16 transposed: 558 MB in 113 us, 4.9 TB/s).
 template <typename T> struct Eight { typedef uint16_t vec __attribute__((ext_vector_type(8), aligned(2))); };
 template <> struct Eight<float> { typedef float vec __attribute__((ext_vector_type(8), aligned(4))); };
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
@@ -590,7 +590,7 @@ __device__ __forceinline__ float2 join_lse(float2 a, float2 b) {
     return make_float2(top, a.y * (a.x == -INFINITY ? 1.f : __expf(a.x - top)) + b.y * (b.x == -INFINITY ? 1.f : __expf(b.x - top)));
 }
 
-// loss and lse of every row from the partial sums of the class tiles (4096 rows of 391 tiles: 15 us; one row of 1000: 4.4 us): 1024 threads, `per` rows (a power of two up to 64) x 1024 / per strands of tiles
+// loss and lse of every row from the partial sums of the class tiles (4096 rows of 391 tiles: 15 us; one row of 1000: 4.1 us): 1024 threads, `per` rows (a power of two up to 64) x 1024 / per strands of tiles
 // One call per piece of the classes: what the pieces so far come to waits in `carry`, the last one gives the results.
 struct XentRows {
     float4* carry; int32_t first, last;        // [rows] (maximum, sum, sum of t, sum of t z)

@@ -8,9 +8,9 @@
 //   * class-contiguous (VC): a lane loads four consecutive classes of one k; element j belongs to class set j, whose sixteen classes lie four
 //     apart -- a permutation of the classes inside the workgroup's 64 that the epilogue undoes.
 // float32 runs on the exact float32 matrix instructions: at 64 rows their rate (154 TFLOP/s measured) and the HBM's meet.
-// Measured: one row x 1024 x 32000 bfloat16 14.4 us = 4.6 TB/s; 12 x 2000 x 40000 bfloat16 dx 27 us = 5.8 TB/s (part of the kernel still lies in the
-// memory-side cache); 12 x 3648 x 22455 float32 dx 67, dW 59 us = 4.9, 5.5 TB/s, class-contiguous logits 115 us = 2.9 TB/s; 128 x 2922 x 25664 float32
-// 241 / 296 / 234 us (logits / dx / dW), 80 / 65 / 82 TFLOP/s.
+// Measured: one row x 1024 x 32000 bfloat16 14.1 us = 4.6 TB/s; 12 x 2000 x 40000 bfloat16 dx 28 us = 5.7 TB/s (part of the kernel still lies in the
+// memory-side cache); 12 x 3648 x 22455 float32 dx 69, dW 62 us = 4.7, 5.3 TB/s, class-contiguous logits (backward) 129 us = 2.5 TB/s; 128 x 2922 x 25664
+// float32 218 / 266 / 229 us (logits / dx / dW), 88 / 72 / 84 TFLOP/s.
 // A workgroup owns 32 (KC) / 64 (VC) classes x up to 64 rows; its waves (four, or sixteen where there are few workgroups and a long inner
 // dimension: 3840 x 222 float32 ran 45 us with four) share the chunks of k and are added through LDS, upper half onto lower half, in a fixed order.
 #pragma once

@@ -405,7 +405,8 @@ int dimn_col_stats_var(const double* a, int64_t n, int64_t g, int64_t ld, const 
  * kernels on the stream and returns; nothing is allocated, copied to the host or waited for, so it can be captured into a graph, and two
  * calls on different streams run side by side as long as their workspaces and outputs differ.  The calling thread's current device is
  * left as it was.  Strides count elements and may be 0 or negative; the last axis of every plane is contiguous and nothing else is assumed about alignment
- * (workspaces: 16 bytes).  Rows past `rows` are neither read nor written.  The same arguments give the same bits. */
+ * (workspaces: 16 bytes for the normalisation, 256 for the cross entropy).  Rows past `rows` are neither read nor written.  Outputs and workspaces
+ * overlap no input unless it says so below.  The same arguments give the same bits. */
 #define DIMN_TYPE_F32 0
 #define DIMN_TYPE_BF16 1
 /* Layer normalisation of [groups][rows] rows of `width` elements (keras.layers.LayerNormalization, axis -1):
@@ -457,7 +458,10 @@ int dimn_linear_cross_entropy_workspace(const dimn_output_loss* d, int32_t grad,
 /* loss, lse: float32 [rows]. */
 int dimn_linear_cross_entropy(const dimn_output_loss* d, void* stream, float* loss, float* lse, void* workspace, int64_t workspace_bytes);
 /* The backward pass from the forward's lse and the gradient dloss [rows] of the losses: dx [rows][width], dkernel [width][classes] (strides
- * as the kernel's, one of them 1), both of element type `type`, and dbias float32 [classes] (NULL: not wanted).  rows = 0 is refused here. */
+ * as the kernel's, one of them 1), both of element type `type`, and dbias float32 [classes] (NULL: not wanted).
+ * Sums are float32.  Of bfloat16 operands the gradient of the logits is rounded to bfloat16 (half a step, 2^-8) before dx and dkernel are summed from
+ * it, and both are rounded once more: 2.4e-3 from the float64 result in norm where a float32 gradient of the logits gives 1.7e-3.  dbias is summed from
+ * the float32 gradient.  rows = 0 is refused here. */
 int dimn_linear_cross_entropy_grad(const dimn_output_loss* d, void* stream, const float* dloss, const float* lse, void* dx, int64_t dx_row,
                                    void* dkernel, int64_t dkernel_in, int64_t dkernel_out, float* dbias, void* workspace, int64_t workspace_bytes);
 
