@@ -37,7 +37,10 @@ template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float v) { return
 
 // The columns of a thread: piece e covers V columns from first(e).  Only the last piece can cross the end of the row; it is moved back to end with
 // the row, and its first `skip` columns (all of them where the thread has no last piece) belong to other threads: they are read, since a full
-// piece is one access without a branch, but take no part in sums.  What two threads store to the same column is the same value.
+// piece is one access without a branch, but take no part in sums.  What two threads store to the same column is the same value -- bit by bit, since
+// which of them comes last is open: every operation between load and store is written out (no contraction, fmaf where one is meant), or the compiler
+// fuses those of a thread's last piece, whose sums are conditional, differently from the others' (2051 float32 columns: the bits of one of them changed
+// from call to call).
 template <int TPR, int E, int V>
 struct Columns {
     int lane, last, skip;
@@ -100,6 +103,7 @@ __device__ __forceinline__ void apply_gate(const float* gate, float (&f)[V]) {
 // grid (workgroups, groups); max(256, TPR) threads; each set of TPR threads takes rows set, set + sets, ... of its group
 template <typename T, int TPR, int E, int V>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm(const NormP p) {
+#pragma clang fp contract(off)
     typedef typename Piece<T, V>::raw raw;
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, SETS = BLOCK / TPR;
     __shared__ float2 red[32];
@@ -140,7 +144,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm(const NormP p) {
             for (int i = 0; i < V; ++i) {
                 const float d = v[e * V + i] - mu;
                 v[e * V + i] = d;
-                q += col.mine(e, i) ? d * d : 0.f;
+                q = col.mine(e, i) ? fmaf(d, d, q) : q;
             }
         none = 0.f;
         row_sum2<TPR>(q, none, red, turn);
@@ -151,7 +155,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm(const NormP p) {
         for (int e = 0; e < E; ++e) {
             float f[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = v[e * V + i] * rs * ga[e * V + i] + be[e * V + i];
+            for (int i = 0; i < V; ++i) f[i] = fmaf(v[e * V + i] * rs, ga[e * V + i], be[e * V + i]);
             apply_gate<T, V>(p.gate ? p.gate + g * p.out_group + r * p.out_row + col.first(e) : nullptr, f);
             raw o;
 #pragma unroll
@@ -165,6 +169,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm(const NormP p) {
 // 1024 threads leave 128 registers each: no next row in flight there, and gamma is read again for every row.
 template <typename T, int TPR, int E, int V>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_grad(const NormP p) {
+#pragma clang fp contract(off)
     typedef typename Piece<T, V>::raw raw;
     constexpr int BLOCK = TPR < 256 ? 256 : TPR, SETS = BLOCK / TPR;
     constexpr bool AHEAD = TPR < 1024;
@@ -207,13 +212,13 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_grad(const NormP
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int k = e * V + i;
-                const float d = to_f32(nd[e][i]), own = col.mine(e, i) ? d : 0.f;
+                const float d = to_f32(nd[e][i]);
                 xh[k] = (to_f32(nx[e][i]) - mu) * rs;
-                dg[k] += d * xh[k];                              // (columns of other threads: summed, but not handed on below)
+                dg[k] = fmaf(d, xh[k], dg[k]);                   // (columns of other threads: summed, but not handed on below)
                 db[k] += d;
                 gy[k] = d * ga[k];
-                s1 += own * ga[k];
-                s2 += own * ga[k] * xh[k];
+                s1 = col.mine(e, i) ? s1 + gy[k] : s1;
+                s2 = col.mine(e, i) ? fmaf(gy[k], xh[k], s2) : s2;
             }
         if (AHEAD && r + sets < p.rows) request(r + sets);
         row_sum2<TPR>(s1, s2, red, turn);
@@ -223,7 +228,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void k_norm_grad(const NormP
         for (int e = 0; e < E; ++e) {
             float f[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = rs * (gy[e * V + i] - s1 - xh[e * V + i] * s2);
+            for (int i = 0; i < V; ++i) f[i] = rs * fmaf(-xh[e * V + i], s2, gy[e * V + i] - s1);
             apply_gate<T, V>(p.gate ? p.gate + g * p.out_group + r * p.out_row + col.first(e) : nullptr, f);
             raw o;
 #pragma unroll

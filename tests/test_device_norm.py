@@ -220,6 +220,25 @@ def test_in_place_at_every_form(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("width", [261, 389, 1027, 1285, 1541, 2049, 2051, 3077, 4099, 6149, 6151])
+def test_the_same_bits_every_time(width, dtype):
+    """Rows whose last piece is moved back over another thread's columns, of another wave too: both write them, and the result is the same bits
+    call after call, in both directions and in place."""
+    from deepimpute_amd import ops
+    rows = 2500
+    x, dy = _make((rows, width), dtype, width), _make((rows, width), dtype, width + 1)
+    gamma, beta = _make((width,), torch.float32, 2), _make((width,), torch.float32, 3)
+    want = ops.layer_norm(x, gamma, beta)
+    grads = ops.layer_norm_grad(dy, x, want[1], want[2], gamma)
+    for _ in range(12):
+        for u, v in zip(ops.layer_norm(x, gamma, beta), want):
+            assert torch.equal(u, v)
+        for u, v in zip(ops.layer_norm_grad(dy, x, want[1], want[2], gamma), grads):
+            assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
 def test_longest_row():
     """A row of 2^26 elements, the most there may be; a thread adds 2^16 of them one after the other: 2^16 + 64 half steps of the largest term."""
     from deepimpute_amd import ops
