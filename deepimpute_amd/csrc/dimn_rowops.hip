@@ -38,6 +38,7 @@ struct OnDevice {
             known.store(n, std::memory_order_relaxed);
         }
         if (device < 0 || device >= n) return dimn_fail(DIMN_ERR_ARG, "%s: device_id %d out of range (%d devices)", who, device, n);
+        (void)hipGetLastError();                                 // (an error that an earlier call of the thread left is not the coming launches')
         HIPCHK(hipGetDevice(&before));
         now = device;
         if (before != now) HIPCHK(hipSetDevice(now));

@@ -407,6 +407,26 @@ def test_refusals_of_tensors():
 
 
 @pytest.mark.gpu
+def test_an_older_error_is_not_reported():
+    """A HIP call of the same thread that failed before (a device that is not there) says nothing about these."""
+    import ctypes
+    from deepimpute_amd import ops
+    x = _make((8, 40), torch.float32, 1)
+    y, mean, rstd = ops.layer_norm(x)
+    with open("/proc/self/maps") as f:
+        path = next(line.split()[-1] for line in f if "libamdhip64" in line)
+    hip = ctypes.CDLL(path)
+    kernel, t = _make((40, 30), torch.float32, 2), torch.zeros(8, dtype=torch.int32, device="cuda")
+    _, lse = ops.linear_cross_entropy(x, kernel, t)
+    for call in (lambda: ops.layer_norm(x), lambda: ops.layer_norm_grad(y, x, mean, rstd), lambda: ops.linear_cross_entropy(x, kernel, t),
+                 lambda: ops.linear_cross_entropy_grad(rstd, x, kernel, t, lse)):
+        want = call()
+        assert hip.hipSetDevice(4096) != 0
+        for u, v in zip(call(), want):
+            assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
 def test_refusals_on_the_device():
     fns = _lib.load()
     x = _make((4, 8), torch.float32, 1)
