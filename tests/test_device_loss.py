@@ -232,6 +232,49 @@ def test_rows_in_descending_order(dtype, rows, width, classes, order):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("target", ["labels", "profile"])
+@pytest.mark.parametrize("rows,width,classes", [(1, 40, 33), (20, 70, 90), (150, 66, 1001), (4000, 130, 2001), (300, 1000, 77), (7698, 22, 900)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_outputs_of_the_c_entries(dtype, rows, width, classes, target):
+    """Gradients into padded planes, dkernel in the kernel's order and in the other one, dbias wanted or not: the bits of the tensors' call where the
+    order is the kernel's, and nothing written behind a row, behind the last row, or behind the workspace."""
+    from deepimpute_amd import ops
+    fns = _lib.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    dt = DTYPES[dtype]
+    for order in ("out_in", "in_out"):
+        x, kernel, t, b, dloss = _problem(rows, width, classes, dt, order, target)
+        _, lse = ops.linear_cross_entropy(x, kernel, t, b)
+        want = ops.linear_cross_entropy_grad(dloss, x, kernel, t, lse, b)
+        ref = _reference(x, kernel, t, b, dloss)
+        d, keep = ops._output_loss("test", x, kernel, t, b)
+        n = C.c_int64()
+        assert fns["linear_cross_entropy_workspace"](d, 1, n) == 0
+        for dk_order in ("out_in", "in_out"):
+            for bias in (True, False):
+                dx = torch.full((rows + 1, width + 3), 7.0, dtype=dt, device="cuda")
+                flat = (classes, width) if dk_order == "out_in" else (width, classes)
+                dk = torch.full((flat[0] + 1, flat[1] + 5), 7.0, dtype=dt, device="cuda")
+                db = torch.full((classes + 1,), 7.0, device="cuda")
+                work = torch.full((n.value + 512,), 77, dtype=torch.uint8, device="cuda")
+                at = -work.data_ptr() % 256
+                ld = flat[1] + 5
+                strides = (1, ld) if dk_order == "out_in" else (ld, 1)
+                assert fns["linear_cross_entropy_grad"](d, stream, dloss.data_ptr(), lse.data_ptr(), dx.data_ptr(), width + 3, dk.data_ptr(), strides[0], strides[1],
+                                                        db.data_ptr() if bias else None, work.data_ptr() + at, n.value) == 0, fns["last_error"]()
+                assert bool((work[at + n.value:] == 77).all()) and bool((work[:at] == 77).all())
+                assert bool((dx[:, width:] == 7).all()) and bool((dx[rows:] == 7).all())
+                assert bool((dk[:, flat[1]:] == 7).all()) and bool((dk[flat[0]:] == 7).all())
+                assert bool((db[classes:] == 7).all()) and (bias or bool((db == 7).all()))
+                got = dk[:flat[0], :flat[1]]
+                got = got.t() if dk_order == "out_in" else got
+                if dk_order == order:
+                    assert torch.equal(got, want[1]) and torch.equal(dx[:rows, :width], want[0]) and (not bias or torch.equal(db[:classes], want[2]))
+                _close("dkernel", got, *ref["dkernel"])
+                _close("dx", dx[:rows, :width], *ref["dx"])
+
+
+@pytest.mark.gpu
 def test_broadcast_inputs():
     """Axes of stride 0: the same row for every sample, one profile for all of them, a kernel of equal rows or columns."""
     from deepimpute_amd import ops
