@@ -251,7 +251,7 @@ int pick_tile(bool f32, int64_t M, int64_t N, int ncu) {
     return cost(t[2]) < cost(t[best]) ? 2 : best;
 }
 
-// A piece's operands (and the G of the form for few rows) take up to 1 GiB: 4096 x 2048 x 64000 / x 100000 bfloat16 backward 3.02 / 4.66 ms (512 MiB:
+// A piece's operands take up to 1 GiB: 4096 x 2048 x 64000 / x 100000 bfloat16 backward 3.02 / 4.66 ms (512 MiB:
 // 3.09 / 4.88, 192 MiB: 3.17 / 5.02, 4 GiB: 2.93 / 4.78 -- but that keeps as much as the logits).
 constexpr int64_t kBudget = (int64_t)1 << 30;
 
@@ -343,8 +343,9 @@ struct XentPlan {
         tiles_n = ceil_div64(std::min(P, V), kTiles[f32][t_logits].bn);
         bytes = 0;
         // Few rows (and at least four of everything the class-contiguous forms take four at a time): no operand is laid out.  Its backward pass keeps G of
-        // all classes: no more of it than a piece takes (a narrow float32 layer would use this form with any number of rows, 65536 x 32 x 100000: 24 GiB).
-        thin = V >= 4 && H >= 4 && (!grad || (f32 ? 4 : 2) * N * V <= std::max(kBudget, P * per_class)) && prefers_thin();
+        // all classes: no more of it than a piece takes, or 2 GiB (a narrow float32 layer would use this form with any number of rows, 65536 x 32 x 100000:
+        // 24 GiB; up to there it is worth its memory, 8000 x 32 x 48000: 2.1 against 2.8 ms).
+        thin = V >= 4 && H >= 4 && (!grad || (f32 ? 4 : 2) * N * V <= std::max(2 * kBudget, P * per_class)) && prefers_thin();
         if (thin) {
             // 64 rows per block read the kernel least often, 32 give twice the workgroups.  float32, bound by the matrix instructions: up to 32, half the
             // registers (64 / 80 x 1344 x 28165 logits 82 / 120 us, with 64 rows 94 / 143), 16 where a third of two blocks of 32 would be no rows (48: 75, 81 us)

@@ -428,7 +428,7 @@ int dimn_layer_norm_grad(int32_t device_id, void* stream, int32_t type, int64_t 
 
 /* Softmax cross entropy of a linear output layer z = x W + b over many classes, computed in pieces of the classes: the logits are never
  * kept.  (The workspace of a call holds the operands it has to lay out, float32 sums of dx, and one piece: up to 1 GiB, 256 classes at least.  Backward,
- * that piece holds the gradient of its logits; a call of few rows whose gradient of ALL logits fits the same 1 GiB takes it whole.)  Per row, with lse = log(sum over the classes of exp(z)):
+ * that piece holds the gradient of its logits; a call of few rows or a narrow layer may keep the gradient of ALL logits, up to 2 GiB.)  Per row, with lse = log(sum over the classes of exp(z)):
  *   labels:   loss = lse - z[label].  A negative label is a row without a target: loss 0, no gradient.  A label >= classes: loss NaN, no
  *             gradient.  A label whose logit is -infinity (masked by the bias): loss +infinity.
  *   profiles: loss = sum(t) lse - sum(t z) for a row t of weights over the classes (counts, probabilities); t = 0 takes no part, a row of zeros
