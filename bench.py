@@ -20,6 +20,7 @@ No torch in this process: the GPU work goes through libdimn.so (ctypes); multi-r
 uses a file rendezvous under /tmp and RCCL itself (libdimn's dimn_comm_*).
 """
 import argparse
+import faulthandler
 import json
 import os
 import sys
@@ -601,9 +602,10 @@ def main():
     os.environ.setdefault("HSA_ENABLE_IPC_MODE_LEGACY", "0")
 
     from deepimpute_amd.engine import HipEngine
-    if world == 1:                                  # what a long-lived process does at start-up: HIP context + pinned bounce buffers, on a helper thread
+    faulthandler.enable()                           # (a crash names its thread and line on stderr)
+    if world == 1:                                  # what a long-lived process does at start-up: HIP context + pinned bounce buffers
         from deepimpute_amd import _lib
-        _lib.warm_up_async(local_rank)
+        _lib.warm_up(local_rank)
     cfg = dict(CONFIGS[args.config])
     if args.hidden:
         cfg["H"] = args.hidden

@@ -82,6 +82,14 @@ def warm_up_async(device_id=0):
     t.start()
 
 
+def warm_up(device_id=0):
+    """The same on the calling thread, once per (process, device): nothing else of the process runs beside the start of the HIP runtime."""
+    device_id = int(device_id)
+    if device_id not in _warm:
+        load()["warm_up"](device_id)
+        _warm[device_id] = True
+
+
 def release_cached_memory():
     """Give the process-wide cache of large device blocks (include/dimn.h: dimn_release_cached_memory) back to the driver: after
     MultiNet.close() / engine.close() the blocks of >= 32 MB otherwise wait, up to DIMN_ARENA_CACHE_GB (default 48), for the next
